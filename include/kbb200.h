@@ -1,11 +1,13 @@
 /*
- * kbb200.h — C ABI of the B200 (sm_100a) fp32 operator library.
+ * kbb200.h — C ABI of the B200 (sm_100a) operator library (fp32, and fp32,
+ * fp16 or bf16 for the language-model operators).
  *
  * One shared library (libkbb200.so) exports every entry point below as plain
  * `extern "C"` functions: device pointers, element counts and a CUDA stream,
  * no torch types.  Each entry replaces the compiled entry of one candidate of
  * the reference operator library (candidates/<problem>/v*.py, whose C++ entry
- * took torch::Tensor arguments and launched on the current stream).
+ * took torch::Tensor arguments and launched on the current stream), unless
+ * its comment says that it replaces none.
  *
  * Conventions (all entries):
  *   - Pointers are device pointers to contiguous fp32 data unless stated.
@@ -45,6 +47,9 @@ typedef enum kbStatus {
   KB_ERR_CUDA = 4,          /* CUDA runtime error (launch / attribute) */
   KB_ERR_DEVICE = 5         /* device is not sm_100 class */
 } kbStatus;
+
+/* Element types of the language-model entries (every other entry is fp32). */
+typedef enum kbDtype { KB_F32 = 0, KB_F16 = 1, KB_BF16 = 2 } kbDtype;
 
 /* ---- library / diagnostics ------------------------------------------- */
 KB_API int kb_version(void);                 /* MAJOR*10000 + MINOR*100 + PATCH */
@@ -355,6 +360,157 @@ KB_API int kb_gemm_splitk_partials_3xtf32(const float* A, const float* B, int64_
                                    int64_t N, int64_t K, void* workspace,
                                    size_t workspace_bytes, int* splits,
                                    kbStream stream);
+
+/* ---- language-model operators ------------------------------------------
+ * What a decoder needs beside the norms, products and softmax above, in
+ * fp32, fp16 or bf16 (`dtype`, a kbDtype): the norms and rotation of queries
+ * and keys, a paged key/value cache, attention over it, and the penalties on
+ * logits.  They replace no reference entry.  Strides are in elements unless
+ * stated; head vectors are contiguous.  Arithmetic is fp32, outputs are
+ * rounded once.                                                            */
+
+/* RMS norm over each head vector of q[tokens, heads_q, dim] and
+ * k[tokens, heads_kv, dim], times the weights [dim] (NULL: ones; fp32 or of
+ * type `dtype`), then the rotation of the first `rotary` elements by row
+ * positions[t] of cos/sin tables [table_rows, rotary / 2]: pairs
+ * (i, i + rotary/2), or (2i, 2i + 1) when interleaved.  positions are int64
+ * (positions_64 != 0) or int32; one outside the table gives NaN in the
+ * rotated elements.  Outputs are contiguous.  dim <= 512.                  */
+KB_API int kb_qk_norm_rope(const void* q, const void* k, const void* q_weight,
+                           const void* k_weight, const float* cos_table,
+                           const float* sin_table, const void* positions,
+                           void* q_out, void* k_out, int64_t tokens,
+                           int64_t heads_q, int64_t heads_kv, int64_t dim,
+                           int64_t rotary, int64_t table_rows,
+                           int64_t q_stride_token, int64_t q_stride_head,
+                           int64_t k_stride_token, int64_t k_stride_head,
+                           int dtype, int weight_dtype, int positions_64,
+                           int interleaved, float eps, kbStream stream);
+/* Its gradients: from those of the outputs (dq_out, dk_out, contiguous) and
+ * the inputs, dq and dk (contiguous) and the weights' dq_weight, dk_weight
+ * (type weight_dtype; NULL: not wanted), summed over tokens and heads in a
+ * fixed order.                                                             */
+KB_API size_t kb_qk_norm_rope_backward_workspace_size(int64_t tokens, int64_t heads_q,
+                                                      int64_t heads_kv, int64_t dim);
+KB_API int kb_qk_norm_rope_backward(const void* dq_out, const void* dk_out, const void* q,
+                                    const void* k, const void* q_weight,
+                                    const void* k_weight, const float* cos_table,
+                                    const float* sin_table, const void* positions,
+                                    void* dq, void* dk, void* dq_weight, void* dk_weight,
+                                    int64_t tokens, int64_t heads_q, int64_t heads_kv,
+                                    int64_t dim, int64_t rotary, int64_t table_rows,
+                                    int64_t q_stride_token, int64_t q_stride_head,
+                                    int64_t k_stride_token, int64_t k_stride_head,
+                                    int dtype, int weight_dtype, int positions_64,
+                                    int interleaved, float eps, void* workspace,
+                                    size_t workspace_bytes, kbStream stream);
+
+/* Attention of the `queries` newest tokens of each of `batch` sequences over
+ * a paged cache whose first prefix_pages pages all sequences share.
+ * q[batch, queries, heads_q, dim] (strides given); pools of pages
+ * [pages, page_size, heads_kv, dim] (strides given); key j of sequence b is
+ * slot j % page_size of page prefix[j / page_size] for j / page_size <
+ * prefix_pages, else of page table[b, j / page_size] (table[batch, width];
+ * its first prefix_pages columns are not read).  lens[b] counts b's keys with
+ * those of the queries: query t sees keys j < lens[b] - queries + t + 1.
+ * Query head h reads key head h / (heads_q / heads_kv).
+ * out[batch, queries, heads_q, dim] = softmax(scale q k) v and
+ * lse[batch, queries, heads_q] (fp32) = log sum exp; a query that sees no key
+ * gets 0 and -inf.  Slots that no query of a sequence sees are not read;
+ * where some of its queries see a key that others do not, its values must be
+ * finite.  dim <= 256, dim * element size, pointers and strides multiples of
+ * 16 bytes.                                                                */
+KB_API size_t kb_shared_prefix_attention_workspace_size(int64_t batch, int64_t queries,
+                                                        int64_t heads_q, int64_t heads_kv,
+                                                        int64_t dim, int64_t prefix_pages,
+                                                        int64_t width, int64_t page_size,
+                                                        int dtype);
+KB_API int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v_pages,
+                                      const int32_t* prefix, const int32_t* table,
+                                      const int32_t* lens, void* out, float* lse,
+                                      int64_t batch, int64_t queries, int64_t heads_q,
+                                      int64_t heads_kv, int64_t dim, int64_t prefix_pages,
+                                      int64_t width, int64_t pages, int64_t page_size,
+                                      int64_t q_stride_seq, int64_t q_stride_query,
+                                      int64_t q_stride_head, int64_t k_stride_page,
+                                      int64_t k_stride_slot, int64_t k_stride_head,
+                                      int64_t v_stride_page, int64_t v_stride_slot,
+                                      int64_t v_stride_head, float scale, int dtype,
+                                      void* workspace, size_t workspace_bytes,
+                                      kbStream stream);
+
+/* The paged cache.  State, all on the device: a pool [planes, pages,
+ * page_bytes] (planes: the keys and the values of each layer), a table
+ * [slots, width] of page ids (-1: none), lens[slots] keys of each slot, and
+ * refs[pages], how many table entries hold a page (0: free).  A slot holds
+ * ceil(lens / page_size) pages from the start of its row; a page that is not
+ * full is held by one slot.  Free pages are taken lowest first.  Requests
+ * are served in their order and granted[i] is 1, or 0 for a request that
+ * leaves its slot as it was: slots out of range, a slot listed again, no
+ * room in the row, or more pages asked for, up to and including this
+ * request, than are free.  At most 2^20 pages, slots, entries of a row and
+ * requests.
+ *   reserve  lens += tokens, with the pages that takes
+ *   append   k, v [n, tokens, key_bytes] (strides in BYTES) into the last
+ *            `tokens` places of slots seqs, of one layer's two planes
+ *   fork     children become copies of their parents: full pages shared, a
+ *            last page that is not full copied, in every plane.  All parents
+ *            are read before any child is replaced, and pages are taken
+ *            before those of the replaced children are given back.
+ *   free     lens = 0, pages given back
+ *   compact  the i-th live page at or above n moves to the i-th hole below,
+ *            n = live[0] = the number of live pages; the table follows
+ *   copy     pages src[i] of one pool to dst[i] of another or the same
+ *            (distinct, none also a source); ids out of range are skipped */
+KB_API size_t kb_cache_reserve_workspace_size(int64_t n, int64_t tokens, int64_t slots,
+                                              int64_t width, int64_t pages, int64_t page_size);
+KB_API int kb_cache_reserve(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* seqs,
+                            int32_t* granted, int64_t n, int64_t tokens, int64_t slots,
+                            int64_t width, int64_t pages, int64_t page_size, void* workspace,
+                            size_t workspace_bytes, kbStream stream);
+KB_API int kb_cache_append(const void* k, const void* v, void* k_pages, void* v_pages,
+                           const int32_t* table, const int32_t* lens, const int32_t* seqs,
+                           int64_t n, int64_t tokens, int64_t slots, int64_t width,
+                           int64_t pages, int64_t page_size, int64_t page_bytes,
+                           int64_t key_bytes, int64_t k_stride_seq, int64_t k_stride_token,
+                           int64_t v_stride_seq, int64_t v_stride_token, kbStream stream);
+KB_API size_t kb_cache_fork_workspace_size(int64_t n, int64_t slots, int64_t width);
+KB_API int kb_cache_fork(void* pool, int32_t* table, int32_t* lens, int32_t* refs,
+                         const int32_t* parents, const int32_t* children, int32_t* granted,
+                         int64_t n, int64_t slots, int64_t width, int64_t planes,
+                         int64_t pages, int64_t page_size, int64_t page_bytes,
+                         void* workspace, size_t workspace_bytes, kbStream stream);
+KB_API int kb_cache_free(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* seqs,
+                         int64_t n, int64_t slots, int64_t width, int64_t pages,
+                         kbStream stream);
+KB_API size_t kb_cache_compact_workspace_size(int64_t pages);
+KB_API int kb_cache_compact(void* pool, int32_t* table, int32_t* refs, int32_t* live,
+                            int64_t slots, int64_t width, int64_t planes, int64_t pages,
+                            int64_t page_bytes, void* workspace, size_t workspace_bytes,
+                            kbStream stream);
+KB_API int kb_cache_copy(const void* src_pool, const int32_t* src, void* dst_pool,
+                         const int32_t* dst, int64_t n, int64_t planes, int64_t page_bytes,
+                         int64_t src_pages, int64_t dst_pages, kbStream stream);
+
+/* Penalties, biases and masks on logits[rows, vocab] (row_stride):
+ *   seen in prompt or output:  l > 0 ? l / repetition : l * repetition
+ *   c times in the output:     l - frequency c - presence
+ *   bias_ids[rows, bias_len]:  l + bias_values (an id listed twice: the last)
+ *   mask bit clear:            -inf (bit v % 32 of word v / 32 of the row)
+ * in that order.  prompt[rows, prompt_len], output[rows, output_len] and
+ * bias_ids are int64 (ids_64 != 0) or int32; ids outside [0, vocab) are
+ * ignored.  repetition, presence, frequency: [rows] fp32 or NULL; mask: 32-bit
+ * words, mask_stride a row (0: one row for all), or NULL.  out[rows, vocab]
+ * is contiguous and may be logits itself.  output_len < 2^20,
+ * bias_len < 2048, rows < 65536.                                           */
+KB_API int kb_penalize_logits(const void* logits, void* out, const void* prompt,
+                              const void* output, const float* repetition,
+                              const float* presence, const float* frequency,
+                              const void* bias_ids, const float* bias_values,
+                              const void* mask, int64_t rows, int64_t vocab,
+                              int64_t row_stride, int64_t prompt_len, int64_t output_len,
+                              int64_t bias_len, int64_t mask_stride, int dtype, int ids_64,
+                              kbStream stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,577 @@
+// lm_attention.cu — attention of a batch of sequences that share a prefix,
+// over a paged cache of keys and values.
+//
+// Key j of sequence b lies in page prefix[j / page_size] for j < P = prefix
+// pages * page_size, else in page table[b][j / page_size].  Query t of the
+// `queries` newest tokens sees the keys j < lens[b] - queries + t + 1.
+//   s_j = scale q . k_j,  o = sum_j exp(s_j) v_j / sum_j exp(s_j),
+//   lse = log sum_j exp(s_j);   no key: o = 0, lse = -inf
+//
+// The prefix is the same for all sequences, so all their query rows of one
+// key head (batch * queries * group of them) meet each tile of it together:
+// it is read once per row tile instead of once per sequence, and the products
+// have enough rows for the tensor cores.  Each sequence's own keys meet its
+// own rows.  Both axes of keys are cut into ranges; a work item (row tile,
+// range) keeps the running maximum and sum of its softmax, in fp32, and writes
+// its normalised part of o and its lse, and a second kernel joins the parts:
+//   o = sum_i exp(lse_i - L) o_i,  L = log sum_i exp(lse_i).
+//
+// Keys at or past what a row tile sees are not read (they count as zeros), so
+// what stands in unused slots of a page does not matter.  Page ids out of
+// range are clamped into the pool.
+#include <type_traits>
+
+#include "lm_common.cuh"
+
+namespace kb {
+namespace lm {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+// 16 bytes from global to shared memory, zeros where `valid` is false.
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool valid) {
+  const int bytes = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+struct AttnArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const int *prefix, *table, *lens;
+  int batch, queries, heads_q, heads_kv, group, dim;
+  int prefix_pages, width, pages, page_size;
+  int64_t q_b, q_t, q_h, k_p, k_s, k_h, v_p, v_s, v_h;  // strides in elements
+  float scale_log2;                                      // scale * log2(e)
+  int prefix_tiles, prefix_splits, prefix_chunk;         // row tiles per key head; ranges and keys per range
+  int own_tiles, own_splits, own_chunk;
+  int64_t prefix_items;
+  float *part_o, *part_lse;  // [splits][batch * queries * heads_q][dim], [splits][rows]; null: one range only
+};
+
+// A work item: rows r of key head h, query of row r = base + r / group, head
+// h * group + r % group; keys [k0, k1) through `pages`.
+struct Item {
+  int h, base, row0, rows, k0, k1, split;
+  const int* pages;
+};
+__device__ __forceinline__ Item item_at(const AttnArgs& a, int64_t id, int tile_rows) {
+  Item w;
+  const int P = a.prefix_pages * a.page_size;
+  if (id < a.prefix_items) {  // key head fastest: CTAs that run together read different heads of the same pages
+    w.h = (int)(id % a.heads_kv);
+    id /= a.heads_kv;
+    const int tile = (int)(id % a.prefix_tiles), s = (int)(id / a.prefix_tiles);
+    w.base = 0;
+    w.row0 = tile * tile_rows;
+    w.rows = min(tile_rows, a.batch * a.queries * a.group - w.row0);
+    w.k0 = s * a.prefix_chunk;
+    w.k1 = min(w.k0 + a.prefix_chunk, P);
+    w.split = s;
+    w.pages = a.prefix;
+  } else {
+    id -= a.prefix_items;
+    w.h = (int)(id % a.heads_kv);
+    id /= a.heads_kv;
+    const int tile = (int)(id % a.own_tiles);
+    id /= a.own_tiles;
+    const int b = (int)(id % a.batch), s = (int)(id / a.batch);
+    w.base = b * a.queries;
+    w.row0 = tile * tile_rows;
+    w.rows = min(tile_rows, a.queries * a.group - w.row0);
+    w.k0 = P + s * a.own_chunk;
+    w.k1 = min(w.k0 + a.own_chunk, a.width * a.page_size);
+    w.split = a.prefix_splits + s;
+    w.pages = a.table + (int64_t)b * a.width;
+  }
+  return w;
+}
+__device__ __forceinline__ int visible(const AttnArgs& a, int bt) {
+  const int b = bt / a.queries, t = bt - b * a.queries;
+  return a.lens[b] - a.queries + t + 1;
+}
+
+// ------------------------------------------------------------------ products
+// Fragments of mma.sync: 16 rows x 8 columns of fp32 accumulators per warp.
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half*) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                      __nv_bfloat16*) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// fp32 as two TF32 values: hi keeps the upper 10 mantissa bits, lo = x - hi
+// (0 for a non-finite x, whose hi says it all).
+struct Split {
+  uint32_t hi, lo;
+};
+__device__ __forceinline__ Split split(float x) {
+  const uint32_t hi = __float_as_uint(x) & 0xffffe000u;
+  const float lo = x - __uint_as_float(hi);
+  return {hi, isfinite(lo) ? __float_as_uint(lo) : 0u};
+}
+// c += A B to fp32 accuracy: lo hi + hi lo + hi hi.
+__device__ __forceinline__ void mma_3xtf32(float (&c)[4], const Split (&a)[4], Split b0, Split b1) {
+  const uint32_t ah[4] = {a[0].hi, a[1].hi, a[2].hi, a[3].hi}, al[4] = {a[0].lo, a[1].lo, a[2].lo, a[3].lo};
+  mma_tf32(c, al, b0.hi, b1.hi);
+  mma_tf32(c, ah, b0.lo, b1.lo);
+  mma_tf32(c, ah, b0.hi, b1.hi);
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __half*) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float x, float y, __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// S[16 x NK] = Q (16 rows at `q`) K^T (NK keys at `k`), both row-major with a
+// row of LD elements; DP of them counted.
+template <typename T, int DP, int NK, int LD>
+__device__ __forceinline__ void scores(float (&s)[NK / 8][4], const T* q, const T* k, int lane) {
+#pragma unroll
+  for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
+  if constexpr (std::is_same_v<T, float>) {
+    const int r = lane >> 2, c = lane & 3;
+#pragma unroll 4
+    for (int d = 0; d < DP; d += 8) {
+      const Split qa[4] = {split(q[r * LD + d + c]), split(q[(r + 8) * LD + d + c]), split(q[r * LD + d + c + 4]),
+                           split(q[(r + 8) * LD + d + c + 4])};
+#pragma unroll
+      for (int n = 0; n < NK / 8; ++n)
+        mma_3xtf32(s[n], qa, split(k[(n * 8 + r) * LD + d + c]), split(k[(n * 8 + r) * LD + d + c + 4]));
+    }
+  } else {
+    const uint32_t qrow = smem_addr(q + (lane & 15) * LD + (lane >> 4) * 8);
+    const uint32_t krow = smem_addr(k + ((lane & 7) + ((lane >> 4) << 3)) * LD + ((lane >> 3) & 1) * 8);
+#pragma unroll
+    for (int d = 0; d < DP; d += 16) {
+      uint32_t qa[4];
+      ldmatrix4(qa, qrow + d * 2);
+#pragma unroll
+      for (int n = 0; n < NK / 16; ++n) {
+        uint32_t kb[4];
+        ldmatrix4(kb, krow + (n * 16 * LD + d) * 2);
+        mma16(s[2 * n], qa, kb[0], kb[1], (T*)nullptr);
+        mma16(s[2 * n + 1], qa, kb[2], kb[3], (T*)nullptr);
+      }
+    }
+  }
+}
+
+// O[16 x DP] += P[16 x NK] V (NK keys at `v`).  With 16-bit V, P is rounded to
+// V's type (the sum that divides it is not); with fp32 V both are split.
+template <typename T, int DP, int NK, int LD>
+__device__ __forceinline__ void weigh(float (&o)[DP / 8][4], const float (&p)[NK / 8][4], const T* v, int lane) {
+  if constexpr (std::is_same_v<T, float>) {
+    const int r = lane >> 2, c = lane & 3;
+#pragma unroll
+    for (int n = 0; n < NK / 8; ++n) {
+      // the order of keys within a product is free: slot c holds key 2c, slot c + 4 key 2c + 1, as P's registers do
+      const Split pa[4] = {split(p[n][0]), split(p[n][2]), split(p[n][1]), split(p[n][3])};
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d)
+        mma_3xtf32(o[d], pa, split(v[(n * 8 + 2 * c) * LD + d * 8 + r]), split(v[(n * 8 + 2 * c + 1) * LD + d * 8 + r]));
+    }
+  } else {
+    const uint32_t vrow = smem_addr(v + ((lane & 7) + ((lane >> 3) & 1) * 8) * LD + (lane >> 4) * 8);
+#pragma unroll
+    for (int n = 0; n < NK / 16; ++n) {
+      const uint32_t pa[4] = {pack2(p[2 * n][0], p[2 * n][1], (T*)nullptr), pack2(p[2 * n][2], p[2 * n][3], (T*)nullptr),
+                              pack2(p[2 * n + 1][0], p[2 * n + 1][1], (T*)nullptr),
+                              pack2(p[2 * n + 1][2], p[2 * n + 1][3], (T*)nullptr)};
+#pragma unroll
+      for (int d = 0; d < DP / 16; ++d) {
+        uint32_t vb[4];
+        ldmatrix4_trans(vb, vrow + (n * 16 * LD + d * 16) * 2);
+        mma16(o[2 * d], pa, vb[0], vb[1], (T*)nullptr);
+        mma16(o[2 * d + 1], pa, vb[2], vb[3], (T*)nullptr);
+      }
+    }
+  }
+}
+
+// The running softmax of a warp's 16 rows (two per thread): maximum m in units
+// of log2, sum l of this thread's columns.
+struct Running {
+  float m[2], l[2];
+};
+// Turns scores into weights exp2(s - m), after masking keys at or past
+// vis[row], and rescales o.
+template <int NK, int ND>
+__device__ __forceinline__ void softmax_step(float (&s)[NK / 8][4], float (&o)[ND][4], Running& st, float scale_log2,
+                                             int key0, const int (&vis)[2], bool masked, int lane) {
+  float top[2] = {st.m[0], st.m[1]};
+#pragma unroll
+  for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[n][i] *= scale_log2;
+      if (masked && key0 + n * 8 + (lane & 3) * 2 + (i & 1) >= vis[i >> 1]) s[n][i] = -INFINITY;
+      top[i >> 1] = fmaxf(top[i >> 1], s[n][i]);
+    }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
+    const float base = top[r] == -INFINITY ? 0.0f : top[r];
+    const float keep = ex2(st.m[r] - base);
+    st.m[r] = top[r];
+    st.l[r] *= keep;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) {
+      o[d][2 * r] *= keep;
+      o[d][2 * r + 1] *= keep;
+    }
+    top[r] = base;
+  }
+#pragma unroll
+  for (int n = 0; n < NK / 8; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s[n][i] = ex2(s[n][i] - top[i >> 1]);
+      st.l[i >> 1] += s[n][i];
+    }
+}
+
+// ------------------------------------------------------------------ rows kernel
+// Four warps of 16 rows each share tiles of NK keys and values, double
+// buffered by cp.async.
+template <typename T, int DP, int NK>
+struct RowsCfg {
+  static constexpr int kRows = 64, kThreads = 128;
+  static constexpr int LD = DP + 16 / (int)sizeof(T);  // rows 16 bytes apart in the banks
+  static constexpr size_t kSmem = sizeof(T) * LD * (kRows + 4 * NK);
+};
+
+template <typename T, int DP, int NK>
+__global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
+  using C = RowsCfg<T, DP, NK>;
+  constexpr int LD = C::LD, kVec = 16 / sizeof(T), kPerRow = DP / kVec;
+  extern __shared__ __align__(16) uint8_t raw[];
+  T* sq = reinterpret_cast<T*>(raw);
+  T* sk = sq + C::kRows * LD;
+  T* sv = sk + 2 * NK * LD;
+  __shared__ int s_max[4];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Item w = item_at(a, blockIdx.x, C::kRows);
+  const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
+
+  // this thread's two rows
+  const int row[2] = {warp * 16 + (lane >> 2), warp * 16 + (lane >> 2) + 8};
+  int vis[2];
+  int top = 0, low = 0x7fffffff;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    vis[r] = row[r] < w.rows ? visible(a, w.base + (w.row0 + row[r]) / a.group) : 0;
+    top = max(top, vis[r]);
+    if (row[r] < w.rows) low = min(low, vis[r]);
+  }
+  top = __reduce_max_sync(0xffffffffu, top);
+  low = __reduce_min_sync(0xffffffffu, low);
+  if (lane == 0) s_max[warp] = top;
+  __syncthreads();
+  const int end = min(w.k1, max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])));
+
+  const T* q = static_cast<const T*>(a.q);
+  const T* kp = static_cast<const T*>(a.k) + w.h * a.k_h;
+  const T* vp = static_cast<const T*>(a.v) + w.h * a.v_h;
+  for (int i = tid; i < C::kRows * kPerRow; i += C::kThreads) {
+    const int r = i / kPerRow, c = (i - r * kPerRow) * kVec;
+    const bool in = r < w.rows && c < a.dim;
+    const int rr = w.row0 + (in ? r : 0), bt = w.base + rr / a.group;
+    const T* src = q + (int64_t)(bt / a.queries) * a.q_b + (int64_t)(bt % a.queries) * a.q_t +
+                   (int64_t)(w.h * a.group + rr % a.group) * a.q_h + (in ? c : 0);
+    cp_async16(sq + r * LD + c, src, in);
+  }
+  auto load = [&](int key0, int buf) {
+    for (int i = tid; i < NK * kPerRow; i += C::kThreads) {
+      const int n = i / kPerRow, c = (i - n * kPerRow) * kVec;
+      const int j = key0 + n;
+      const bool in = j < end && c < a.dim;
+      int64_t page = 0;
+      int slot = 0;
+      if (in) {
+        const int pj = j / a.page_size;
+        slot = j - pj * a.page_size;
+        page = min(max(w.pages[pj], 0), a.pages - 1);
+      }
+      const int cc = in ? c : 0;
+      cp_async16(sk + (buf * NK + n) * LD + c, kp + page * a.k_p + slot * a.k_s + cc, in);
+      cp_async16(sv + (buf * NK + n) * LD + c, vp + page * a.v_p + slot * a.v_s + cc, in);
+    }
+    cp_async_commit();
+  };
+
+  float o[DP / 8][4];
+#pragma unroll
+  for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[d][i] = 0.0f;
+  Running st{{-INFINITY, -INFINITY}, {0.0f, 0.0f}};
+  if (w.k0 < end) load(w.k0, 0);
+  int buf = 0;
+  for (int key0 = w.k0; key0 < end; key0 += NK, buf ^= 1) {
+    if (key0 + NK < end) {
+      load(key0 + NK, buf ^ 1);
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncthreads();
+    float s[NK / 8][4];
+    scores<T, DP, NK, LD>(s, sq + warp * 16 * LD, sk + buf * NK * LD, lane);
+    const int seen[2] = {min(vis[0], end), min(vis[1], end)};
+    softmax_step<NK, DP / 8>(s, o, st, a.scale_log2, key0, seen, key0 + NK > min(low, end), lane);
+    weigh<T, DP, NK, LD>(o, s, sv + buf * NK * LD, lane);
+    __syncthreads();
+  }
+  cp_async_wait<0>();  // the queries' copies, where there was no key
+
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 1);
+    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 2);
+    if (row[r] >= w.rows) continue;
+    const int rr = w.row0 + row[r];
+    const int64_t at = (int64_t)(w.base + rr / a.group) * a.heads_q + w.h * a.group + rr % a.group;
+    const bool none = st.l[r] == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / st.l[r];
+    const float lse = none ? -INFINITY : st.m[r] * kLn2 + logf(st.l[r]);
+    if (a.part_o) {
+      const int64_t slot = (int64_t)w.split * n_rows + at;
+      if ((lane & 3) == 0) a.part_lse[slot] = lse;
+      if (none) continue;  // the join does not read it
+      float* y = a.part_o + slot * a.dim;
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) {
+        const int c = d * 8 + (lane & 3) * 2;
+        if (c < a.dim) *reinterpret_cast<float2*>(y + c) = make_float2(o[d][2 * r] * inv, o[d][2 * r + 1] * inv);
+      }
+    } else {
+      if ((lane & 3) == 0) a.lse[at] = lse;
+      T* y = static_cast<T*>(a.out) + at * a.dim;
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) {
+        const int c = d * 8 + (lane & 3) * 2;
+        if (c < a.dim) {
+          y[c] = from_f32<T>(none ? 0.0f : o[d][2 * r] * inv);
+          y[c + 1] = from_f32<T>(none ? 0.0f : o[d][2 * r + 1] * inv);
+        }
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ join
+// One warp per row: the parts weighed by exp(lse_i - L), in their order.
+template <typename T>
+__global__ void __launch_bounds__(128) attn_join_kernel(const float* __restrict__ part_o,
+                                                        const float* __restrict__ part_lse, int splits, int64_t rows,
+                                                        int dim, T* __restrict__ out, float* __restrict__ lse) {
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int lane = threadIdx.x & 31;
+  float top = -INFINITY;
+  for (int i = lane; i < splits; i += 32) top = fmaxf(top, part_lse[i * rows + row]);
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.0f : top;
+  float total = 0.0f;  // a NaN part makes it NaN
+  for (int i = lane; i < splits; i += 32) total += ex2((part_lse[i * rows + row] - base) * kLog2e);
+  total = warp_sum(total);
+  const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+  for (int d0 = 0; d0 < dim; d0 += 32) {
+    const int d = d0 + lane;
+    float acc = 0.0f;
+    for (int i = 0; i < splits; ++i) {
+      const float l = part_lse[i * rows + row];
+      if (l == -INFINITY) continue;  // not written
+      if (d < dim) acc += ex2((l - base) * kLog2e) * inv * part_o[(i * rows + row) * dim + d];
+    }
+    if (d < dim) out[row * dim + d] = from_f32<T>(acc);
+  }
+  if (lane == 0) lse[row] = total == 0.0f ? -INFINITY : base + logf(total);
+}
+
+// ------------------------------------------------------------------ host side
+struct Plan {
+  int prefix_tiles = 0, prefix_splits = 0, prefix_chunk = 1;
+  int own_tiles = 0, own_splits = 0, own_chunk = 1;
+  int splits() const { return prefix_splits + own_splits; }
+};
+
+// Ranges of keys: enough work items to fill the SMs, none shorter than a few
+// tiles.
+Plan plan(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv, int64_t prefix_keys, int64_t own_keys) {
+  constexpr int kTile = 64;
+  Plan p;
+  const int64_t group = heads_q / heads_kv, sms = sm_count();
+  if (prefix_keys > 0) {
+    p.prefix_tiles = (int)ceil_div(batch * queries * group, kTile);
+    const int64_t items = p.prefix_tiles * heads_kv;
+    const int64_t s = std::max<int64_t>(1, std::min(ceil_div(4 * sms, items), ceil_div(prefix_keys, 4 * kTile)));
+    p.prefix_chunk = (int)(ceil_div(ceil_div(prefix_keys, s), kTile) * kTile);
+    p.prefix_splits = (int)ceil_div(prefix_keys, p.prefix_chunk);
+  }
+  if (own_keys > 0) {
+    p.own_tiles = (int)ceil_div(queries * group, kTile);
+    const int64_t items = p.own_tiles * heads_kv * batch;
+    const int64_t s = std::max<int64_t>(1, std::min(ceil_div(4 * sms, items), ceil_div(own_keys, 4 * kTile)));
+    p.own_chunk = (int)(ceil_div(ceil_div(own_keys, s), kTile) * kTile);
+    p.own_splits = (int)ceil_div(own_keys, p.own_chunk);
+  }
+  return p;
+}
+
+template <typename T, int DP, int NK>
+int launch_rows(const AttnArgs& a, int64_t items, cudaStream_t stream) {
+  auto kern = attn_rows_kernel<T, DP, NK>;
+  constexpr size_t smem = RowsCfg<T, DP, NK>::kSmem;
+  static uint64_t attr_set = 0;  // one bit per device ordinal
+  int dev = 0;
+  KB_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !(attr_set >> dev & 1)) {
+    KB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    if (dev < 64) attr_set |= 1ull << dev;
+  }
+  kern<<<(unsigned)items, 128, smem, stream>>>(a);
+  return check_launch("kb_shared_prefix_attention");
+}
+
+template <typename T>
+int launch_by_dim(const AttnArgs& a, int64_t items, cudaStream_t stream) {
+  if (a.dim <= 64) return launch_rows<T, 64, 64>(a, items, stream);
+  if (a.dim <= 128) return launch_rows<T, 128, 64>(a, items, stream);
+  return launch_rows<T, 256, sizeof(T) == 4 ? 32 : 64>(a, items, stream);
+}
+
+}  // namespace
+}  // namespace lm
+}  // namespace kb
+
+extern "C" {
+
+size_t kb_shared_prefix_attention_workspace_size(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv,
+                                                 int64_t dim, int64_t prefix_pages, int64_t width,
+                                                 int64_t page_size, int dtype) {
+  (void)dtype;
+  if (batch <= 0 || queries <= 0 || heads_q <= 0 || heads_kv <= 0 || dim <= 0 || page_size <= 0) return 0;
+  const kb::lm::Plan p = kb::lm::plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size,
+                                      std::max<int64_t>(0, width - prefix_pages) * page_size);
+  if (p.splits() <= 1) return 0;
+  const int64_t rows = batch * queries * heads_q;
+  return (size_t)p.splits() * (rows * dim + kb::ceil_div(rows, 4) * 4) * sizeof(float);
+}
+
+int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* prefix,
+                               const int32_t* table, const int32_t* lens, void* out, float* lse, int64_t batch,
+                               int64_t queries, int64_t heads_q, int64_t heads_kv, int64_t dim, int64_t prefix_pages,
+                               int64_t width, int64_t pages, int64_t page_size, int64_t q_stride_seq,
+                               int64_t q_stride_query, int64_t q_stride_head, int64_t k_stride_page,
+                               int64_t k_stride_slot, int64_t k_stride_head, int64_t v_stride_page,
+                               int64_t v_stride_slot, int64_t v_stride_head, float scale, int dtype, void* workspace,
+                               size_t workspace_bytes, kbStream stream) {
+  const char* name = "kb_shared_prefix_attention";
+  using namespace kb::lm;
+  KB_REQUIRE(batch >= 0 && queries >= 0 && heads_q >= 0 && heads_kv >= 0 && dim >= 0 && prefix_pages >= 0 &&
+                 width >= 0 && pages >= 0 && page_size >= 1,
+             KB_ERR_INVALID_ARG, "%s: negative size", name);
+  KB_REQUIRE(dtype_size(dtype), KB_ERR_INVALID_ARG, "%s: unknown element type", name);
+  const int64_t rows = batch * queries * heads_q;
+  if (rows == 0 || dim == 0) return KB_OK;
+  KB_REQUIRE(heads_kv >= 1 && heads_q % heads_kv == 0, KB_ERR_INVALID_ARG,
+             "%s: %lld query heads do not divide into %lld key heads", name, (long long)heads_q, (long long)heads_kv);
+  KB_REQUIRE(q && lens && out && lse, KB_ERR_INVALID_ARG, "%s: null pointer", name);
+  const int64_t own_pages = std::max<int64_t>(0, width - prefix_pages);
+  KB_REQUIRE((prefix_pages == 0 || prefix) && (own_pages == 0 || table), KB_ERR_INVALID_ARG, "%s: null table", name);
+  KB_REQUIRE(prefix_pages + own_pages == 0 || (pages >= 1 && k_pages && v_pages), KB_ERR_INVALID_ARG,
+             "%s: pages without a pool", name);
+  const int e = dtype_size(dtype);
+  KB_REQUIRE(dim <= 256 && dim * e % 16 == 0, KB_ERR_UNSUPPORTED,
+             "%s: head dim %lld must be at most 256 and fill whole 16-byte vectors", name, (long long)dim);
+  auto whole = [&](int64_t s) { return s * e % 16 == 0; };
+  KB_REQUIRE(kb::aligned16(q) && kb::aligned16(k_pages) && kb::aligned16(v_pages) && kb::aligned16(out) &&
+                 whole(q_stride_seq) && whole(q_stride_query) && whole(q_stride_head) && whole(k_stride_page) &&
+                 whole(k_stride_slot) && whole(k_stride_head) && whole(v_stride_page) && whole(v_stride_slot) &&
+                 whole(v_stride_head),
+             KB_ERR_UNSUPPORTED, "%s: queries, pools and their strides must be multiples of 16 bytes", name);
+  KB_REQUIRE(rows <= 0x3fffffff && (prefix_pages + own_pages) * page_size <= 0x3fffffff && pages <= 0x7fffffff,
+             KB_ERR_UNSUPPORTED, "%s: too many rows or keys", name);
+  const Plan p = plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size, own_pages * page_size);
+  AttnArgs a{};
+  a.q = q, a.k = k_pages, a.v = v_pages, a.out = out, a.lse = lse;
+  a.prefix = prefix, a.table = table, a.lens = lens;
+  a.batch = (int)batch, a.queries = (int)queries, a.heads_q = (int)heads_q, a.heads_kv = (int)heads_kv;
+  a.group = (int)(heads_q / heads_kv), a.dim = (int)dim;
+  a.prefix_pages = (int)prefix_pages, a.width = (int)width, a.pages = (int)pages, a.page_size = (int)page_size;
+  a.q_b = q_stride_seq, a.q_t = q_stride_query, a.q_h = q_stride_head;
+  a.k_p = k_stride_page, a.k_s = k_stride_slot, a.k_h = k_stride_head;
+  a.v_p = v_stride_page, a.v_s = v_stride_slot, a.v_h = v_stride_head;
+  a.scale_log2 = scale * kLog2e;
+  a.prefix_tiles = p.prefix_tiles, a.prefix_splits = p.prefix_splits, a.prefix_chunk = p.prefix_chunk;
+  a.own_tiles = p.own_tiles, a.own_splits = p.own_splits, a.own_chunk = p.own_chunk;
+  a.prefix_items = (int64_t)p.prefix_tiles * p.prefix_splits * heads_kv;
+  const int64_t items = a.prefix_items + (int64_t)p.own_tiles * p.own_splits * heads_kv * batch;
+  KB_REQUIRE(items <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many work items", name);
+  if (p.splits() > 1) {
+    const size_t need = kb_shared_prefix_attention_workspace_size(batch, queries, heads_q, heads_kv, dim,
+                                                                  prefix_pages, width, page_size, dtype);
+    KB_REQUIRE(workspace && workspace_bytes >= need, KB_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", name, need, workspace_bytes);
+    KB_REQUIRE(kb::aligned16(workspace), KB_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
+    a.part_o = static_cast<float*>(workspace);
+    a.part_lse = a.part_o + (int64_t)p.splits() * rows * dim;
+  }
+  return with_dtype(dtype, [&](auto* x) {
+    using T = std::remove_pointer_t<decltype(x)>;
+    if (items) {
+      if (int st = launch_by_dim<T>(a, items, stream)) return st;
+      if (p.splits() == 1) return (int)KB_OK;
+    }
+    // also where there are no keys at all: zeros and -inf
+    attn_join_kernel<T><<<(unsigned)kb::ceil_div(rows, 4), 128, 0, stream>>>(
+        a.part_o, a.part_lse, p.splits(), rows, (int)dim, static_cast<T*>(out), lse);
+    return kb::check_launch(name);
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,502 @@
+// lm_cache.cu — the page operations of a paged key/value cache, kept and
+// decided on the GPU: no call waits for the host.
+//
+// State: a pool [planes, pages, page bytes] (planes: keys and values of each
+// layer), a table [slots, width] of page ids (-1: none), the number of keys
+// lens[slots], and refs[pages], the number of table entries that hold each
+// page (0: free).  A slot holds ceil(lens / page_size) pages from the start
+// of its row; a page that is not full belongs to one slot alone.
+//
+//   reserve  grows slots by `tokens` keys, taking pages
+//   append   writes keys and values at a slot's last `tokens` places
+//   fork     makes child slots copies of parent slots: full pages are
+//            shared, a last page that is not full is copied
+//   free     empties slots
+//   compact  moves the live pages to the low end of the pool
+//   copy     copies listed pages between pools
+//
+// Free pages are taken in ascending order, requests are served in their
+// order, and a request is granted while the pages asked for up to and
+// including it are there: results do not depend on timing.  Page ids and
+// slots read from device memory are checked before use; one out of range is
+// passed over.
+#include "lm_common.cuh"
+
+namespace kb {
+namespace lm {
+namespace {
+
+constexpr int kPlanThreads = 1024;
+constexpr int kMaxPages = 1 << 20, kMaxSlots = 1 << 20;
+
+// Exclusive prefix sum over the block, and the total.
+__device__ __forceinline__ int block_scan(int v, int* red, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += n;
+  }
+  if (lane == 31) red[warp] = inc;
+  __syncthreads();
+  int w = lane < (int)(blockDim.x >> 5) ? red[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int n = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += n;
+  }
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = warp ? __shfl_sync(0xffffffffu, w, warp - 1) : 0;
+  __syncthreads();
+  return before + inc - v;
+}
+
+// list[r] = the r-th lowest page with refs == 0, for r < want; returns how
+// many there are, at most `want`.
+__device__ int free_pages(const int* refs, int pages, int want, int* list, int* red) {
+  int found = 0;
+  for (int base = 0; base < pages && found < want; base += kPlanThreads) {
+    const int p = base + threadIdx.x;
+    const int is_free = p < pages && refs[p] == 0;
+    int total;
+    const int at = found + block_scan(is_free, red, total);
+    if (is_free && at < want) list[at] = p;
+    found += total;
+  }
+  __syncthreads();
+  return min(found, want);
+}
+
+// ------------------------------------------------------------------ fork
+struct ForkArgs {
+  int *table, *lens, *refs;
+  const int *parents, *children;
+  int* granted;
+  int n, slots, width, pages, page_size;
+  int *owner;   // [slots] lowest request that names the slot as its child
+  int *list;    // [n] free pages
+  int *src, *dst;  // [n] page to copy and where to, or -1
+  int *len;     // [n] the child's new length, or -1 where nothing changes
+  int *rows;    // [n][width] the children's new rows
+};
+
+__global__ void __launch_bounds__(kPlanThreads) fork_plan(ForkArgs a) {
+  __shared__ int red[32];
+  for (int i = threadIdx.x; i < a.slots; i += kPlanThreads) a.owner[i] = a.n;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
+    const int c = a.children[i];
+    if (c >= 0 && c < a.slots) atomicMin(&a.owner[c], i);
+  }
+  __syncthreads();
+  const int have = free_pages(a.refs, a.pages, a.n, a.list, red);
+  int asked = 0;
+  for (int base = 0; base < a.n; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int need = 0, len = -1, ok = 0, src = -1;
+    if (i < a.n) {
+      const int p = a.parents[i], c = a.children[i];
+      ok = p >= 0 && p < a.slots && c >= 0 && c < a.slots && a.owner[c] == i;
+      if (ok && p != c) {
+        len = max(0, min(a.lens[p], a.width * a.page_size));
+        if (len % a.page_size) {
+          src = a.table[(int64_t)p * a.width + len / a.page_size];
+          need = src >= 0 && src < a.pages;
+        }
+      }
+    }
+    int total;
+    const int rank = asked + block_scan(need, red, total);
+    asked += total;
+    if (i < a.n) {
+      if (need && rank >= have) ok = 0, len = -1, need = 0;
+      a.granted[i] = ok;
+      a.len[i] = len;
+      a.src[i] = need ? src : -1;
+      a.dst[i] = need ? a.list[rank] : -1;
+    }
+  }
+}
+
+// The children's new rows, from the parents' before any of them is replaced.
+__global__ void fork_rows(ForkArgs a) {
+  const int i = blockIdx.x, len = a.len[i];
+  if (len < 0) return;
+  const int held = (len + a.page_size - 1) / a.page_size;
+  const int* from = a.table + (int64_t)a.parents[i] * a.width;
+  int* to = a.rows + (int64_t)i * a.width;
+  for (int j = threadIdx.x; j < a.width; j += blockDim.x)
+    to[j] = j >= held ? -1 : (a.dst[i] >= 0 && j == held - 1) ? a.dst[i] : from[j];
+}
+
+__global__ void fork_commit(ForkArgs a) {
+  const int i = blockIdx.x, len = a.len[i];
+  if (len < 0) return;
+  const int c = a.children[i];
+  int* row = a.table + (int64_t)c * a.width;
+  const int* to = a.rows + (int64_t)i * a.width;
+  for (int j = threadIdx.x; j < a.width; j += blockDim.x) {
+    const int before = row[j], after = to[j];
+    if (before >= 0 && before < a.pages) atomicSub(&a.refs[before], 1);
+    if (after >= 0 && after < a.pages) atomicAdd(&a.refs[after], 1);
+    row[j] = after;
+  }
+  if (threadIdx.x == 0) a.lens[c] = len;
+}
+
+// ------------------------------------------------------------------ copy
+// plane-wise copies of pages src[i] -> dst[i]; `count` (device) where it is
+// not null, else n, pairs.  Pairs with an id out of range are passed over.
+__global__ void __launch_bounds__(256) copy_pages(const char* __restrict__ from, char* __restrict__ to,
+                                                  const int* __restrict__ src, const int* __restrict__ dst,
+                                                  const int* __restrict__ count, int n, int64_t planes,
+                                                  int64_t page_bytes, int64_t from_pages, int64_t to_pages) {
+  const int64_t pairs = count ? min(*count, n) : n;
+  const bool wide = page_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0 &&
+                    (reinterpret_cast<uintptr_t>(to) & 15) == 0;
+  for (int64_t it = blockIdx.x; it < pairs * planes; it += gridDim.x) {
+    const int64_t i = it / planes, plane = it - i * planes;
+    const int s = src[i], d = dst[i];
+    if (s < 0 || s >= from_pages || d < 0 || d >= to_pages) continue;
+    const char* x = from + (plane * from_pages + s) * page_bytes;
+    char* y = to + (plane * to_pages + d) * page_bytes;
+    if (wide) {
+      const int64_t vecs = page_bytes / 16;
+      for (int64_t j = threadIdx.x; j < vecs; j += blockDim.x)
+        reinterpret_cast<uint4*>(y)[j] = reinterpret_cast<const uint4*>(x)[j];
+    } else {
+      for (int64_t j = threadIdx.x; j < page_bytes; j += blockDim.x) y[j] = x[j];
+    }
+  }
+}
+
+// ------------------------------------------------------------------ reserve
+struct ReserveArgs {
+  int *table, *lens, *refs;
+  const int* seqs;
+  int* granted;
+  int n, tokens, slots, width, pages, page_size;
+  int *owner, *list;
+};
+
+__global__ void __launch_bounds__(kPlanThreads) reserve_kernel(ReserveArgs a) {
+  __shared__ int red[32];
+  for (int i = threadIdx.x; i < a.slots; i += kPlanThreads) a.owner[i] = a.n;
+  __syncthreads();
+  for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
+    const int c = a.seqs[i];
+    if (c >= 0 && c < a.slots) atomicMin(&a.owner[c], i);
+  }
+  __syncthreads();
+  // no slot takes more pages than its row is wide, nor all more than there are
+  const int most = (int)min((int64_t)a.pages, (int64_t)a.n * min(a.width, a.tokens / a.page_size + 1));
+  const int have = free_pages(a.refs, a.pages, most, a.list, red);
+  int asked = 0;
+  for (int base = 0; base < a.n; base += kPlanThreads) {
+    const int i = base + threadIdx.x;
+    int need = 0, ok = 0, held = 0, len = 0, c = -1;
+    if (i < a.n) {
+      c = a.seqs[i];
+      ok = c >= 0 && c < a.slots && a.owner[c] == i;
+      if (ok) {
+        len = a.lens[c];
+        ok = len >= 0 && (int64_t)len + a.tokens <= (int64_t)a.width * a.page_size;
+      }
+      if (ok) {
+        held = (len + a.page_size - 1) / a.page_size;
+        // capped past the pool, so that sums over a block stay in 32 bits
+        need = min((len + a.tokens + a.page_size - 1) / a.page_size - held, a.pages + 1);
+      }
+    }
+    int total;
+    const int rank = asked + block_scan(need, red, total);
+    asked = (int)min((int64_t)asked + total, (int64_t)1 << 26);
+    if (i < a.n) {
+      if (need && rank + need > have) ok = 0;
+      a.granted[i] = ok;
+      if (ok) {
+        for (int j = 0; j < need; ++j) {
+          const int p = a.list[rank + j];
+          a.table[(int64_t)c * a.width + held + j] = p;
+          a.refs[p] = 1;
+        }
+        a.lens[c] = len + a.tokens;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ append
+struct AppendArgs {
+  const char *k, *v;
+  char *k_pages, *v_pages;
+  const int *table, *lens, *seqs;
+  int64_t k_stride_seq, k_stride_tok, v_stride_seq, v_stride_tok;  // bytes
+  int64_t page_bytes, key_bytes;  // a page, and one token's heads, of one plane
+  int n, tokens, slots, width, pages, page_size;
+};
+
+__global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
+  const int64_t i = blockIdx.x / a.tokens;
+  const int t = (int)(blockIdx.x - i * a.tokens);
+  const int c = a.seqs[i];
+  if (c < 0 || c >= a.slots) return;
+  const int pos = a.lens[c] - a.tokens + t;
+  if (pos < 0 || pos / a.page_size >= a.width) return;
+  const int p = a.table[(int64_t)c * a.width + pos / a.page_size];
+  if (p < 0 || p >= a.pages) return;
+  const int64_t at = p * a.page_bytes + (pos % a.page_size) * a.key_bytes;
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const char* x = kv ? a.v + i * a.v_stride_seq + t * a.v_stride_tok : a.k + i * a.k_stride_seq + t * a.k_stride_tok;
+    char* y = (kv ? a.v_pages : a.k_pages) + at;
+    if (a.key_bytes % 16 == 0 && ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) & 15) == 0) {
+      for (int64_t j = threadIdx.x; j < a.key_bytes / 16; j += blockDim.x)
+        reinterpret_cast<uint4*>(y)[j] = reinterpret_cast<const uint4*>(x)[j];
+    } else {
+      for (int64_t j = threadIdx.x; j < a.key_bytes; j += blockDim.x) y[j] = x[j];
+    }
+  }
+}
+
+// ------------------------------------------------------------------ free
+__global__ void free_kernel(int* table, int* lens, int* refs, const int* seqs, int slots, int width, int pages) {
+  __shared__ int len;
+  const int c = seqs[blockIdx.x];
+  if (c < 0 || c >= slots) return;
+  if (threadIdx.x == 0) len = atomicExch(&lens[c], 0);  // a slot that is listed twice is emptied once
+  __syncthreads();
+  if (len <= 0) return;
+  int* row = table + (int64_t)c * width;
+  for (int j = threadIdx.x; j < width; j += blockDim.x) {
+    const int p = row[j];
+    if (p >= 0 && p < pages) atomicSub(&refs[p], 1);
+    row[j] = -1;
+  }
+}
+
+// ------------------------------------------------------------------ compact
+struct CompactArgs {
+  int *table, *refs;
+  int* live;
+  int64_t entries;
+  int pages;
+  int *src, *dst, *count;  // the moves
+  int* map;                // [pages] where a moved page goes, or -1
+};
+
+__global__ void __launch_bounds__(kPlanThreads) compact_plan(CompactArgs a) {
+  __shared__ int red[32];
+  int mine = 0, live;
+  for (int p = threadIdx.x; p < a.pages; p += kPlanThreads) mine += a.refs[p] > 0;
+  block_scan(mine, red, live);
+  int holes = 0, moved = 0;
+  for (int base = 0; base < a.pages; base += kPlanThreads) {
+    const int p = base + threadIdx.x;
+    const bool used = p < a.pages && a.refs[p] > 0;
+    const int hole = p < live && !used, move = p >= live && used;
+    int total;
+    const int h = holes + block_scan(hole, red, total);
+    holes += total;
+    const int m = moved + block_scan(move, red, total);
+    moved += total;
+    if (hole) a.dst[h] = p;
+    if (move) a.src[m] = p;
+  }
+  // as many holes below the live count as live pages above it
+  __syncthreads();
+  for (int p = threadIdx.x; p < a.pages; p += kPlanThreads) a.map[p] = -1;
+  __syncthreads();
+  for (int i = threadIdx.x; i < moved; i += kPlanThreads) {
+    const int s = a.src[i], d = a.dst[i];
+    a.map[s] = d;
+    a.refs[d] = a.refs[s];
+    a.refs[s] = 0;
+  }
+  if (threadIdx.x == 0) {
+    *a.count = moved;
+    *a.live = live;
+  }
+}
+
+__global__ void compact_table(CompactArgs a) {
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < a.entries;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int p = a.table[i];
+    if (p >= 0 && p < a.pages && a.map[p] >= 0) a.table[i] = a.map[p];
+  }
+}
+
+unsigned copy_grid(int64_t items) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(items, sm_count() * 8)); }
+
+size_t ints(int64_t n) { return (size_t)ceil_div(n, 4) * 16; }
+
+}  // namespace
+}  // namespace lm
+}  // namespace kb
+
+extern "C" {
+
+#define KB_CACHE_COMMON(n)                                                                                       \
+  KB_REQUIRE((n) >= 0 && slots >= 0 && width >= 0 && pages >= 0, KB_ERR_INVALID_ARG, "%s: negative size", name); \
+  KB_REQUIRE(slots <= kMaxSlots && width <= kMaxSlots && pages <= kMaxPages && (n) <= kMaxSlots,                  \
+             KB_ERR_UNSUPPORTED, "%s: more than %d pages or %d slots, entries of a row or requests", name,        \
+             kMaxPages, kMaxSlots)
+
+#define KB_CACHE_WORKSPACE(need)                                                                       \
+  KB_REQUIRE(workspace && workspace_bytes >= (need), KB_ERR_WORKSPACE,                                 \
+             "%s: workspace of %zu bytes needed, %zu given", name, (size_t)(need), workspace_bytes);   \
+  KB_REQUIRE(kb::aligned16(workspace), KB_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name)
+
+size_t kb_cache_fork_workspace_size(int64_t n, int64_t slots, int64_t width) {
+  if (n <= 0 || slots < 0 || width < 0) return 0;
+  return kb::lm::ints(slots) + 4 * kb::lm::ints(n) + kb::lm::ints(n * width);
+}
+
+int kb_cache_fork(void* pool, int32_t* table, int32_t* lens, int32_t* refs, const int32_t* parents,
+                  const int32_t* children, int32_t* granted, int64_t n, int64_t slots, int64_t width, int64_t planes,
+                  int64_t pages, int64_t page_size, int64_t page_bytes, void* workspace, size_t workspace_bytes,
+                  kbStream stream) {
+  const char* name = "kb_cache_fork";
+  using namespace kb::lm;
+  KB_CACHE_COMMON(n);
+  KB_REQUIRE(planes >= 0 && page_bytes >= 0 && page_size >= 1, KB_ERR_INVALID_ARG, "%s: bad page", name);
+  KB_REQUIRE(page_size * width <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: rows of more than 2^31 keys", name);
+  if (n == 0) return KB_OK;
+  KB_REQUIRE(parents && children && granted && (!slots || (lens && (!width || table))) && (!pages || refs),
+             KB_ERR_INVALID_ARG, "%s: null pointer", name);
+  KB_REQUIRE(pool || !planes || !pages || !page_bytes, KB_ERR_INVALID_ARG, "%s: null pool", name);
+  KB_CACHE_WORKSPACE(kb_cache_fork_workspace_size(n, slots, width));
+  char* w = static_cast<char*>(workspace);
+  ForkArgs a{table, lens, refs, parents, children, granted, (int)n, (int)slots, (int)width, (int)pages, (int)page_size,
+             nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+  auto take = [&](int64_t m) {
+    int* p = reinterpret_cast<int*>(w);
+    w += ints(m);
+    return p;
+  };
+  a.owner = take(slots), a.list = take(n), a.src = take(n), a.dst = take(n), a.len = take(n), a.rows = take(n * width);
+  fork_plan<<<1, kPlanThreads, 0, stream>>>(a);
+  if (int st = kb::check_launch(name)) return st;
+  fork_rows<<<(unsigned)n, 256, 0, stream>>>(a);
+  if (int st = kb::check_launch(name)) return st;
+  if (planes && page_bytes && pages) {
+    copy_pages<<<copy_grid(n * planes), 256, 0, stream>>>(static_cast<const char*>(pool), static_cast<char*>(pool),
+                                                          a.src, a.dst, nullptr, (int)n, planes, page_bytes, pages,
+                                                          pages);
+    if (int st = kb::check_launch(name)) return st;
+  }
+  fork_commit<<<(unsigned)n, 256, 0, stream>>>(a);
+  return kb::check_launch(name);
+}
+
+size_t kb_cache_reserve_workspace_size(int64_t n, int64_t tokens, int64_t slots, int64_t width, int64_t pages,
+                                       int64_t page_size) {
+  if (n <= 0 || slots < 0 || width < 0 || pages < 0 || tokens < 0 || page_size < 1) return 0;
+  const int64_t most = std::min<int64_t>(pages, n * std::min<int64_t>(width, tokens / page_size + 1));
+  return kb::lm::ints(slots) + kb::lm::ints(most);
+}
+
+int kb_cache_reserve(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* seqs, int32_t* granted, int64_t n,
+                     int64_t tokens, int64_t slots, int64_t width, int64_t pages, int64_t page_size, void* workspace,
+                     size_t workspace_bytes, kbStream stream) {
+  const char* name = "kb_cache_reserve";
+  using namespace kb::lm;
+  KB_CACHE_COMMON(n);
+  KB_REQUIRE(tokens >= 0 && page_size >= 1, KB_ERR_INVALID_ARG, "%s: bad page or token count", name);
+  KB_REQUIRE(page_size * width <= 0x3fffffff && tokens <= 0x3fffffff, KB_ERR_UNSUPPORTED, "%s: too many keys", name);
+  if (n == 0) return KB_OK;
+  KB_REQUIRE(seqs && granted && (!slots || (lens && (!width || table))) && (!pages || refs), KB_ERR_INVALID_ARG,
+             "%s: null pointer", name);
+  KB_CACHE_WORKSPACE(kb_cache_reserve_workspace_size(n, tokens, slots, width, pages, page_size));
+  ReserveArgs a{table, lens, refs, seqs, granted, (int)n, (int)tokens, (int)slots, (int)width, (int)pages,
+                (int)page_size, static_cast<int*>(workspace),
+                reinterpret_cast<int*>(static_cast<char*>(workspace) + ints(slots))};
+  reserve_kernel<<<1, kPlanThreads, 0, stream>>>(a);
+  return kb::check_launch(name);
+}
+
+int kb_cache_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
+                    const int32_t* lens, const int32_t* seqs, int64_t n, int64_t tokens, int64_t slots, int64_t width,
+                    int64_t pages, int64_t page_size, int64_t page_bytes, int64_t key_bytes, int64_t k_stride_seq,
+                    int64_t k_stride_token, int64_t v_stride_seq, int64_t v_stride_token, kbStream stream) {
+  const char* name = "kb_cache_append";
+  using namespace kb::lm;
+  KB_CACHE_COMMON(n);
+  KB_REQUIRE(tokens >= 0 && page_size >= 1 && key_bytes >= 0 && page_bytes >= page_size * key_bytes,
+             KB_ERR_INVALID_ARG, "%s: bad page or token count", name);
+  KB_REQUIRE(page_size <= 0x7fffffff && n * tokens <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many tokens", name);
+  if (n == 0 || tokens == 0 || key_bytes == 0 || slots == 0 || width == 0 || pages == 0) return KB_OK;
+  KB_REQUIRE(k && v && k_pages && v_pages && table && lens && seqs, KB_ERR_INVALID_ARG, "%s: null pointer", name);
+  AppendArgs a{static_cast<const char*>(k), static_cast<const char*>(v), static_cast<char*>(k_pages),
+               static_cast<char*>(v_pages), table, lens, seqs, k_stride_seq, k_stride_token, v_stride_seq,
+               v_stride_token, page_bytes, key_bytes, (int)n, (int)tokens, (int)slots, (int)width, (int)pages,
+               (int)page_size};
+  append_kernel<<<(unsigned)(n * tokens), 128, 0, stream>>>(a);
+  return kb::check_launch(name);
+}
+
+int kb_cache_free(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* seqs, int64_t n, int64_t slots,
+                  int64_t width, int64_t pages, kbStream stream) {
+  const char* name = "kb_cache_free";
+  using namespace kb::lm;
+  KB_CACHE_COMMON(n);
+  if (n == 0 || slots == 0) return KB_OK;
+  KB_REQUIRE(lens && seqs && (!width || table) && (!pages || refs), KB_ERR_INVALID_ARG, "%s: null pointer", name);
+  free_kernel<<<(unsigned)n, 256, 0, stream>>>(table, lens, refs, seqs, (int)slots, (int)width, (int)pages);
+  return kb::check_launch(name);
+}
+
+size_t kb_cache_compact_workspace_size(int64_t pages) {
+  return pages > 0 ? 3 * kb::lm::ints(pages) + 16 : 16;
+}
+
+int kb_cache_compact(void* pool, int32_t* table, int32_t* refs, int32_t* live, int64_t slots, int64_t width,
+                     int64_t planes, int64_t pages, int64_t page_bytes, void* workspace, size_t workspace_bytes,
+                     kbStream stream) {
+  const char* name = "kb_cache_compact";
+  using namespace kb::lm;
+  KB_CACHE_COMMON(0);
+  KB_REQUIRE(planes >= 0 && page_bytes >= 0, KB_ERR_INVALID_ARG, "%s: negative size", name);
+  KB_REQUIRE(live && (!pages || refs) && (!slots || !width || table), KB_ERR_INVALID_ARG, "%s: null pointer", name);
+  KB_REQUIRE(pool || !planes || !pages || !page_bytes, KB_ERR_INVALID_ARG, "%s: null pool", name);
+  KB_CACHE_WORKSPACE(kb_cache_compact_workspace_size(pages));
+  char* w = static_cast<char*>(workspace);
+  CompactArgs a{table, refs, live, slots * width, (int)pages, nullptr, nullptr, nullptr, nullptr};
+  a.count = reinterpret_cast<int*>(w);
+  a.src = reinterpret_cast<int*>(w + 16);
+  a.dst = reinterpret_cast<int*>(w + 16 + ints(pages));
+  a.map = reinterpret_cast<int*>(w + 16 + 2 * ints(pages));
+  compact_plan<<<1, kPlanThreads, 0, stream>>>(a);
+  if (int st = kb::check_launch(name)) return st;
+  if (pages == 0) return KB_OK;
+  if (a.entries) {
+    compact_table<<<copy_grid(kb::ceil_div(a.entries, 256)), 256, 0, stream>>>(a);
+    if (int st = kb::check_launch(name)) return st;
+  }
+  if (planes && page_bytes) {
+    copy_pages<<<copy_grid(pages * planes), 256, 0, stream>>>(static_cast<const char*>(pool), static_cast<char*>(pool),
+                                                              a.src, a.dst, a.count, (int)pages, planes, page_bytes,
+                                                              pages, pages);
+    return kb::check_launch(name);
+  }
+  return KB_OK;
+}
+
+int kb_cache_copy(const void* src_pool, const int32_t* src, void* dst_pool, const int32_t* dst, int64_t n,
+                  int64_t planes, int64_t page_bytes, int64_t src_pages, int64_t dst_pages, kbStream stream) {
+  const char* name = "kb_cache_copy";
+  using namespace kb::lm;
+  KB_REQUIRE(n >= 0 && planes >= 0 && page_bytes >= 0 && src_pages >= 0 && dst_pages >= 0, KB_ERR_INVALID_ARG,
+             "%s: negative size", name);
+  KB_REQUIRE(n <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many pages", name);
+  if (n == 0 || planes == 0 || page_bytes == 0 || src_pages == 0 || dst_pages == 0) return KB_OK;
+  KB_REQUIRE(src_pool && dst_pool && src && dst, KB_ERR_INVALID_ARG, "%s: null pointer", name);
+  copy_pages<<<copy_grid(n * planes), 256, 0, stream>>>(static_cast<const char*>(src_pool),
+                                                        static_cast<char*>(dst_pool), src, dst, nullptr, (int)n,
+                                                        planes, page_bytes, src_pages, dst_pages);
+  return kb::check_launch(name);
+}
+
+}  // extern "C"

@@ -1,0 +1,45 @@
+// lm_common.cuh — helpers shared by the language-model operators: element
+// types, 16-byte vectors of them, and page lookups.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "kb_common.cuh"
+
+namespace kb {
+namespace lm {
+
+template <typename T>
+__device__ __forceinline__ float to_f32(T v);
+template <>
+__device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// round to nearest even; the only rounding an output sees
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+inline int dtype_size(int dtype) { return dtype == KB_F32 ? 4 : (dtype == KB_F16 || dtype == KB_BF16) ? 2 : 0; }
+
+// Calls f with a null pointer of the element type that `dtype` names.
+template <typename F>
+int with_dtype(int dtype, F f) {
+  switch (dtype) {
+    case KB_F32: return f(static_cast<float*>(nullptr));
+    case KB_F16: return f(static_cast<__half*>(nullptr));
+    default: return f(static_cast<__nv_bfloat16*>(nullptr));
+  }
+}
+
+}  // namespace lm
+}  // namespace kb

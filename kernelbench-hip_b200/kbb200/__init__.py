@@ -3,9 +3,10 @@ candidate API.
 
     import kbb200
     y = kbb200.ops.gelu_tanh(x)          # tensor-level API
+    q, k = kbb200.lm.qk_norm_rope(...)   # language-model operators (fp32, fp16, bf16)
     kbb200.ext.mingpt_gelu_entry(x, y)   # candidate entry names (EXT.<ENTRY>)
 
-The submodules that launch kernels (`ops`, `ext`, `p2p`, `_lib`) load
+The submodules that launch kernels (`ops`, `lm`, `ext`, `p2p`, `_lib`) load
 libkbb200.so (C ABI, include/kbb200.h) when they are first imported, and
 `dist` when it first calls a kernel; they fail if it has not been built, and
 there is no other implementation to fall back to.  Importing the package
@@ -19,7 +20,7 @@ import importlib
 
 __version__ = "0.2.0"
 
-_SUBMODULES = {"_lib", "ops", "ext", "dist", "p2p", "workloads", "launch", "milestone_table"}
+_SUBMODULES = {"_lib", "ops", "lm", "ext", "dist", "p2p", "workloads", "launch", "milestone_table"}
 _FROM_LIB = {"LIB", "KbError", "LIB_PATH"}
 
 

@@ -87,6 +87,21 @@ SIGNATURES: dict[str, tuple] = {
                                               C.c_uint64, _p]),
     "kb_gemm_splitk_partials_workspace_size": (_sz, [_i64, _i64, _i64]),
     "kb_gemm_splitk_partials_3xtf32": (_int, [_p, _p, _i64, _i64, _i64, _p, _sz, C.POINTER(C.c_int), _p]),
+    "kb_qk_norm_rope": (_int, [_p] * 9 + [_i64] * 10 + [_int] * 4 + [_float, _p]),
+    "kb_qk_norm_rope_backward_workspace_size": (_sz, [_i64] * 4),
+    "kb_qk_norm_rope_backward": (_int, [_p] * 13 + [_i64] * 10 + [_int] * 4 + [_float, _p, _sz, _p]),
+    "kb_shared_prefix_attention_workspace_size": (_sz, [_i64] * 8 + [_int]),
+    "kb_shared_prefix_attention": (_int, [_p] * 8 + [_i64] * 18 + [_float, _int, _p, _sz, _p]),
+    "kb_cache_reserve_workspace_size": (_sz, [_i64] * 6),
+    "kb_cache_reserve": (_int, [_p] * 5 + [_i64] * 6 + [_p, _sz, _p]),
+    "kb_cache_append": (_int, [_p] * 7 + [_i64] * 12 + [_p]),
+    "kb_cache_fork_workspace_size": (_sz, [_i64] * 3),
+    "kb_cache_fork": (_int, [_p] * 7 + [_i64] * 7 + [_p, _sz, _p]),
+    "kb_cache_free": (_int, [_p] * 4 + [_i64] * 4 + [_p]),
+    "kb_cache_compact_workspace_size": (_sz, [_i64]),
+    "kb_cache_compact": (_int, [_p] * 4 + [_i64] * 5 + [_p, _sz, _p]),
+    "kb_cache_copy": (_int, [_p] * 4 + [_i64] * 5 + [_p]),
+    "kb_penalize_logits": (_int, [_p] * 10 + [_i64] * 7 + [_int] * 2 + [_p]),
 }
 
 
