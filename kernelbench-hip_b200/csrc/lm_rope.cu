@@ -14,9 +14,18 @@
 // kept from the forward pass.
 //
 // Statistics and products are fp32; outputs are rounded once.  dw is summed
-// in fp64 per warp, then over warps and CTAs in a fixed order, so it does not
-// depend on timing.  A position outside the table gives NaN in the rotated
-// elements.
+// in fp64 over warps and CTAs in a fixed order, so it does not depend on
+// timing.  A position outside the table gives NaN in the rotated elements.
+//
+// Both passes are bound by HBM (2 and 3 times the heads' bytes), so the work
+// is laid out to need no second look at an element and few shuffles: L lanes
+// hold one head vector, each lane four pairs (a, b), both elements of a pair
+// in the same lane.  With the half-split pairs that is four elements of the
+// first half and the four that they turn with, two 8-byte (16-bit types) or
+// 16-byte loads; interleaved, eight elements in a row.  The norm's sum is
+// log2(L) shuffles, the rotation none.  A warp takes kBatch x 32 / L heads of
+// one token, all loads issued before the first use, so cos and sin are read
+// once per token and warp.
 #include "lm_common.cuh"
 
 namespace kb {
@@ -38,8 +47,10 @@ struct RopeArgs {
   int64_t tokens, table_rows;
   int64_t stride_t[2], stride_h[2];
   int heads[2];
-  int dim, rotary, interleaved, pos64;
-  float eps;
+  int dim, rotary, interleaved, pos64, weight32, table_vec;
+  float eps, inv_dim;
+  int unit_heads;
+  uint32_t units_q, units_token;  // units of the queries, and in all, of one token
   double* partial;  // backward: [grid][2][dim]
 };
 
@@ -67,8 +78,340 @@ __device__ __forceinline__ float weight_at(const void* w, int e) {
   return w ? to_f32(static_cast<const W*>(w)[e]) : 1.0f;
 }
 
-// One warp per (token, head), the vector staged in shared memory: any dim up
-// to kMaxDim, any rotary size, any alignment and strides.
+constexpr int kVecDim = 256;   // heads up to here stay in registers
+constexpr int kVecThreads = 128, kVecWarps = kVecThreads / 32;
+constexpr int64_t kMaxUnits = 1ll << 31;
+constexpr int kFlush = 128;    // terms of a sum for dw in fp32 before it moves to fp64
+
+// Four elements as they lie in memory, 8 or 16 bytes.
+template <typename T>
+struct Raw4 {
+  uint2 v;
+  __device__ void set(int i, T x) { reinterpret_cast<T*>(&v)[i] = x; }
+};
+template <>
+struct Raw4<float> {
+  float4 v;
+  __device__ void set(int i, float x) { reinterpret_cast<float*>(&v)[i] = x; }
+};
+__device__ __forceinline__ void unpack(const Raw4<float>& r, float (&x)[4]) {
+  x[0] = r.v.x, x[1] = r.v.y, x[2] = r.v.z, x[3] = r.v.w;
+}
+__device__ __forceinline__ void unpack(const Raw4<__half>& r, float (&x)[4]) {
+  const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&r.v.x));
+  const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&r.v.y));
+  x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+}
+__device__ __forceinline__ void unpack(const Raw4<__nv_bfloat16>& r, float (&x)[4]) {
+  x[0] = __uint_as_float(r.v.x << 16), x[1] = __uint_as_float(r.v.x & 0xffff0000u);
+  x[2] = __uint_as_float(r.v.y << 16), x[3] = __uint_as_float(r.v.y & 0xffff0000u);
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store4(__half* p, const float (&v)[4]) {
+  const __half2 lo = __floats2half2_rn(v[0], v[1]), hi = __floats2half2_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&v)[4]) {
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+  *reinterpret_cast<uint2*>(p) =
+      make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+}
+// A lane's part of a head vector, unconverted (loads in flight hold few registers).
+template <typename T>
+struct Raw8 {
+  Raw4<T> a, b;
+};
+
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// How a lane's pairs lie in memory: two vectors of four whose elements turn
+// with each other; eight elements in a row, each turning with its neighbour;
+// or element by element, for any size and alignment.
+enum Layout { kHalves, kNeighbours, kAny };
+
+// The four pairs of lane `l` of a head vector: pair p = 4 l + j turns when
+// p < rotary / 2.
+template <int LAYOUT>
+struct Pairs {
+  int first, half, dim, off_a, off_b, interleaved;
+  bool on;  // this lane holds elements of the head
+  __device__ Pairs(const RopeArgs& a, int l) {
+    first = 4 * l;
+    half = a.rotary >> 1;
+    dim = a.dim;
+    interleaved = a.interleaved;
+    on = 8 * l < dim;
+    off_a = LAYOUT == kNeighbours ? 8 * l : first < half ? first : a.rotary + 2 * (first - half);
+    off_b = LAYOUT == kNeighbours ? 8 * l + 4 : first < half ? first + half : off_a + 4;
+  }
+  // the elements of pair p; b is dim or more where there is none
+  __device__ int ea(int p) const { return interleaved ? 2 * p : p < half ? p : 2 * p; }
+  __device__ int eb(int p) const { return interleaved ? 2 * p + 1 : p < half ? p + half : 2 * p + 1; }
+  __device__ bool turns(int j) const {  // with kHalves a lane turns all its pairs or none
+    return LAYOUT == kHalves ? first < half : first + j < half;
+  }
+  template <typename T>
+  __device__ void fetch(const T* x, Raw8<T>& r) const {
+    if (LAYOUT != kAny) {
+      r.a = *reinterpret_cast<const Raw4<T>*>(x + off_a);
+      r.b = *reinterpret_cast<const Raw4<T>*>(x + off_b);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = ea(first + j), k = eb(first + j);
+        r.a.set(j, i < dim ? x[i] : from_f32<T>(0.0f));
+        r.b.set(j, k < dim ? x[k] : from_f32<T>(0.0f));
+      }
+    }
+  }
+  template <typename T>
+  __device__ void get(const Raw8<T>& r, float (&a)[4], float (&b)[4]) const {
+    unpack(r.a, a);
+    unpack(r.b, b);
+    if (LAYOUT == kNeighbours) {
+      const float t0 = a[1], t1 = a[3];
+      a[1] = a[2], a[2] = b[0], a[3] = b[2];
+      b[0] = t0, b[2] = b[1], b[1] = t1;
+    }
+  }
+  template <typename T>
+  __device__ void store(T* x, float (&a)[4], float (&b)[4]) const {
+    if (LAYOUT == kNeighbours) {
+      const float lo[4] = {a[0], b[0], a[1], b[1]}, hi[4] = {a[2], b[2], a[3], b[3]};
+      store4(x + off_a, lo);
+      store4(x + off_b, hi);
+    } else if (LAYOUT == kHalves) {
+      store4(x + off_a, a);
+      store4(x + off_b, b);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = ea(first + j), k = eb(first + j);
+        if (i < dim) x[i] = from_f32<T>(a[j]);
+        if (k < dim) x[k] = from_f32<T>(b[j]);
+      }
+    }
+  }
+  // cos and sin of the four pairs at token t; 1 and 0 where a pair does not turn
+  __device__ void table(const RopeArgs& a, int64_t t, float (&c)[4], float (&s)[4]) const {
+    const int64_t p = position(a, t);
+    const bool inside = p >= 0 && p < a.table_rows;
+    const float nan = __int_as_float(0x7fc00000);
+    const float *ct = a.cos_t + (inside ? p : 0) * half + first, *st = a.sin_t + (inside ? p : 0) * half + first;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c[j] = 1.0f, s[j] = 0.0f;
+    if (!inside) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (turns(j)) c[j] = s[j] = nan;
+    } else if (a.table_vec) {  // rows of whole vectors: a lane turns all its pairs or none
+      if (first < half) {
+        unpack(*reinterpret_cast<const Raw4<float>*>(ct), c);
+        unpack(*reinterpret_cast<const Raw4<float>*>(st), s);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (turns(j)) c[j] = ct[j], s[j] = st[j];
+    }
+  }
+  template <typename T>
+  __device__ void weights(const void* w, int w32, float (&a)[4], float (&b)[4]) const {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a[j] = b[j] = 1.0f;
+    if (!w || !on) return;
+    if (w32) {
+      Raw8<float> r;
+      fetch(static_cast<const float*>(w), r);
+      get(r, a, b);
+    } else {
+      Raw8<T> r;
+      fetch(static_cast<const T*>(w), r);
+      get(r, a, b);
+    }
+  }
+  // the element that slot i holds: a[i], then b[i - 4]
+  __device__ int element(int i) const {
+    const int j = i & 3;
+    if (LAYOUT == kHalves) return (i < 4 ? off_a : off_b) + j;
+    return i < 4 ? ea(first + j) : eb(first + j);
+  }
+};
+
+// A unit of work: a.unit_heads heads of one token, of its queries or keys.
+template <typename T, int L, int LAYOUT>
+__global__ void __launch_bounds__(kVecThreads, 8) rope_forward(RopeArgs a, uint32_t units) {
+  constexpr int kGroups = 32 / L, kBatch = sizeof(T) == 2 ? 4 : 2;
+  const uint32_t id = blockIdx.x * kVecWarps + (threadIdx.x >> 5);
+  if (id >= units) return;
+  const int lane = threadIdx.x & 31, group = lane / L;
+  const Pairs<LAYOUT> pr(a, lane % L);
+  const uint32_t t = id / a.units_token, i = id - t * a.units_token;
+  const int which = i >= a.units_q;
+  const int heads = a.heads[which];
+  const int64_t stride = a.stride_h[which];
+  int h = (int)(which ? i - a.units_q : i) * a.unit_heads + group;
+  const int last = min(h - group + a.unit_heads, heads);
+  const T* x = static_cast<const T*>(a.x[which]) + (int64_t)t * a.stride_t[which];
+  T* z = static_cast<T*>(a.out[which]) + (int64_t)t * heads * a.dim;
+  // z_a = r (x_a aa - x_b ab), z_b = r (x_b bb + x_a ba): the weights times cos and sin
+  float aa[4], ab[4], bb[4], ba[4];
+  bool ready = false;
+  for (; h - group < last; h += kBatch * kGroups) {
+    Raw8<T> xr[kBatch] = {};
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (h + k * kGroups < last && pr.on) pr.fetch(x + (h + k * kGroups) * stride, xr[k]);
+    if (!ready) {  // while the first heads are on their way
+      float c[4], s[4], wa[4], wb[4];
+      pr.table(a, t, c, s);
+      pr.template weights<T>(a.w[which], a.weight32, wa, wb);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) aa[j] = wa[j] * c[j], ab[j] = wb[j] * s[j], bb[j] = wb[j] * c[j], ba[j] = wa[j] * s[j];
+      ready = true;
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int at = h + k * kGroups;
+      if (at - group >= last) break;
+      float xa[4], xb[4], ss = 0.0f;
+      pr.get(xr[k], xa, xb);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ss += xa[j] * xa[j] + xb[j] * xb[j];
+      const float r = rsqrtf(group_sum<L>(ss) * a.inv_dim + a.eps);
+      float za[4], zb[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        za[j] = xa[j] * aa[j];
+        zb[j] = xb[j] * bb[j];
+        if (pr.turns(j)) {  // not a product with 0: the partner may be infinite
+          za[j] -= xb[j] * ab[j];
+          zb[j] += xa[j] * ba[j];
+        }
+        za[j] *= r;
+        zb[j] *= r;
+      }
+      if (at < last && pr.on) pr.store(z + at * a.dim, za, zb);
+    }
+  }
+}
+
+// Persistent: warps walk the units of the queries, then those of the keys,
+// with their sums for dw in registers, moved to fp64 in shared memory often
+// enough that no fp32 sum runs over more than kFlush terms.
+template <typename T, int L, int LAYOUT>
+__global__ void __launch_bounds__(kVecThreads, 4) rope_backward(RopeArgs a) {
+  constexpr int kGroups = 32 / L, kBatch = 2;
+  __shared__ double acc[kVecWarps][16][32];  // [warp][which * 8 + a0..3 b0..3][lane]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / L;
+  const Pairs<LAYOUT> pr(a, lane % L);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) acc[warp][i][lane] = 0.0;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const int heads = a.heads[which];
+    const int64_t stride = a.stride_h[which];
+    const uint32_t per_token = which ? a.units_token - a.units_q : a.units_q;
+    const uint32_t units = (uint32_t)a.tokens * per_token;
+    float wa[4], wb[4], ga[4] = {}, gb[4] = {};
+    pr.template weights<T>(a.w[which], a.weight32, wa, wb);
+    int terms = 0;
+    auto flush = [&] {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        acc[warp][which * 8 + j][lane] += (double)ga[j];
+        acc[warp][which * 8 + 4 + j][lane] += (double)gb[j];
+        ga[j] = gb[j] = 0.0f;
+      }
+      terms = 0;
+    };
+    for (uint32_t id = blockIdx.x * kVecWarps + warp; id < units; id += gridDim.x * kVecWarps) {
+      const uint32_t t = id / per_token;
+      int h = (int)(id - t * per_token) * a.unit_heads + group;
+      const int last = min(h - group + a.unit_heads, heads);
+      const T* x = static_cast<const T*>(a.x[which]) + (int64_t)t * a.stride_t[which];
+      const T* dz = static_cast<const T*>(a.dz[which]) + (int64_t)t * heads * a.dim;
+      T* dx = static_cast<T*>(a.out[which]) + (int64_t)t * heads * a.dim;
+      float c[4], s[4];
+      Raw8<T> xr[kBatch] = {}, dr[kBatch] = {};
+      auto fetch = [&](int k, int at) {
+        if (at < last && pr.on) {
+          pr.fetch(x + at * stride, xr[k]);
+          pr.fetch(dz + at * a.dim, dr[k]);
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) fetch(k, h + k * kGroups);
+      pr.table(a, t, c, s);
+      for (; h - group < last; h += kBatch * kGroups) {
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int at = h + k * kGroups;
+          if (at - group >= last) break;
+          float xa[4], xb[4], da[4], db[4], ya[4], yb[4], ss = 0.0f, dot = 0.0f;
+          pr.get(xr[k], xa, xb);
+          pr.get(dr[k], da, db);
+          fetch(k, at + kBatch * kGroups);  // the head that takes this one's place
+          float ta[4], tb[4];  // dy x
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            ya[j] = da[j] * c[j];
+            yb[j] = db[j] * c[j];
+            if (pr.turns(j)) {
+              ya[j] += db[j] * s[j];
+              yb[j] -= da[j] * s[j];
+            }
+            ta[j] = ya[j] * xa[j];
+            tb[j] = yb[j] * xb[j];
+            ss += xa[j] * xa[j] + xb[j] * xb[j];
+            dot += ta[j] * wa[j] + tb[j] * wb[j];
+          }
+#pragma unroll
+          for (int o = L / 2; o > 0; o >>= 1) {
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            dot += __shfl_xor_sync(0xffffffffu, dot, o);
+          }
+          const float r = rsqrtf(ss * a.inv_dim + a.eps);
+          const float m = r * dot * a.inv_dim * r;  // r mean(dy w xh)
+          const bool mine = at < last && pr.on;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if (mine) {
+              ga[j] += ta[j] * r;
+              gb[j] += tb[j] * r;
+            }
+            ya[j] = r * (ya[j] * wa[j] - xa[j] * m);
+            yb[j] = r * (yb[j] * wb[j] - xb[j] * m);
+          }
+          if (mine) pr.store(dx + at * a.dim, ya, yb);
+        }
+        if (++terms == kFlush / kBatch) flush();
+      }
+    }
+    flush();
+  }
+  __syncthreads();
+  // element e of weight `which`: over warps and groups of lanes, in order
+  for (int i = threadIdx.x; i < 16 * L; i += kVecThreads) {
+    const int slot = i / L, of = i % L;
+    double sum = 0.0;
+    for (int w = 0; w < kVecWarps; ++w)
+      for (int g = 0; g < kGroups; ++g) sum += acc[w][slot][g * L + of];
+    const int e = Pairs<LAYOUT>(a, of).element(slot & 7);
+    if (e < a.dim) a.partial[(int64_t)blockIdx.x * 2 * a.dim + (slot >> 3) * a.dim + e] = sum;
+  }
+}
+
+// Heads larger than kVecDim: one warp per (token, head), the vector staged in
+// shared memory.
 template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads) rope_forward_any(RopeArgs a) {
   extern __shared__ float smem[];
@@ -175,22 +518,62 @@ __global__ void __launch_bounds__(kThreads) rope_backward_any(RopeArgs a) {
 template <typename W>
 __global__ void rope_weight_grads(const double* __restrict__ partial, int parts, int dim, W* __restrict__ dqw,
                                   W* __restrict__ dkw) {
-  __shared__ double red[8][33];
-  const int lane = threadIdx.x, row = threadIdx.y;  // 32 x 8: a column of the partials per lane
+  __shared__ double red[32][33];
+  const int lane = threadIdx.x, row = threadIdx.y;  // 32 x 32: a column of the partials per lane
   const int e = blockIdx.x * 32 + lane;
   double s = 0.0;
   if (e < 2 * dim)
-    for (int i = row; i < parts; i += 8) s += partial[(int64_t)i * 2 * dim + e];
+    for (int i = row; i < parts; i += 32) s += partial[(int64_t)i * 2 * dim + e];
   red[row][lane] = s;
   __syncthreads();
   if (row || e >= 2 * dim) return;
-  for (int i = 1; i < 8; ++i) s += red[i][lane];
+  for (int i = 1; i < 32; ++i) s += red[i][lane];
   W* out = e < dim ? dqw : dkw;
   if (out) out[e < dim ? e : e - dim] = from_f32<W>((float)s);
 }
 
 int backward_grid(int64_t tokens, int heads) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(tokens * heads, kWarps), (int64_t)sm_count() * 4));
+}
+
+// Lanes per head: the power of two that holds dim / 8 of them.
+int lanes_for(int64_t dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
+// Fills in the layout of the register kernels; returns the units of work.  A
+// unit takes up to 16 heads per group of lanes (cos, sin and weights are
+// prepared once for them), fewer while that leaves SMs without work.
+int64_t lay_out(RopeArgs& a) {
+  const int step = 32 / lanes_for(a.dim) * 4;
+  auto units = [&](int64_t heads) { return ceil_div(a.heads[0], heads) + ceil_div(a.heads[1], heads); };
+  a.unit_heads = step * 4;
+  while (a.unit_heads > step && a.tokens * units(a.unit_heads) < (int64_t)sm_count() * 64) a.unit_heads /= 2;
+  a.units_q = (uint32_t)ceil_div(a.heads[0], a.unit_heads);
+  a.units_token = (uint32_t)units(a.unit_heads);
+  a.inv_dim = 1.0f / (float)a.dim;
+  a.table_vec = a.rotary % 8 == 0 && aligned16(a.cos_t) && aligned16(a.sin_t);
+  return a.tokens * a.units_token;
+}
+// Whether a lane's elements can be read as vectors of four.
+bool vector_ok(const RopeArgs& a, int e, bool backward) {
+  auto whole = [&](const void* p) { return p == nullptr || reinterpret_cast<uintptr_t>(p) % (4 * e) == 0; };
+  if (a.dim % 8 || (!a.interleaved && a.rotary % 8)) return false;
+  for (int i = 0; i < 2; ++i) {
+    if (a.stride_t[i] % 4 || a.stride_h[i] % 4 || !whole(a.x[i]) || !whole(a.out[i]) || !aligned16(a.w[i])) return false;
+    if (backward && !whole(a.dz[i])) return false;
+  }
+  return true;
+}
+// f(lanes per head, layout): both as types that hold a constant
+template <typename F>
+int with_layout(const RopeArgs& a, bool vec, F f) {
+  auto lanes = [&](auto layout) {
+    const int l = lanes_for(a.dim);
+    if (l == 8) return f(std::integral_constant<int, 8>{}, layout);
+    if (l == 16) return f(std::integral_constant<int, 16>{}, layout);
+    return f(std::integral_constant<int, 32>{}, layout);
+  };
+  if (!vec) return lanes(std::integral_constant<int, kAny>{});
+  if (a.interleaved) return lanes(std::integral_constant<int, kNeighbours>{});
+  return lanes(std::integral_constant<int, kHalves>{});
 }
 
 int check_shape(const char* name, int64_t tokens, int64_t heads_q, int64_t heads_kv, int64_t dim, int64_t rotary,
@@ -244,6 +627,18 @@ int kb_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
   a.stride_h[0] = q_stride_head, a.stride_h[1] = k_stride_head;
   a.heads[0] = (int)heads_q, a.heads[1] = (int)heads_kv;
   a.dim = (int)dim, a.rotary = (int)rotary, a.interleaved = interleaved, a.pos64 = positions_64, a.eps = eps;
+  a.weight32 = weight_dtype == KB_F32;
+  if (dim <= kVecDim) {
+    const int64_t units = lay_out(a), blocks = kb::ceil_div(units, kVecWarps);
+    KB_REQUIRE(units <= kMaxUnits, KB_ERR_UNSUPPORTED, "%s: too many tokens", name);
+    return with_dtype(dtype, [&](auto* x) {
+      using T = std::remove_pointer_t<decltype(x)>;
+      return with_layout(a, vector_ok(a, sizeof(T), false), [&](auto l, auto v) {
+        rope_forward<T, decltype(l)::value, decltype(v)::value><<<(unsigned)blocks, kVecThreads, 0, stream>>>(a, (uint32_t)units);
+        return kb::check_launch(name);
+      });
+    });
+  }
   const int64_t items = tokens * (heads_q + heads_kv);
   const unsigned grid = (unsigned)std::min<int64_t>(kb::ceil_div(items, kWarps), (int64_t)kb::sm_count() * 16);
   return with_types(dtype, weight_dtype, [&](auto* x, auto* w) {
@@ -294,17 +689,27 @@ int kb_qk_norm_rope_backward(const void* dq_out, const void* dk_out, const void*
   a.stride_h[0] = q_stride_head, a.stride_h[1] = k_stride_head;
   a.heads[0] = (int)heads_q, a.heads[1] = (int)heads_kv;
   a.dim = (int)dim, a.rotary = (int)rotary, a.interleaved = interleaved, a.pos64 = positions_64, a.eps = eps;
+  a.weight32 = weight_dtype == KB_F32;
   a.partial = partial;
   return with_types(dtype, weight_dtype, [&](auto* x, auto* w) {
     using T = std::remove_pointer_t<decltype(x)>;
     using W = std::remove_pointer_t<decltype(w)>;
-    if (any) {
+    if (any && dim <= kVecDim) {
+      const int64_t units = lay_out(a);
+      KB_REQUIRE(units <= kMaxUnits, KB_ERR_UNSUPPORTED, "%s: too many tokens", name);
+      grid = (int)std::min<int64_t>(kb::ceil_div(units, kVecWarps), (int64_t)kb::sm_count() * 4);  // four per SM
+      if (int st = with_layout(a, vector_ok(a, sizeof(T), true), [&](auto l, auto v) {
+            rope_backward<T, decltype(l)::value, decltype(v)::value><<<grid, kVecThreads, 0, stream>>>(a);
+            return kb::check_launch(name);
+          }))
+        return st;
+    } else if (any) {
       const size_t smem = (size_t)kWarps * dim * (2 * sizeof(double) + sizeof(float));
       rope_backward_any<T, W><<<grid, kThreads, smem, stream>>>(a);
       if (int st = kb::check_launch(name)) return st;
     }
     if (!dq_weight && !dk_weight) return (int)KB_OK;
-    rope_weight_grads<W><<<(unsigned)kb::ceil_div(2 * dim, 32), dim3(32, 8), 0, stream>>>(
+    rope_weight_grads<W><<<(unsigned)kb::ceil_div(2 * dim, 32), dim3(32, 32), 0, stream>>>(
         partial, grid, (int)dim, static_cast<W*>(dq_weight), static_cast<W*>(dk_weight));
     return kb::check_launch(name);
   });
