@@ -54,12 +54,12 @@ struct AttnArgs {
   float* lse;
   const int *prefix, *table, *lens;
   int batch, queries, heads_q, heads_kv, group, dim;
-  int prefix_pages, width, pages, page_size;
+  int prefix_pages, width, pages, page_size, page_shift;  // page_shift: its logarithm, or -1
   int64_t q_b, q_t, q_h, k_p, k_s, k_h, v_p, v_s, v_h;  // strides in elements
   float scale_log2;                                      // scale * log2(e)
   int prefix_tiles, prefix_splits, prefix_chunk;         // row tiles per key head; ranges and keys per range
   int own_tiles, own_splits, own_chunk;
-  int64_t prefix_items;
+  int64_t prefix_items, first_item;                      // items of the prefix come first; the launch's first one
   float *part_o, *part_lse;  // [splits][batch * queries * heads_q][dim], [splits][rows]; null: one range only
 };
 
@@ -146,13 +146,16 @@ __device__ __forceinline__ Split split(float x) {
   const float lo = x - __uint_as_float(hi);
   return {hi, isfinite(lo) ? __float_as_uint(lo) : 0u};
 }
-// c += A B to fp32 accuracy: lo hi + hi lo + hi hi.
-__device__ __forceinline__ void mma_3xtf32(float (&c)[4], const Split (&a)[4], Split b0, Split b1) {
+// hh += A_hi B_hi, x += A_lo B_hi + A_hi B_lo; the sum is A B to fp32 accuracy.
+// The tensor cores' accumulation truncates, so chains are kept short and the
+// small cross terms apart; the callers add with rounding.
+__device__ __forceinline__ void mma_3xtf32(float (&hh)[4], float (&x)[4], const Split (&a)[4], Split b0, Split b1) {
   const uint32_t ah[4] = {a[0].hi, a[1].hi, a[2].hi, a[3].hi}, al[4] = {a[0].lo, a[1].lo, a[2].lo, a[3].lo};
-  mma_tf32(c, al, b0.hi, b1.hi);
-  mma_tf32(c, ah, b0.lo, b1.lo);
-  mma_tf32(c, ah, b0.hi, b1.hi);
+  mma_tf32(x, al, b0.hi, b1.hi);
+  mma_tf32(x, ah, b0.lo, b1.lo);
+  mma_tf32(hh, ah, b0.hi, b1.hi);
 }
+constexpr int kChain = 4;  // products of depth 8 chained in one accumulator
 __device__ __forceinline__ uint32_t pack2(float x, float y, __half*) {
   const __half2 h = __floats2half2_rn(x, y);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -172,13 +175,25 @@ __device__ __forceinline__ void scores(float (&s)[NK / 8][4], const T* q, const 
     for (int i = 0; i < 4; ++i) s[n][i] = 0.0f;
   if constexpr (std::is_same_v<T, float>) {
     const int r = lane >> 2, c = lane & 3;
-#pragma unroll 4
-    for (int d = 0; d < DP; d += 8) {
-      const Split qa[4] = {split(q[r * LD + d + c]), split(q[(r + 8) * LD + d + c]), split(q[r * LD + d + c + 4]),
-                           split(q[(r + 8) * LD + d + c + 4])};
+#pragma unroll 1
+    for (int d0 = 0; d0 < DP; d0 += 8 * kChain) {
+      Split qa[kChain][4];
 #pragma unroll
-      for (int n = 0; n < NK / 8; ++n)
-        mma_3xtf32(s[n], qa, split(k[(n * 8 + r) * LD + d + c]), split(k[(n * 8 + r) * LD + d + c + 4]));
+      for (int i = 0; i < kChain; ++i) {
+        const float* x = q + r * LD + d0 + 8 * i + c;
+        qa[i][0] = split(x[0]), qa[i][1] = split(x[8 * LD]), qa[i][2] = split(x[4]), qa[i][3] = split(x[8 * LD + 4]);
+      }
+#pragma unroll
+      for (int n = 0; n < NK / 8; ++n) {
+        float hh[4] = {}, x[4] = {};
+#pragma unroll
+        for (int i = 0; i < kChain; ++i) {
+          const float* y = k + (n * 8 + r) * LD + d0 + 8 * i + c;
+          mma_3xtf32(hh, x, qa[i], split(y[0]), split(y[4]));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][i] += hh[i] + x[i];
+      }
     }
   } else {
     const uint32_t qrow = smem_addr(q + (lane & 15) * LD + (lane >> 4) * 8);
@@ -204,13 +219,27 @@ template <typename T, int DP, int NK, int LD>
 __device__ __forceinline__ void weigh(float (&o)[DP / 8][4], const float (&p)[NK / 8][4], const T* v, int lane) {
   if constexpr (std::is_same_v<T, float>) {
     const int r = lane >> 2, c = lane & 3;
+    constexpr int kKeys = NK / 8 < kChain ? NK / 8 : kChain;
 #pragma unroll
-    for (int n = 0; n < NK / 8; ++n) {
-      // the order of keys within a product is free: slot c holds key 2c, slot c + 4 key 2c + 1, as P's registers do
-      const Split pa[4] = {split(p[n][0]), split(p[n][2]), split(p[n][1]), split(p[n][3])};
+    for (int n0 = 0; n0 < NK / 8; n0 += kKeys) {
+      // the order of keys within a product is free: slot c holds key 2c, slot c + 4 key 2c + 1, as p's registers do
+      Split pa[kKeys][4];
 #pragma unroll
-      for (int d = 0; d < DP / 8; ++d)
-        mma_3xtf32(o[d], pa, split(v[(n * 8 + 2 * c) * LD + d * 8 + r]), split(v[(n * 8 + 2 * c + 1) * LD + d * 8 + r]));
+      for (int i = 0; i < kKeys; ++i) {
+        const float(&x)[4] = p[n0 + i];
+        pa[i][0] = split(x[0]), pa[i][1] = split(x[2]), pa[i][2] = split(x[1]), pa[i][3] = split(x[3]);
+      }
+#pragma unroll
+      for (int d = 0; d < DP / 8; ++d) {
+        float hh[4] = {}, x[4] = {};
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i) {
+          const float* y = v + ((n0 + i) * 8 + 2 * c) * LD + d * 8 + r;
+          mma_3xtf32(hh, x, pa[i], split(y[0]), split(y[LD]));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d][i] += hh[i] + x[i];
+      }
     }
   } else {
     const uint32_t vrow = smem_addr(v + ((lane & 7) + ((lane >> 3) & 1) * 8) * LD + (lane >> 4) * 8);
@@ -292,8 +321,9 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
   T* sk = sq + C::kRows * LD;
   T* sv = sk + 2 * NK * LD;
   __shared__ int s_max[4];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Item w = item_at(a, blockIdx.x, C::kRows);
+  const Item w = item_at(a, a.first_item + blockIdx.x, C::kRows);
   const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
 
   // this thread's two rows
@@ -331,7 +361,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
       int64_t page = 0;
       int slot = 0;
       if (in) {
-        const int pj = j / a.page_size;
+        const int pj = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
         slot = j - pj * a.page_size;
         page = min(max(w.pages[pj], 0), a.pages - 1);
       }
@@ -402,86 +432,304 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
   }
 }
 
+// ------------------------------------------------------------------ keys kernel
+// Up to 16 rows: each of four warps takes every fourth block of NK keys, with
+// a ring of its own filled by cp.async (no barrier until the end), and its own
+// running softmax; the four are joined in shared memory.  This is the shape of
+// decoding: a few query heads per key head against a sequence's own keys,
+// bound by the bytes of the cache.
+template <typename T, int DP, int NK, int STAGES>
+struct KeysCfg {
+  static constexpr int kRows = 16, kWarps = 4, kThreads = 128;
+  static constexpr int LD = DP + 16 / (int)sizeof(T);
+  static constexpr int kStage = 2 * NK * LD;  // elements: keys, values
+  static constexpr size_t kRing = sizeof(T) * kWarps * STAGES * kStage;
+  static constexpr size_t kJoin = sizeof(float) * kWarps * kRows * (DP + 4);
+  static constexpr size_t kSmem = sizeof(T) * kRows * LD + (kRing > kJoin ? kRing : kJoin);
+};
+
+template <typename T, int DP, int NK, int STAGES>
+__global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
+  using C = KeysCfg<T, DP, NK, STAGES>;
+  constexpr int LD = C::LD, kVec = 16 / sizeof(T), kPerRow = DP / kVec;
+  extern __shared__ __align__(16) uint8_t raw[];
+  T* sq = reinterpret_cast<T*>(raw);
+  T* ring = sq + C::kRows * LD;
+  __shared__ float s_m[4][16], s_l[4][16];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const Item w = item_at(a, a.first_item + blockIdx.x, C::kRows);
+  const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
+  const int row[2] = {lane >> 2, (lane >> 2) + 8};
+  int vis[2], top = 0, low = 0x7fffffff;
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    vis[r] = row[r] < w.rows ? visible(a, w.base + (w.row0 + row[r]) / a.group) : 0;
+    top = max(top, vis[r]);
+    if (row[r] < w.rows) low = min(low, vis[r]);
+  }
+  const int end = min(w.k1, __reduce_max_sync(0xffffffffu, top));
+  low = __reduce_min_sync(0xffffffffu, low);
+
+  const T* kp = static_cast<const T*>(a.k) + w.h * a.k_h;
+  const T* vp = static_cast<const T*>(a.v) + w.h * a.v_h;
+  T* mine = ring + warp * STAGES * C::kStage;
+  // Where this lane's key of the block at key0 lies (lanes past NK repeat):
+  // looked up once per key, a block before its copies are issued.
+  const bool alike = a.k_p == a.v_p && a.k_s == a.v_s;
+  struct Place {
+    int64_t k, v;
+  };
+  auto place = [&](int key0) {
+    const int j = key0 + lane % NK;
+    Place p{0, 0};
+    if (j < end) {
+      const int pj = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+      const int slot = j - pj * a.page_size;
+      const int64_t page = min(max(w.pages[pj], 0), a.pages - 1);
+      p.k = page * a.k_p + slot * a.k_s;
+      p.v = alike ? p.k : page * a.v_p + slot * a.v_s;
+    }
+    return p;
+  };
+  auto load = [&](int key0, const Place& p, int stage) {
+    T* sk = mine + stage * C::kStage;
+    T* sv = sk + NK * LD;
+#pragma unroll
+    for (int i = 0; i < NK * kPerRow / 32; ++i) {
+      const int at = i * 32 + lane, n = at / kPerRow, c = at % kPerRow * kVec;
+      const int64_t k = __shfl_sync(0xffffffffu, p.k, n);
+      const int64_t v = alike ? k : __shfl_sync(0xffffffffu, p.v, n);
+      const bool in = key0 + n < end && c < a.dim;
+      const int cc = in ? c : 0;
+      cp_async16(sk + n * LD + c, kp + k + cc, in);
+      cp_async16(sv + n * LD + c, vp + v + cc, in);
+    }
+  };
+  constexpr int kStep = C::kWarps * NK;
+  const int begin = w.k0 + warp * NK;
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    if (begin + i * kStep < end) load(begin + i * kStep, place(begin + i * kStep), i);
+    cp_async_commit();
+  }
+  Place next = place(begin + (STAGES - 1) * kStep);
+  // the queries, while the first keys are on their way
+  for (int i = tid; i < C::kRows * kPerRow; i += C::kThreads) {
+    const int r = i / kPerRow, c = (i - r * kPerRow) * kVec;
+    uint4 x = make_uint4(0, 0, 0, 0);
+    if (r < w.rows && c < a.dim) {
+      const int rr = w.row0 + r, bt = w.base + rr / a.group;
+      x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(bt / a.queries) * a.q_b +
+                                          (int64_t)(bt % a.queries) * a.q_t +
+                                          (int64_t)(w.h * a.group + rr % a.group) * a.q_h + c);
+    }
+    *reinterpret_cast<uint4*>(sq + r * LD + c) = x;
+  }
+  __syncthreads();
+
+  float o[DP / 8][4];
+#pragma unroll
+  for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[d][i] = 0.0f;
+  Running st{{-INFINITY, -INFINITY}, {0.0f, 0.0f}};
+  const int seen[2] = {min(vis[0], end), min(vis[1], end)};
+  int stage = 0;
+  for (int key0 = begin; key0 < end; key0 += kStep) {
+    const int ahead = key0 + (STAGES - 1) * kStep;
+    if (ahead < end) load(ahead, next, stage == 0 ? STAGES - 1 : stage - 1);
+    cp_async_commit();
+    next = place(ahead + kStep);
+    cp_async_wait<STAGES - 1>();
+    __syncwarp();
+    const T* sk = mine + stage * C::kStage;
+    float s[NK / 8][4];
+    scores<T, DP, NK, LD>(s, sq, sk, lane);
+    softmax_step<NK, DP / 8>(s, o, st, a.scale_log2, key0, seen, key0 + NK > min(low, end), lane);
+    weigh<T, DP, NK, LD>(o, s, sk + NK * LD, lane);
+    __syncwarp();  // all lanes are done with the stage that the next load fills
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 1);
+    st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 2);
+    if ((lane & 3) == 0) s_m[warp][row[r]] = st.m[r], s_l[warp][row[r]] = st.l[r];
+  }
+  __syncthreads();  // the rings are free
+  float* so = reinterpret_cast<float*>(ring);
+  constexpr int LO = DP + 4;
+#pragma unroll
+  for (int d = 0; d < DP / 8; ++d)
+#pragma unroll
+    for (int r = 0; r < 2; ++r)
+      *reinterpret_cast<float2*>(so + (warp * 16 + row[r]) * LO + d * 8 + (lane & 3) * 2) =
+          make_float2(o[d][2 * r], o[d][2 * r + 1]);
+  __syncthreads();
+  // eight threads a row
+  const int r = tid >> 3;
+  if (r >= w.rows) return;
+  float m = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+  const float base = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f, f[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[i] = ex2(s_m[i][r] - base);
+    l += f[i] * s_l[i][r];
+  }
+  const int rr = w.row0 + r;
+  const int64_t at = (int64_t)(w.base + rr / a.group) * a.heads_q + w.h * a.group + rr % a.group;
+  const int64_t slot = (int64_t)w.split * n_rows + at;
+  const bool none = l == 0.0f;
+  const float inv = none ? 0.0f : 1.0f / l;
+  const float lse = none ? -INFINITY : m * kLn2 + logf(l);
+  if ((tid & 7) == 0) (a.part_o ? a.part_lse[slot] : a.lse[at]) = lse;
+  if (a.part_o && none) return;  // the join does not read it
+  for (int d = (tid & 7) * 4; d < a.dim; d += 32) {
+    float y[4] = {};
+    if (!none) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (f[i] == 0.0f) continue;  // a warp without keys
+        const float4 x = *reinterpret_cast<const float4*>(so + (i * 16 + r) * LO + d);
+        y[0] += f[i] * x.x, y[1] += f[i] * x.y, y[2] += f[i] * x.z, y[3] += f[i] * x.w;
+      }
+    }
+    if (a.part_o) {
+      *reinterpret_cast<float4*>(a.part_o + slot * a.dim + d) = make_float4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv);
+    } else {
+      T* z = static_cast<T*>(a.out) + at * a.dim + d;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) z[i] = from_f32<T>(y[i] * inv);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ join
-// One warp per row: the parts weighed by exp(lse_i - L), in their order.
+// One warp per row: the parts weighed by exp(lse_i - L), in their order.  Lane
+// i holds the weight of part i; a part without keys has weight 0 and is not
+// read (nothing was written there).
 template <typename T>
 __global__ void __launch_bounds__(128) attn_join_kernel(const float* __restrict__ part_o,
                                                         const float* __restrict__ part_lse, int splits, int64_t rows,
                                                         int dim, T* __restrict__ out, float* __restrict__ lse) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= rows) return;
   const int lane = threadIdx.x & 31;
-  float top = -INFINITY;
-  for (int i = lane; i < splits; i += 32) top = fmaxf(top, part_lse[i * rows + row]);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the parts
+  if (row >= rows) return;
+  const float first = lane < splits ? part_lse[lane * rows + row] : -INFINITY;
+  float top = first;
+  for (int i = lane + 32; i < splits; i += 32) top = fmaxf(top, part_lse[i * rows + row]);
   top = warp_max(top);
   const float base = top == -INFINITY ? 0.0f : top;
   float total = 0.0f;  // a NaN part makes it NaN
-  for (int i = lane; i < splits; i += 32) total += ex2((part_lse[i * rows + row] - base) * kLog2e);
+  float acc[2][4] = {};
+  for (int i0 = 0; i0 < splits; i0 += 32) {
+    const float l = i0 == 0 ? first : i0 + lane < splits ? part_lse[(i0 + lane) * rows + row] : -INFINITY;
+    const float weight = ex2((l - base) * kLog2e);
+    total += weight;
+    const int n = min(32, splits - i0);
+    const float* y = part_o + (i0 * rows + row) * dim + lane * 4;
+    const int64_t step = rows * dim;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) {
+      const float f = __shfl_sync(0xffffffffu, weight, i);
+      if (f == 0.0f) continue;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (lane * 4 + h * 128 < dim) {
+          const float4 x = *reinterpret_cast<const float4*>(y + i * step + h * 128);
+          acc[h][0] += f * x.x, acc[h][1] += f * x.y, acc[h][2] += f * x.z, acc[h][3] += f * x.w;
+        }
+    }
+  }
   total = warp_sum(total);
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-  for (int d0 = 0; d0 < dim; d0 += 32) {
-    const int d = d0 + lane;
-    float acc = 0.0f;
-    for (int i = 0; i < splits; ++i) {
-      const float l = part_lse[i * rows + row];
-      if (l == -INFINITY) continue;  // not written
-      if (d < dim) acc += ex2((l - base) * kLog2e) * inv * part_o[(i * rows + row) * dim + d];
-    }
-    if (d < dim) out[row * dim + d] = from_f32<T>(acc);
-  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    if (lane * 4 + h * 128 < dim)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[row * dim + lane * 4 + h * 128 + i] = from_f32<T>(acc[h][i] * inv);
   if (lane == 0) lse[row] = total == 0.0f ? -INFINITY : base + logf(total);
 }
 
 // ------------------------------------------------------------------ host side
+enum Kind { kKeys, kRows };
+struct Part {
+  Kind kind = kKeys;
+  int tiles = 0, splits = 0, chunk = 1;
+};
 struct Plan {
-  int prefix_tiles = 0, prefix_splits = 0, prefix_chunk = 1;
-  int own_tiles = 0, own_splits = 0, own_chunk = 1;
-  int splits() const { return prefix_splits + own_splits; }
+  Part prefix, own;
+  int splits() const { return prefix.splits + own.splits; }
 };
 
-// Ranges of keys: enough work items to fill the SMs, none shorter than a few
-// tiles.
-Plan plan(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv, int64_t prefix_keys, int64_t own_keys) {
-  constexpr int kTile = 64;
-  Plan p;
-  const int64_t group = heads_q / heads_kv, sms = sm_count();
-  if (prefix_keys > 0) {
-    p.prefix_tiles = (int)ceil_div(batch * queries * group, kTile);
-    const int64_t items = p.prefix_tiles * heads_kv;
-    const int64_t s = std::max<int64_t>(1, std::min(ceil_div(4 * sms, items), ceil_div(prefix_keys, 4 * kTile)));
-    p.prefix_chunk = (int)(ceil_div(ceil_div(prefix_keys, s), kTile) * kTile);
-    p.prefix_splits = (int)ceil_div(prefix_keys, p.prefix_chunk);
-  }
-  if (own_keys > 0) {
-    p.own_tiles = (int)ceil_div(queries * group, kTile);
-    const int64_t items = p.own_tiles * heads_kv * batch;
-    const int64_t s = std::max<int64_t>(1, std::min(ceil_div(4 * sms, items), ceil_div(own_keys, 4 * kTile)));
-    p.own_chunk = (int)(ceil_div(ceil_div(own_keys, s), kTile) * kTile);
-    p.own_splits = (int)ceil_div(own_keys, p.own_chunk);
-  }
+// One axis of keys for `sets` sets of `rows` query rows each: the kernel by
+// the number of rows, and ranges of keys that give every SM a few CTAs but no
+// CTA less than one block of keys.
+Part plan_part(int64_t sets, int64_t rows, int64_t keys) {
+  Part p;
+  if (keys <= 0) return p;
+  p.kind = rows <= 16 ? kKeys : kRows;
+  p.tiles = (int)ceil_div(rows, p.kind == kKeys ? 16 : 64);
+  const int64_t block = 64, least = p.kind == kKeys ? block : 4 * block;
+  const int64_t items = p.tiles * sets;
+  const int64_t s = std::max<int64_t>(1, std::min(ceil_div((int64_t)4 * sm_count(), items), ceil_div(keys, least)));
+  p.chunk = (int)(ceil_div(ceil_div(keys, s), block) * block);
+  p.splits = (int)ceil_div(keys, p.chunk);
   return p;
 }
+Plan plan(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv, int64_t prefix_keys, int64_t own_keys) {
+  const int64_t rows = queries * (heads_q / heads_kv);
+  return {plan_part(heads_kv, batch * rows, prefix_keys), plan_part(heads_kv * batch, rows, own_keys)};
+}
 
-template <typename T, int DP, int NK>
-int launch_rows(const AttnArgs& a, int64_t items, cudaStream_t stream) {
-  auto kern = attn_rows_kernel<T, DP, NK>;
-  constexpr size_t smem = RowsCfg<T, DP, NK>::kSmem;
-  static uint64_t attr_set = 0;  // one bit per device ordinal
+// The launch may begin once every CTA of the one before it has begun; the
+// kernel itself waits for that one's results (griddepcontrol.wait).
+cudaLaunchAttribute after_start() {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  return attr;
+}
+
+template <typename K>
+int launch(K kern, size_t smem, AttnArgs a, int64_t first, int64_t items, uint64_t& attr_set, cudaStream_t stream) {
+  if (items == 0) return KB_OK;
   int dev = 0;
   KB_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64 || !(attr_set >> dev & 1)) {
+  if (dev >= 64 || !(attr_set >> dev & 1)) {  // one bit per device ordinal
     KB_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     if (dev < 64) attr_set |= 1ull << dev;
   }
+  a.first_item = first;
   kern<<<(unsigned)items, 128, smem, stream>>>(a);
   return check_launch("kb_shared_prefix_attention");
 }
-
+template <typename T, int DP, int NK>
+int launch_rows(const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {
+  static uint64_t attr_set = 0;
+  return launch(attn_rows_kernel<T, DP, NK>, RowsCfg<T, DP, NK>::kSmem, a, first, items, attr_set, stream);
+}
+template <typename T, int DP, int NK, int STAGES>
+int launch_keys(const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {
+  static uint64_t attr_set = 0;
+  return launch(attn_keys_kernel<T, DP, NK, STAGES>, KeysCfg<T, DP, NK, STAGES>::kSmem, a, first, items, attr_set,
+                stream);
+}
 template <typename T>
-int launch_by_dim(const AttnArgs& a, int64_t items, cudaStream_t stream) {
-  if (a.dim <= 64) return launch_rows<T, 64, 64>(a, items, stream);
-  if (a.dim <= 128) return launch_rows<T, 128, 64>(a, items, stream);
-  return launch_rows<T, 256, sizeof(T) == 4 ? 32 : 64>(a, items, stream);
+int launch_kind(Kind kind, const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {
+  constexpr bool f32 = sizeof(T) == 4;
+  if (kind == kKeys) {
+    if (a.dim <= 64) return launch_keys<T, 64, 16, 4>(a, first, items, stream);
+    if (a.dim <= 128) return launch_keys<T, 128, 16, 3>(a, first, items, stream);
+    return launch_keys<T, 256, f32 ? 8 : 16, 3>(a, first, items, stream);
+  }
+  if (a.dim <= 64) return launch_rows<T, 64, 64>(a, first, items, stream);
+  if (a.dim <= 128) return launch_rows<T, 128, 64>(a, first, items, stream);
+  return launch_rows<T, 256, f32 ? 32 : 64>(a, first, items, stream);
 }
 
 }  // namespace
@@ -543,14 +791,18 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
   a.batch = (int)batch, a.queries = (int)queries, a.heads_q = (int)heads_q, a.heads_kv = (int)heads_kv;
   a.group = (int)(heads_q / heads_kv), a.dim = (int)dim;
   a.prefix_pages = (int)prefix_pages, a.width = (int)width, a.pages = (int)pages, a.page_size = (int)page_size;
+  a.page_shift = -1;
+  if ((page_size & (page_size - 1)) == 0)
+    while ((int64_t)1 << ++a.page_shift < page_size) {
+    }
   a.q_b = q_stride_seq, a.q_t = q_stride_query, a.q_h = q_stride_head;
   a.k_p = k_stride_page, a.k_s = k_stride_slot, a.k_h = k_stride_head;
   a.v_p = v_stride_page, a.v_s = v_stride_slot, a.v_h = v_stride_head;
   a.scale_log2 = scale * kLog2e;
-  a.prefix_tiles = p.prefix_tiles, a.prefix_splits = p.prefix_splits, a.prefix_chunk = p.prefix_chunk;
-  a.own_tiles = p.own_tiles, a.own_splits = p.own_splits, a.own_chunk = p.own_chunk;
-  a.prefix_items = (int64_t)p.prefix_tiles * p.prefix_splits * heads_kv;
-  const int64_t items = a.prefix_items + (int64_t)p.own_tiles * p.own_splits * heads_kv * batch;
+  a.prefix_tiles = p.prefix.tiles, a.prefix_splits = p.prefix.splits, a.prefix_chunk = p.prefix.chunk;
+  a.own_tiles = p.own.tiles, a.own_splits = p.own.splits, a.own_chunk = p.own.chunk;
+  a.prefix_items = (int64_t)p.prefix.tiles * p.prefix.splits * heads_kv;
+  const int64_t items = a.prefix_items + (int64_t)p.own.tiles * p.own.splits * heads_kv * batch;
   KB_REQUIRE(items <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many work items", name);
   if (p.splits() > 1) {
     const size_t need = kb_shared_prefix_attention_workspace_size(batch, queries, heads_q, heads_kv, dim,
@@ -564,13 +816,22 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
   return with_dtype(dtype, [&](auto* x) {
     using T = std::remove_pointer_t<decltype(x)>;
     if (items) {
-      if (int st = launch_by_dim<T>(a, items, stream)) return st;
+      if (p.prefix.kind == p.own.kind) {
+        if (int st = launch_kind<T>(p.own.kind, a, 0, items, stream)) return st;
+      } else {
+        if (int st = launch_kind<T>(p.prefix.kind, a, 0, a.prefix_items, stream)) return st;
+        if (int st = launch_kind<T>(p.own.kind, a, a.prefix_items, items - a.prefix_items, stream)) return st;
+      }
       if (p.splits() == 1) return (int)KB_OK;
     }
     // also where there are no keys at all: zeros and -inf
-    attn_join_kernel<T><<<(unsigned)kb::ceil_div(rows, 4), 128, 0, stream>>>(
-        a.part_o, a.part_lse, p.splits(), rows, (int)dim, static_cast<T*>(out), lse);
-    return kb::check_launch(name);
+    cudaLaunchConfig_t config{};
+    cudaLaunchAttribute attr = after_start();
+    config.gridDim = dim3((unsigned)kb::ceil_div(rows, 4)), config.blockDim = dim3(128), config.stream = stream;
+    config.attrs = &attr, config.numAttrs = 1;
+    KB_CUDA(cudaLaunchKernelEx(&config, attn_join_kernel<T>, (const float*)a.part_o, (const float*)a.part_lse,
+                               p.splits(), rows, (int)dim, static_cast<T*>(out), lse));
+    return (int)KB_OK;
   });
 }
 

@@ -523,6 +523,7 @@ __global__ void rope_weight_grads(const double* __restrict__ partial, int parts,
   const int e = blockIdx.x * 32 + lane;
   double s = 0.0;
   if (e < 2 * dim)
+#pragma unroll 8
     for (int i = row; i < parts; i += 32) s += partial[(int64_t)i * 2 * dim + e];
   red[row][lane] = s;
   __syncthreads();
