@@ -74,6 +74,12 @@
 
 namespace kb {
 
+namespace lm {
+namespace attn {
+int tc_read_fault(bool clear, int* value);  // the attention kernel's fault word
+}
+}  // namespace lm
+
 __device__ int g_gemm_fault = 0;  // nonzero after a CTA gave up waiting
 
 namespace gemm {
@@ -1060,6 +1066,9 @@ int kb_read_fault(int clear, int* value) {
     const int zero = 0;
     KB_CUDA(cudaMemcpyToSymbol(kb::g_gemm_fault, &zero, sizeof(int)));
   }
+  int attention = 0;
+  if (int st = kb::lm::attn::tc_read_fault(clear != 0, &attention)) return st;
+  *value |= attention;
   return KB_OK;
 }
 

@@ -21,19 +21,13 @@
 // range are clamped into the pool.
 #include <type_traits>
 
-#include "lm_common.cuh"
+#include "lm_attention.cuh"
 
 namespace kb {
 namespace lm {
+namespace attn {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ uint32_t smem_addr(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -46,63 +40,6 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-struct AttnArgs {
-  const void *q, *k, *v;
-  void* out;
-  float* lse;
-  const int *prefix, *table, *lens;
-  int batch, queries, heads_q, heads_kv, group, dim;
-  int prefix_pages, width, pages, page_size, page_shift;  // page_shift: its logarithm, or -1
-  int64_t q_b, q_t, q_h, k_p, k_s, k_h, v_p, v_s, v_h;  // strides in elements
-  float scale_log2;                                      // scale * log2(e)
-  int prefix_tiles, prefix_splits, prefix_chunk;         // row tiles per key head; ranges and keys per range
-  int own_tiles, own_splits, own_chunk;
-  int64_t prefix_items, first_item;                      // items of the prefix come first; the launch's first one
-  float *part_o, *part_lse;  // [splits][batch * queries * heads_q][dim], [splits][rows]; null: one range only
-};
-
-// A work item: rows r of key head h, query of row r = base + r / group, head
-// h * group + r % group; keys [k0, k1) through `pages`.
-struct Item {
-  int h, base, row0, rows, k0, k1, split;
-  const int* pages;
-};
-__device__ __forceinline__ Item item_at(const AttnArgs& a, int64_t id, int tile_rows) {
-  Item w;
-  const int P = a.prefix_pages * a.page_size;
-  if (id < a.prefix_items) {  // key head fastest: CTAs that run together read different heads of the same pages
-    w.h = (int)(id % a.heads_kv);
-    id /= a.heads_kv;
-    const int tile = (int)(id % a.prefix_tiles), s = (int)(id / a.prefix_tiles);
-    w.base = 0;
-    w.row0 = tile * tile_rows;
-    w.rows = min(tile_rows, a.batch * a.queries * a.group - w.row0);
-    w.k0 = s * a.prefix_chunk;
-    w.k1 = min(w.k0 + a.prefix_chunk, P);
-    w.split = s;
-    w.pages = a.prefix;
-  } else {
-    id -= a.prefix_items;
-    w.h = (int)(id % a.heads_kv);
-    id /= a.heads_kv;
-    const int tile = (int)(id % a.own_tiles);
-    id /= a.own_tiles;
-    const int b = (int)(id % a.batch), s = (int)(id / a.batch);
-    w.base = b * a.queries;
-    w.row0 = tile * tile_rows;
-    w.rows = min(tile_rows, a.queries * a.group - w.row0);
-    w.k0 = P + s * a.own_chunk;
-    w.k1 = min(w.k0 + a.own_chunk, a.width * a.page_size);
-    w.split = a.prefix_splits + s;
-    w.pages = a.table + (int64_t)b * a.width;
-  }
-  return w;
-}
-__device__ __forceinline__ int visible(const AttnArgs& a, int bt) {
-  const int b = bt / a.queries, t = bt - b * a.queries;
-  return a.lens[b] - a.queries + t + 1;
 }
 
 // ------------------------------------------------------------------ products
@@ -264,9 +201,13 @@ __device__ __forceinline__ void weigh(float (&o)[DP / 8][4], const float (&p)[NK
 struct Running {
   float m[2], l[2];
 };
-// Turns scores into weights exp2(s - m), after masking keys at or past
+template <typename T>
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return ((m == -INFINITY ? 0.0f : m) - kShift<T>) * kLn2 + logf(l);
+}
+// Turns scores into weights exp2(s - m + kShift), after masking keys at or past
 // vis[row], and rescales o.
-template <int NK, int ND>
+template <typename T, int NK, int ND>
 __device__ __forceinline__ void softmax_step(float (&s)[NK / 8][4], float (&o)[ND][4], Running& st, float scale_log2,
                                              int key0, const int (&vis)[2], bool masked, int lane) {
   float top[2] = {st.m[0], st.m[1]};
@@ -291,7 +232,7 @@ __device__ __forceinline__ void softmax_step(float (&s)[NK / 8][4], float (&o)[N
       o[d][2 * r] *= keep;
       o[d][2 * r + 1] *= keep;
     }
-    top[r] = base;
+    top[r] = base - kShift<T>;
   }
 #pragma unroll
   for (int n = 0; n < NK / 8; ++n)
@@ -321,7 +262,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
   T* sk = sq + C::kRows * LD;
   T* sv = sk + 2 * NK * LD;
   __shared__ int s_max[4];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  allow_next();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Item w = item_at(a, a.first_item + blockIdx.x, C::kRows);
   const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
@@ -342,16 +283,12 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
   __syncthreads();
   const int end = min(w.k1, max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])));
 
-  const T* q = static_cast<const T*>(a.q);
   const T* kp = static_cast<const T*>(a.k) + w.h * a.k_h;
   const T* vp = static_cast<const T*>(a.v) + w.h * a.v_h;
   for (int i = tid; i < C::kRows * kPerRow; i += C::kThreads) {
     const int r = i / kPerRow, c = (i - r * kPerRow) * kVec;
     const bool in = r < w.rows && c < a.dim;
-    const int rr = w.row0 + (in ? r : 0), bt = w.base + rr / a.group;
-    const T* src = q + (int64_t)(bt / a.queries) * a.q_b + (int64_t)(bt % a.queries) * a.q_t +
-                   (int64_t)(w.h * a.group + rr % a.group) * a.q_h + (in ? c : 0);
-    cp_async16(sq + r * LD + c, src, in);
+    cp_async16(sq + r * LD + c, static_cast<const T*>(query_of(a, w, in ? r : 0, sizeof(T))) + (in ? c : 0), in);
   }
   auto load = [&](int key0, int buf) {
     for (int i = tid; i < NK * kPerRow; i += C::kThreads) {
@@ -391,7 +328,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
     float s[NK / 8][4];
     scores<T, DP, NK, LD>(s, sq + warp * 16 * LD, sk + buf * NK * LD, lane);
     const int seen[2] = {min(vis[0], end), min(vis[1], end)};
-    softmax_step<NK, DP / 8>(s, o, st, a.scale_log2, key0, seen, key0 + NK > min(low, end), lane);
+    softmax_step<T, NK, DP / 8>(s, o, st, a.scale_log2, key0, seen, key0 + NK > min(low, end), lane);
     weigh<T, DP, NK, LD>(o, s, sv + buf * NK * LD, lane);
     __syncthreads();
   }
@@ -402,14 +339,13 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
     st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 1);
     st.l[r] += __shfl_xor_sync(0xffffffffu, st.l[r], 2);
     if (row[r] >= w.rows) continue;
-    const int rr = w.row0 + row[r];
-    const int64_t at = (int64_t)(w.base + rr / a.group) * a.heads_q + w.h * a.group + rr % a.group;
+    const int64_t at = row_index(a, w, row[r]);
     const bool none = st.l[r] == 0.0f;
     const float inv = none ? 0.0f : 1.0f / st.l[r];
-    const float lse = none ? -INFINITY : st.m[r] * kLn2 + logf(st.l[r]);
+    const float lse = none ? -INFINITY : lse_of<T>(st.m[r], st.l[r]);
     if (a.part_o) {
       const int64_t slot = (int64_t)w.split * n_rows + at;
-      if ((lane & 3) == 0) a.part_lse[slot] = lse;
+      if ((lane & 3) == 0) a.part_lse[at * a.splits + w.split] = lse;
       if (none) continue;  // the join does not read it
       float* y = a.part_o + slot * a.dim;
 #pragma unroll
@@ -456,7 +392,7 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
   T* sq = reinterpret_cast<T*>(raw);
   T* ring = sq + C::kRows * LD;
   __shared__ float s_m[4][16], s_l[4][16];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  allow_next();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Item w = item_at(a, a.first_item + blockIdx.x, C::kRows);
   const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
@@ -519,10 +455,7 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
     const int r = i / kPerRow, c = (i - r * kPerRow) * kVec;
     uint4 x = make_uint4(0, 0, 0, 0);
     if (r < w.rows && c < a.dim) {
-      const int rr = w.row0 + r, bt = w.base + rr / a.group;
-      x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (int64_t)(bt / a.queries) * a.q_b +
-                                          (int64_t)(bt % a.queries) * a.q_t +
-                                          (int64_t)(w.h * a.group + rr % a.group) * a.q_h + c);
+      x = *reinterpret_cast<const uint4*>(static_cast<const T*>(query_of(a, w, r, sizeof(T))) + c);
     }
     *reinterpret_cast<uint4*>(sq + r * LD + c) = x;
   }
@@ -546,7 +479,7 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
     const T* sk = mine + stage * C::kStage;
     float s[NK / 8][4];
     scores<T, DP, NK, LD>(s, sq, sk, lane);
-    softmax_step<NK, DP / 8>(s, o, st, a.scale_log2, key0, seen, key0 + NK > min(low, end), lane);
+    softmax_step<T, NK, DP / 8>(s, o, st, a.scale_log2, key0, seen, key0 + NK > min(low, end), lane);
     weigh<T, DP, NK, LD>(o, s, sk + NK * LD, lane);
     __syncwarp();  // all lanes are done with the stage that the next load fills
     stage = stage == STAGES - 1 ? 0 : stage + 1;
@@ -579,13 +512,12 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
     f[i] = ex2(s_m[i][r] - base);
     l += f[i] * s_l[i][r];
   }
-  const int rr = w.row0 + r;
-  const int64_t at = (int64_t)(w.base + rr / a.group) * a.heads_q + w.h * a.group + rr % a.group;
+  const int64_t at = row_index(a, w, r);
   const int64_t slot = (int64_t)w.split * n_rows + at;
   const bool none = l == 0.0f;
   const float inv = none ? 0.0f : 1.0f / l;
-  const float lse = none ? -INFINITY : m * kLn2 + logf(l);
-  if ((tid & 7) == 0) (a.part_o ? a.part_lse[slot] : a.lse[at]) = lse;
+  const float lse = none ? -INFINITY : lse_of<T>(m, l);
+  if ((tid & 7) == 0) (a.part_o ? a.part_lse[at * a.splits + w.split] : a.lse[at]) = lse;
   if (a.part_o && none) return;  // the join does not read it
   for (int d = (tid & 7) * 4; d < a.dim; d += 32) {
     float y[4] = {};
@@ -611,38 +543,48 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
 // One warp per row: the parts weighed by exp(lse_i - L), in their order.  Lane
 // i holds the weight of part i; a part without keys has weight 0 and is not
 // read (nothing was written there).
+constexpr int kJoin = 8;
 template <typename T>
 __global__ void __launch_bounds__(128) attn_join_kernel(const float* __restrict__ part_o,
                                                         const float* __restrict__ part_lse, int splits, int64_t rows,
                                                         int dim, T* __restrict__ out, float* __restrict__ lse) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the parts
+  wait_for_previous();  // for the parts
   if (row >= rows) return;
-  const float first = lane < splits ? part_lse[lane * rows + row] : -INFINITY;
+  part_lse += row * splits;
+  const float first = lane < splits ? part_lse[lane] : -INFINITY;
   float top = first;
-  for (int i = lane + 32; i < splits; i += 32) top = fmaxf(top, part_lse[i * rows + row]);
+  for (int i = lane + 32; i < splits; i += 32) top = fmaxf(top, part_lse[i]);
   top = warp_max(top);
   const float base = top == -INFINITY ? 0.0f : top;
   float total = 0.0f;  // a NaN part makes it NaN
   float acc[2][4] = {};
   for (int i0 = 0; i0 < splits; i0 += 32) {
-    const float l = i0 == 0 ? first : i0 + lane < splits ? part_lse[(i0 + lane) * rows + row] : -INFINITY;
+    const float l = i0 == 0 ? first : i0 + lane < splits ? part_lse[i0 + lane] : -INFINITY;
     const float weight = ex2((l - base) * kLog2e);
     total += weight;
     const int n = min(32, splits - i0);
     const float* y = part_o + (i0 * rows + row) * dim + lane * 4;
     const int64_t step = rows * dim;
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      const float f = __shfl_sync(0xffffffffu, weight, i);
-      if (f == 0.0f) continue;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (lane * 4 + h * 128 < dim) {
-          const float4 x = *reinterpret_cast<const float4*>(y + i * step + h * 128);
-          acc[h][0] += f * x.x, acc[h][1] += f * x.y, acc[h][2] += f * x.z, acc[h][3] += f * x.w;
+    for (int h = 0; h < 2; ++h) {
+      if (h * 128 >= dim) break;
+      const bool mine = lane * 4 + h * 128 < dim;
+      for (int j = 0; j < n; j += kJoin) {  // loads of kJoin parts in flight
+        float4 x[kJoin];
+        float f[kJoin];
+#pragma unroll
+        for (int i = 0; i < kJoin; ++i) {
+          f[i] = __shfl_sync(0xffffffffu, weight, (j + i) & 31);
+          if (j + i >= n) f[i] = 0.0f;
+          x[i] = mine && f[i] != 0.0f ? *reinterpret_cast<const float4*>(y + (j + i) * step + h * 128)
+                                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
+#pragma unroll
+        for (int i = 0; i < kJoin; ++i)
+          acc[h][0] += f[i] * x[i].x, acc[h][1] += f[i] * x[i].y, acc[h][2] += f[i] * x[i].z, acc[h][3] += f[i] * x[i].w;
+      }
     }
   }
   total = warp_sum(total);
@@ -656,7 +598,7 @@ __global__ void __launch_bounds__(128) attn_join_kernel(const float* __restrict_
 }
 
 // ------------------------------------------------------------------ host side
-enum Kind { kKeys, kRows };
+enum Kind { kKeys, kRows, kTensor };
 struct Part {
   Kind kind = kKeys;
   int tiles = 0, splits = 0, chunk = 1;
@@ -669,10 +611,25 @@ struct Plan {
 // One axis of keys for `sets` sets of `rows` query rows each: the kernel by
 // the number of rows, and ranges of keys that give every SM a few CTAs but no
 // CTA less than one block of keys.
-Part plan_part(int64_t sets, int64_t rows, int64_t keys) {
+Part plan_part(int64_t sets, int64_t rows, int64_t keys, bool tensor) {
   Part p;
   if (keys <= 0) return p;
-  p.kind = rows <= 16 ? kKeys : kRows;
+  p.kind = rows <= 16 ? kKeys : tensor ? kTensor : kRows;
+  if (p.kind == kTensor) {
+    // One CTA per SM, equal ranges of whole 128-key tiles: the number of
+    // ranges that makes the last wave end first, a range's fixed cost (the
+    // queries, the first scores, the way out) counted as kFixed tiles.
+    constexpr int64_t kFixed = 3;
+    p.tiles = (int)ceil_div(rows, (int64_t)tc_tile_rows(rows));
+    const int64_t items = p.tiles * sets, tiles = ceil_div(keys, 128), most = std::min<int64_t>(tiles, 64);
+    int64_t best = 0;
+    for (int64_t s = 1; s <= most; ++s) {
+      const int64_t each = ceil_div(tiles, s), n = ceil_div(tiles, each);
+      const int64_t cost = ceil_div(items * n, (int64_t)sm_count()) * (each + kFixed);
+      if (best == 0 || cost < best) best = cost, p.chunk = (int)each * 128, p.splits = (int)n;
+    }
+    return p;
+  }
   p.tiles = (int)ceil_div(rows, p.kind == kKeys ? 16 : 64);
   const int64_t block = 64, least = p.kind == kKeys ? block : 4 * block;
   const int64_t items = p.tiles * sets;
@@ -681,9 +638,13 @@ Part plan_part(int64_t sets, int64_t rows, int64_t keys) {
   p.splits = (int)ceil_div(keys, p.chunk);
   return p;
 }
-Plan plan(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv, int64_t prefix_keys, int64_t own_keys) {
+Plan plan(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv, int64_t prefix_keys, int64_t own_keys,
+          bool tensor) {
   const int64_t rows = queries * (heads_q / heads_kv);
-  return {plan_part(heads_kv, batch * rows, prefix_keys), plan_part(heads_kv * batch, rows, own_keys)};
+  return {plan_part(heads_kv, batch * rows, prefix_keys, tensor), plan_part(heads_kv * batch, rows, own_keys, false)};
+}
+size_t plan_bytes(const Plan& p, int64_t rows, int64_t dim) {
+  return p.splits() <= 1 ? 0 : (size_t)p.splits() * rows * (dim + 1) * sizeof(float);
 }
 
 // The launch may begin once every CTA of the one before it has begun; the
@@ -733,6 +694,7 @@ int launch_kind(Kind kind, const AttnArgs& a, int64_t first, int64_t items, cuda
 }
 
 }  // namespace
+}  // namespace attn
 }  // namespace lm
 }  // namespace kb
 
@@ -741,13 +703,15 @@ extern "C" {
 size_t kb_shared_prefix_attention_workspace_size(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv,
                                                  int64_t dim, int64_t prefix_pages, int64_t width,
                                                  int64_t page_size, int dtype) {
-  (void)dtype;
-  if (batch <= 0 || queries <= 0 || heads_q <= 0 || heads_kv <= 0 || dim <= 0 || page_size <= 0) return 0;
-  const kb::lm::Plan p = kb::lm::plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size,
-                                      std::max<int64_t>(0, width - prefix_pages) * page_size);
-  if (p.splits() <= 1) return 0;
-  const int64_t rows = batch * queries * heads_q;
-  return (size_t)p.splits() * (rows * dim + kb::ceil_div(rows, 4) * 4) * sizeof(float);
+  using namespace kb::lm::attn;
+  if (heads_q % heads_kv) return 0;
+  auto bytes = [&](bool tensor) {
+    return plan_bytes(plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size,
+                           std::max<int64_t>(0, width - prefix_pages) * page_size, tensor),
+                      batch * queries * heads_q, dim);
+  };
+  // strides decide whether the tensor-core kernel can take the prefix
+  return dtype == KB_F32 ? bytes(false) : std::max(bytes(false), bytes(true));
 }
 
 int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* prefix,
@@ -760,6 +724,7 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
                                size_t workspace_bytes, kbStream stream) {
   const char* name = "kb_shared_prefix_attention";
   using namespace kb::lm;
+  using namespace kb::lm::attn;
   KB_REQUIRE(batch >= 0 && queries >= 0 && heads_q >= 0 && heads_kv >= 0 && dim >= 0 && prefix_pages >= 0 &&
                  width >= 0 && pages >= 0 && page_size >= 1,
              KB_ERR_INVALID_ARG, "%s: negative size", name);
@@ -784,7 +749,6 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
              KB_ERR_UNSUPPORTED, "%s: queries, pools and their strides must be multiples of 16 bytes", name);
   KB_REQUIRE(rows <= 0x3fffffff && (prefix_pages + own_pages) * page_size <= 0x3fffffff && pages <= 0x7fffffff,
              KB_ERR_UNSUPPORTED, "%s: too many rows or keys", name);
-  const Plan p = plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size, own_pages * page_size);
   AttnArgs a{};
   a.q = q, a.k = k_pages, a.v = v_pages, a.out = out, a.lse = lse;
   a.prefix = prefix, a.table = table, a.lens = lens;
@@ -799,14 +763,16 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
   a.k_p = k_stride_page, a.k_s = k_stride_slot, a.k_h = k_stride_head;
   a.v_p = v_stride_page, a.v_s = v_stride_slot, a.v_h = v_stride_head;
   a.scale_log2 = scale * kLog2e;
+  const Plan p = plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size, own_pages * page_size,
+                      tc_fits(a, dtype));
+  a.splits = p.splits();
   a.prefix_tiles = p.prefix.tiles, a.prefix_splits = p.prefix.splits, a.prefix_chunk = p.prefix.chunk;
   a.own_tiles = p.own.tiles, a.own_splits = p.own.splits, a.own_chunk = p.own.chunk;
   a.prefix_items = (int64_t)p.prefix.tiles * p.prefix.splits * heads_kv;
   const int64_t items = a.prefix_items + (int64_t)p.own.tiles * p.own.splits * heads_kv * batch;
   KB_REQUIRE(items <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many work items", name);
   if (p.splits() > 1) {
-    const size_t need = kb_shared_prefix_attention_workspace_size(batch, queries, heads_q, heads_kv, dim,
-                                                                  prefix_pages, width, page_size, dtype);
+    const size_t need = plan_bytes(p, rows, dim);
     KB_REQUIRE(workspace && workspace_bytes >= need, KB_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", name, need, workspace_bytes);
     KB_REQUIRE(kb::aligned16(workspace), KB_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
@@ -819,7 +785,9 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
       if (p.prefix.kind == p.own.kind) {
         if (int st = launch_kind<T>(p.own.kind, a, 0, items, stream)) return st;
       } else {
-        if (int st = launch_kind<T>(p.prefix.kind, a, 0, a.prefix_items, stream)) return st;
+        if (int st = p.prefix.kind == kTensor ? tc_launch(a, dtype, stream)
+                                              : launch_kind<T>(p.prefix.kind, a, 0, a.prefix_items, stream))
+          return st;
         if (int st = launch_kind<T>(p.own.kind, a, a.prefix_items, items - a.prefix_items, stream)) return st;
       }
       if (p.splits() == 1) return (int)KB_OK;

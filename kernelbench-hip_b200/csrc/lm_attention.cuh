@@ -1,0 +1,110 @@
+// lm_attention.cuh — what the kernels of attention over the paged cache share:
+// their arguments, work items and the running softmax's exponential.
+#pragma once
+
+#include <type_traits>
+
+#include "lm_common.cuh"
+
+namespace kb {
+namespace lm {
+namespace attn {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The weights exp2(s - m) are rounded to the values' type.  fp16 keeps 10 bits
+// down to 2^-14 only, so its weights are held 2^kShift higher (far below its
+// largest), and small ones do not lose bits; bf16 has fp32's range.
+template <typename T>
+constexpr float kShift = std::is_same_v<T, __half> ? 10.0f : 0.0f;
+
+// Lets the next launch begin where it was made with programmatic stream
+// serialisation; it waits for this one's results by itself.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+struct AttnArgs {
+  const void *q, *k, *v;
+  void* out;
+  float* lse;
+  const int *prefix, *table, *lens;
+  int batch, queries, heads_q, heads_kv, group, dim;
+  int prefix_pages, width, pages, page_size, page_shift;  // page_shift: its logarithm, or -1
+  int64_t q_b, q_t, q_h, k_p, k_s, k_h, v_p, v_s, v_h;  // strides in elements
+  float scale_log2;                                      // scale * log2(e)
+  int prefix_tiles, prefix_splits, prefix_chunk;         // row tiles per key head; ranges and keys per range
+  int own_tiles, own_splits, own_chunk, splits;
+  int64_t prefix_items, first_item;                      // items of the prefix come first; the launch's first one
+  float *part_o, *part_lse;  // [splits][rows][dim], [rows][splits] (rows: batch * queries * heads_q); null: one range
+};
+
+// A work item: rows r of key head h, query of row r = base + r / group, head
+// h * group + r % group; keys [k0, k1) through `pages`.
+struct Item {
+  int h, base, row0, rows, k0, k1, split;
+  const int* pages;
+};
+__device__ __forceinline__ Item item_at(const AttnArgs& a, int64_t id, int tile_rows) {
+  Item w;
+  const int P = a.prefix_pages * a.page_size;
+  if (id < a.prefix_items) {  // key head fastest: CTAs that run together read different heads of the same pages
+    w.h = (int)(id % a.heads_kv);
+    id /= a.heads_kv;
+    const int tile = (int)(id % a.prefix_tiles), s = (int)(id / a.prefix_tiles);
+    w.base = 0;
+    w.row0 = tile * tile_rows;
+    w.rows = min(tile_rows, a.batch * a.queries * a.group - w.row0);
+    w.k0 = s * a.prefix_chunk;
+    w.k1 = min(w.k0 + a.prefix_chunk, P);
+    w.split = s;
+    w.pages = a.prefix;
+  } else {
+    id -= a.prefix_items;
+    w.h = (int)(id % a.heads_kv);
+    id /= a.heads_kv;
+    const int tile = (int)(id % a.own_tiles);
+    id /= a.own_tiles;
+    const int b = (int)(id % a.batch), s = (int)(id / a.batch);
+    w.base = b * a.queries;
+    w.row0 = tile * tile_rows;
+    w.rows = min(tile_rows, a.queries * a.group - w.row0);
+    w.k0 = P + s * a.own_chunk;
+    w.k1 = min(w.k0 + a.own_chunk, a.width * a.page_size);
+    w.split = a.prefix_splits + s;
+    w.pages = a.table + (int64_t)b * a.width;
+  }
+  return w;
+}
+__device__ __forceinline__ int visible(const AttnArgs& a, int bt) {
+  const int b = bt / a.queries, t = bt - b * a.queries;
+  return a.lens[b] - a.queries + t + 1;
+}
+// Row r of the item in the tensors' order [batch, queries, heads_q].
+__device__ __forceinline__ int64_t row_index(const AttnArgs& a, const Item& w, int r) {
+  const int rr = w.row0 + r;
+  return (int64_t)(w.base + rr / a.group) * a.heads_q + w.h * a.group + rr % a.group;
+}
+__device__ __forceinline__ const void* query_of(const AttnArgs& a, const Item& w, int r, int element_size) {
+  const int rr = w.row0 + r, bt = w.base + rr / a.group;
+  return static_cast<const char*>(a.q) +
+         ((int64_t)(bt / a.queries) * a.q_b + (int64_t)(bt % a.queries) * a.q_t +
+          (int64_t)(w.h * a.group + rr % a.group) * a.q_h) * element_size;
+}
+
+// ------------------------------------------------------------------ tensor-core prefix (lm_attention_tc.cu)
+// Whether it can take the prefix (16-bit types, head and page sizes, strides).
+bool tc_fits(const AttnArgs& a, int dtype);
+// Row tiles it makes of `rows` rows of one key head.
+int tc_tile_rows(int64_t rows);
+int tc_launch(const AttnArgs& a, int dtype, cudaStream_t stream);
+// The device's fault word: nonzero after a wait ran out.
+int tc_read_fault(bool clear, int* value);
+
+}  // namespace attn
+}  // namespace lm
+}  // namespace kb

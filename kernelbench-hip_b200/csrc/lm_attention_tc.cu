@@ -1,0 +1,580 @@
+// lm_attention_tc.cu — the shared prefix on the fifth-generation tensor cores:
+// all query rows of one key head against the prefix's keys and values, in
+// fp16 or bf16.
+//
+// A CTA takes up to two tiles of 128 query rows and a range of keys, in tiles
+// of 128.  Per key tile j and row tile t:
+//   S_t = Q_t K_j^T            tcgen05.mma, 128 x 128, accumulators in TMEM
+//   P_t = exp2(S_t c - m)      one thread per row (tcgen05.ld), rounded to 16
+//                              bits into TMEM over S_t (tcgen05.st)
+//   O_t += P_t V_j             tcgen05.mma with P from TMEM, O in TMEM
+// c = scale log2(e).  m is a row's reference, not its exact maximum: it only
+// moves when the maximum has grown past it by more than 2^kSlack, and then the
+// row's O is scaled in TMEM (rare after the first tiles); l and O carry the
+// same m, so it cancels in O / l.  l sums the unrounded exponentials in fp32.
+//
+// Roles (10 warps): warps 0-3 and 4-7 are the softmax of the two row tiles,
+// warp 8 loads K and V tiles by TMA, one copy per page and 64 columns (the
+// page table is the gather), warp 9 issues the products in the order
+//   O_0 += P_0 V_j, S_0 = Q_0 K_j+1, O_1 += P_1 V_j, S_1 = Q_1 K_j+1
+// so that one row tile's products run during the other's softmax.  The
+// products of a thread are executed in order, so S_t(j + 1) may overwrite the
+// P_t(j) that the product before it reads.
+//
+// TMEM (512 columns): S_0, S_1 (P_t in the first 64 columns of S_t), O_0, O_1.
+// Shared memory: Q 64 KB, two stages of K and of V, 32 KB each, all in rows of
+// 128 bytes with the 128-byte swizzle: K-major for Q and K, MN-major for V.
+// Columns past the head size are zeros (TMA fills them), and so are V rows
+// past the last key that any row of the CTA sees.
+//
+// Bound: 4 rows keys dim operations on the tensor cores, and as many cycles
+// again of exponentials (16 per clock and SM against 128 x 128 x 128 products
+// in 512 cycles), which overlap.
+//
+// Every wait is bounded: one that runs out raises the CTA's abort flag and the
+// device's fault word, every role leaves, copies in flight are waited for
+// (bounded), TMEM is freed; outputs are then invalid.
+#include <cuda.h>
+
+#include <type_traits>
+
+#include "lm_attention.cuh"
+
+namespace kb {
+namespace lm {
+namespace attn {
+
+__device__ int g_fault = 0;  // nonzero after a CTA gave up waiting
+
+namespace {
+
+constexpr int kTile = 128;                      // rows of a row tile, keys of a key tile
+constexpr int kHalfBytes = kTile * 128;         // 128 rows of 64 16-bit columns
+constexpr int kTileBytes = 2 * kHalfBytes;      // 128 x 128 elements
+constexpr int kStages = 2;
+constexpr int kThreads = 320;
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kSmemBytes = (2 + 2 * kStages) * kTileBytes + 256 + 1024;  // + barriers, alignment
+constexpr uint64_t kWaitLimitNs = 2000000000ull;
+constexpr float kSlack = 4.0f;                  // log2 of how far a maximum may pass the reference
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ uint64_t globaltimer() {
+  uint64_t t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// False once this or another CTA has given up, or after kWaitLimitNs.
+__device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  const uint64_t t0 = globaltimer();
+  for (uint32_t n = 1;; ++n) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((n & 63) == 0) {
+      if (*abort_flag || *(volatile int*)&g_fault) {
+        *abort_flag = 1;
+        return false;
+      }
+      if (globaltimer() - t0 > kWaitLimitNs) {
+        *abort_flag = 1;
+        atomicExch(&g_fault, 1);
+        return false;
+      }
+    }
+  }
+}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return mbar_try_wait(bar, parity) || mbar_wait_slow(bar, parity, abort_flag);
+}
+// All lanes of the warp leave together.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int col, int head, int slot,
+                                         int page) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(dst), "l"(reinterpret_cast<uint64_t>(tm)), "r"(bar), "r"(col), "r"(head), "r"(slot), "r"(page)
+      : "memory");
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_alloc(uint32_t dst_smem, uint32_t cols) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(cols) : "memory");
+}
+__device__ __forceinline__ void tmem_relinquish() {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t cols) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(cols) : "memory");
+}
+// D[128 x N] (+)= A B, A from shared memory or TMEM
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+#define KB_R32(r)                                                                                                 \
+  "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),      \
+      "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),       \
+      "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),      \
+      "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+#define KB_R32_IN(r)                                                                                              \
+  "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),    \
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),  \
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),  \
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+// 32 columns of this warp's 32 lanes
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : KB_R32(r)
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::KB_R32_IN(r),
+      "r"(taddr)
+      : "memory");
+}
+#define KB_R32_IO(r)                                                                                              \
+  "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),      \
+      "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),       \
+      "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),      \
+      "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+// Waits for the loads; the registers pass through, so that no use of them is moved before the wait.
+__device__ __forceinline__ void tmem_ld_wait(uint32_t* r) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" : KB_R32_IO(r)::"memory");
+}
+__device__ __forceinline__ void after_wait(uint32_t* r) { asm volatile("" : KB_R32_IO(r)::"memory"); }
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory descriptors, 128-byte swizzle (layout type 2): rows of 128
+// bytes in groups of eight, 1024 bytes apart (SBO).  K-major (Q, K): 64
+// elements of the contraction per row; a step of 16 advances 32 bytes.
+// MN-major (V): 64 columns per row, one row per key; the next 64 columns lie
+// LBO = kHalfBytes further; a step of 16 keys advances 2048 bytes.
+__device__ __forceinline__ uint64_t make_desc(uint32_t saddr, uint32_t lbo) {
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// D fp32, A and B of one 16-bit type, A K-major, B K-major or MN-major.
+template <typename T>
+__host__ __device__ constexpr uint32_t make_idesc(int n, bool b_mn) {
+  const uint32_t f = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
+  return (1u << 4) | (f << 7) | (f << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) |
+         ((uint32_t)(kTile >> 4) << 24);
+}
+
+__device__ __forceinline__ uint32_t pack(float x, float y, __half*) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack(float x, float y, __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, AttnArgs a,
+                   int row_tiles) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* s_q = smem;
+  uint8_t* s_k = smem + 2 * kTileBytes;
+  uint8_t* s_v = s_k + kStages * kTileBytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + kStages * kTileBytes);
+  auto bar = [&](int i) { return smem_u32(bars + i); };
+  const uint32_t q_full = bar(0);  // [2]
+  auto k_full = [&](int s) { return bar(2 + s); };
+  auto k_empty = [&](int s) { return bar(4 + s); };
+  auto v_full = [&](int s) { return bar(6 + s); };
+  auto v_empty = [&](int s) { return bar(8 + s); };
+  auto s_full = [&](int t) { return bar(10 + t); };
+  auto p_full = [&](int t) { return bar(12 + t); };
+  auto o_full = [&](int t) { return bar(14 + t); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_end = reinterpret_cast<int*>(tmem_slot + 2);
+  allow_next();
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Item w = item_at(a, blockIdx.x, row_tiles * kTile);
+  const int cols = row_tiles == 2 ? 512 : 256;
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(q_full + 8 * t, kTile);
+      mbar_init(s_full(t), 1);
+      mbar_init(p_full(t), kTile);
+      mbar_init(o_full(t), 1);
+    }
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+      mbar_init(v_full(s), 1);
+      mbar_init(v_empty(s), 1);
+    }
+    *abort_flag = 0;
+    *s_end = 0;
+    fence_barrier_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(smem_u32(tmem_slot), cols);
+    tmem_relinquish();
+  }
+  __syncthreads();
+  // the keys that any row of this CTA sees
+  const int t = warp >> 2, row = threadIdx.x & (kTile - 1);  // softmax warps: row tile, row in it
+  const int r = t * kTile + row;
+  int vis = 0;
+  if (warp < 4 * row_tiles) {
+    if (r < w.rows) vis = visible(a, w.base + (w.row0 + r) / a.group);
+    const int top = __reduce_max_sync(0xffffffffu, vis);
+    if (lane == 0) atomicMax(s_end, top);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int end = min(w.k1, *s_end);
+  const int n = end > w.k0 ? (end - w.k0 + kTile - 1) / kTile : 0;
+  const int halves = a.dim > 64 ? 2 : 1;
+  const uint32_t o_col = row_tiles == 2 ? 256 : 128;
+
+  if (warp == kLoadWarp) {
+    // ---------------- K and V tiles: lane i copies page i of the tile
+    const int slots = min(a.page_size, kTile), per_tile = kTile / slots;
+    bool alive = true;
+    int issued = 0;
+    for (int j = 0; j < n && alive; ++j) {
+      const int key0 = w.k0 + j * kTile, s = j % kStages;
+      // past the prefix, or past what anyone sees: a page that is not there reads as zeros
+      int page = a.pages, slot = 0;
+      const int key = key0 + lane * slots;
+      if (lane < per_tile && key < end) {
+        page = min(max(w.pages[key / a.page_size], 0), a.pages - 1);
+        slot = key % a.page_size;
+      }
+      const uint32_t parity = ((j / kStages) & 1) ^ 1;
+      for (int kv = 0; kv < 2 && alive; ++kv) {
+        const uint32_t full = kv ? v_full(s) : k_full(s);
+        if (!warp_wait(kv ? v_empty(s) : k_empty(s), parity, abort_flag)) {
+          alive = false;
+          break;
+        }
+        if (lane == 0) mbar_expect_tx(full, halves * kHalfBytes);
+        __syncwarp();
+        if (lane < per_tile) {
+          const uint32_t dst = smem_u32((kv ? s_v : s_k) + s * kTileBytes + lane * slots * 128);
+          for (int h = 0; h < halves; ++h)
+            tma_load(dst + h * kHalfBytes, kv ? &tm_v : &tm_k, full, h * 64, w.h, slot, page);
+        }
+        ++issued;
+      }
+    }
+    // every issued copy must land before the CTA may exit
+    if (lane == 0)
+      for (int i = max(issued - 2 * kStages, 0); i < issued; ++i) {
+        const int j = i / 2, s = j % kStages;
+        const uint64_t t0 = globaltimer();
+        while (!mbar_try_wait(i & 1 ? v_full(s) : k_full(s), (j / kStages) & 1))
+          if (globaltimer() - t0 > kWaitLimitNs) break;
+      }
+  } else if (warp == kMmaWarp) {
+    // ---------------- products
+    if (lane == 0 && n > 0) {
+      const int depth = (a.dim + 15) / 16;  // steps of 16 columns of Q and K
+      const uint32_t idesc_s = make_idesc<T>(kTile, false), idesc_o = make_idesc<T>(depth * 16, true);
+      auto scores = [&](int i, int s) {
+        for (int k = 0; k < depth; ++k) {
+          const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
+          mma_ss(tmem + i * kTile, make_desc(smem_u32(s_q + i * kTileBytes) + off, 16),
+                 make_desc(smem_u32(s_k + s * kTileBytes) + off, 16), idesc_s, k > 0);
+        }
+        mma_commit(s_full(i));
+      };
+      bool alive = mbar_wait(k_full(0), 0, abort_flag);
+      for (int i = 0; i < row_tiles && alive; ++i) {
+        alive = mbar_wait(q_full + 8 * i, 0, abort_flag);
+        if (!alive) break;
+        tc_fence_after();
+        scores(i, 0);
+      }
+      if (alive) mma_commit(k_empty(0));
+      for (int j = 0; j < n && alive; ++j) {
+        const int s = j % kStages, next = (j + 1) % kStages;
+        const uint32_t parity = (j / kStages) & 1, next_parity = ((j + 1) / kStages) & 1;
+        for (int i = 0; i < row_tiles && alive; ++i) {
+          alive = mbar_wait(p_full(i), j & 1, abort_flag) && (i > 0 || mbar_wait(v_full(s), parity, abort_flag));
+          if (!alive) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = 0; k < kTile / 16; ++k)
+            mma_ts(tmem + o_col + i * kTile, tmem + i * kTile + k * 8,
+                   make_desc(smem_u32(s_v + s * kTileBytes) + k * 2048, kHalfBytes), idesc_o, j > 0 || k > 0);
+          mma_commit(o_full(i));
+          if (i == row_tiles - 1) mma_commit(v_empty(s));
+          if (j + 1 < n) {
+            alive = i > 0 || mbar_wait(k_full(next), next_parity, abort_flag);
+            if (!alive) break;
+            scores(i, next);
+            if (i == row_tiles - 1) mma_commit(k_empty(next));
+          }
+        }
+      }
+    }
+  } else if (t < row_tiles) {
+    // ---------------- softmax: this thread's row
+    const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
+    const uint32_t s_addr = tmem + lanes + t * kTile, o_addr = tmem + lanes + o_col + t * kTile;
+    const float c = fabsf(a.scale_log2);
+    if (n > 0) {
+      // the row of Q into the swizzled tile, its sign turned where the scale is negative
+      const uint4* src = static_cast<const uint4*>(query_of(a, w, r < w.rows ? r : 0, 2));
+      const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+      uint8_t* dst = s_q + t * kTileBytes + row * 128;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (i >= halves * 8) break;
+        if (r < w.rows && i * 8 < a.dim) {
+          x = src[i];
+          x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
+        }
+        *reinterpret_cast<uint4*>(dst + (i >> 3) * kHalfBytes + (((i & 7) ^ (row & 7)) << 4)) = x;
+      }
+      fence_proxy_async();
+      mbar_arrive(q_full + 8 * t);
+    }
+    float m = -INFINITY, l = 0.0f;  // the reference, in units of log2, and the sum
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      ok = warp_wait(s_full(t), j & 1, abort_flag);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t x[kTile];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tmem_ld(s_addr + i * 32, x + i * 32);
+      tmem_ld_wait(x);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) after_wait(x + i * 32);
+      auto f = [&](int i) { return __uint_as_float(x[i]); };
+      const int lim = min(vis, end) - (w.k0 + j * kTile);  // keys of this tile that the row sees
+      if (__any_sync(0xffffffffu, lim < kTile)) {
+#pragma unroll
+        for (int i = 0; i < kTile; ++i)
+          if (i >= lim) x[i] = 0xff800000u;
+      }
+      float top[4] = {f(0), f(1), f(2), f(3)};
+#pragma unroll
+      for (int i = 4; i < kTile; ++i) top[i & 3] = fmaxf(top[i & 3], f(i));
+      const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+      // move the reference where the maximum has outgrown it
+      const bool move = now > m + kSlack;  // also from -inf; not for a NaN
+      if (__any_sync(0xffffffffu, move)) {
+        const float keep = move ? ex2(m - now) : 1.0f;
+        if (move) m = now;
+        l *= keep;
+        if (j > 0) {
+          ok = warp_wait(o_full(t), (j - 1) & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int i = 0; i < a.dim; i += 32) {
+            uint32_t y[32];
+            tmem_ld(o_addr + i, y);
+            tmem_ld_wait(y);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * keep);
+            tmem_st(o_addr + i, y);
+          }
+          tmem_st_wait();
+        }
+      }
+      const float base = (m == -INFINITY ? 0.0f : m) - kShift<T>;
+      float sum[4] = {};
+#pragma unroll
+      for (int i = 0; i < kTile; i += 2) {
+        const float p0 = ex2(fmaf(f(i), c, -base)), p1 = ex2(fmaf(f(i + 1), c, -base));
+        sum[i & 2] += p0;
+        sum[(i & 2) + 1] += p1;
+        x[i >> 1] = pack(p0, p1, (T*)nullptr);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st(s_addr, x);
+      tmem_st(s_addr + 32, x + 32);
+      tmem_st_wait();
+      // V rows that nobody sees, in a page that is partly seen: zeros, for 0 x NaN
+      if (j == n - 1 && t == 0 && end < w.k0 + n * kTile && end % a.page_size != 0) {
+        ok = warp_wait(v_full(j % kStages), (j / kStages) & 1, abort_flag);
+        if (!ok) break;
+        if (w.k0 + j * kTile + row >= end)
+          for (int i = 0; i < halves * 8; ++i)
+            *reinterpret_cast<uint4*>(s_v + (j % kStages) * kTileBytes + (i >> 3) * kHalfBytes + row * 128 +
+                                      ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();
+      }
+      tc_fence_before();
+      mbar_arrive(p_full(t));
+    }
+    if (ok && n > 0) ok = warp_wait(o_full(t), (n - 1) & 1, abort_flag);
+    tc_fence_after();
+    const bool none = l == 0.0f || n == 0;
+    const int64_t at = r < w.rows ? row_index(a, w, r) : 0;
+    const float base = m - kShift<T>, inv = none ? 0.0f : 1.0f / l;
+    const float lse = none ? -INFINITY : (m == -INFINITY ? 0.0f : base) * kLn2 + logf(l);
+    if (r < w.rows) (a.part_o ? a.part_lse[at * a.splits + w.split] : a.lse[at]) = lse;
+    if (ok) {
+      const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
+#pragma unroll 1
+      for (int i = 0; i < a.dim; i += 32) {
+        uint32_t y[32];
+        if (n > 0) {
+          tmem_ld(o_addr + i, y);
+          tmem_ld_wait(y);
+        }
+        if (r >= w.rows || (none && a.part_o)) continue;  // a part without keys is not read
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) {
+          if (i + k >= a.dim) break;
+          float z[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) z[e] = none ? 0.0f : __uint_as_float(y[k + e]) * inv;
+          if (a.part_o) {
+            *reinterpret_cast<float4*>(a.part_o + ((int64_t)w.split * n_rows + at) * a.dim + i + k) =
+                make_float4(z[0], z[1], z[2], z[3]);
+          } else {
+            T* out = static_cast<T*>(a.out) + at * a.dim + i + k;
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack(z[0], z[1], (T*)nullptr), pack(z[2], z[3], (T*)nullptr));
+          }
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, cols);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static EncodeFn fn = nullptr;
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+  }
+  return fn;
+}
+
+// Pool of pages as {column, head, slot, page}; a box is one head's 64 columns
+// of a page's slots (at most 128), in 128-byte rows with the 128-byte swizzle.
+int make_map(CUtensorMap* tm, const void* base, const AttnArgs& a, int dtype, int64_t page, int64_t slot, int64_t head) {
+  EncodeFn enc = encode_fn();
+  KB_REQUIRE(enc != nullptr, KB_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[4] = {(cuuint64_t)a.dim, (cuuint64_t)a.heads_kv, (cuuint64_t)a.page_size, (cuuint64_t)a.pages};
+  cuuint64_t strides[3] = {(cuuint64_t)head * 2, (cuuint64_t)slot * 2, (cuuint64_t)page * 2};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)std::min(a.page_size, kTile), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = enc(tm, dtype == KB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                         const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  KB_REQUIRE(r == CUDA_SUCCESS, KB_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return KB_OK;
+}
+
+template <typename T>
+int launch_as(const AttnArgs& a, int dtype, int row_tiles, cudaStream_t stream) {
+  CUtensorMap tk, tv;
+  if (int st = make_map(&tk, a.k, a, dtype, a.k_p, a.k_s, a.k_h)) return st;
+  if (int st = make_map(&tv, a.v, a, dtype, a.v_p, a.v_s, a.v_h)) return st;
+  static uint64_t attr_set = 0;  // one bit per device ordinal
+  int dev = 0;
+  KB_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !(attr_set >> dev & 1)) {
+    KB_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    if (dev < 64) attr_set |= 1ull << dev;
+  }
+  attn_prefix_kernel<T><<<(unsigned)a.prefix_items, kThreads, kSmemBytes, stream>>>(tk, tv, a, row_tiles);
+  return check_launch("kb_shared_prefix_attention");
+}
+
+}  // namespace
+
+int tc_tile_rows(int64_t rows) { return rows <= kTile ? kTile : 2 * kTile; }
+
+bool tc_fits(const AttnArgs& a, int dtype) {
+  // a page is a whole part of a 128-key tile, of at least one swizzle group, or whole tiles
+  const bool pages = (kTile % a.page_size == 0 && a.page_size >= 8) || a.page_size % kTile == 0;
+  auto stride = [](int64_t s) { return s > 0 && s * 2 < ((int64_t)1 << 40); };
+  return dtype != KB_F32 && a.dim <= kTile && a.prefix_pages > 0 && pages && stride(a.k_p) && stride(a.k_s) &&
+         stride(a.k_h) && stride(a.v_p) && stride(a.v_s) && stride(a.v_h);
+}
+
+int tc_launch(const AttnArgs& a, int dtype, cudaStream_t stream) {
+  const int row_tiles = tc_tile_rows((int64_t)a.batch * a.queries * a.group) / kTile;
+  return dtype == KB_F16 ? launch_as<__half>(a, dtype, row_tiles, stream)
+                         : launch_as<__nv_bfloat16>(a, dtype, row_tiles, stream);
+}
+
+int tc_read_fault(bool clear, int* value) {
+  KB_CUDA(cudaMemcpyFromSymbol(value, g_fault, sizeof(int)));
+  if (clear) {
+    const int zero = 0;
+    KB_CUDA(cudaMemcpyToSymbol(g_fault, &zero, sizeof(int)));
+  }
+  return KB_OK;
+}
+
+}  // namespace attn
+}  // namespace lm
+}  // namespace kb
