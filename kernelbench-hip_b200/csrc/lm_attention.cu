@@ -68,7 +68,7 @@ __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uin
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -93,6 +93,7 @@ __device__ __forceinline__ void mma_3xtf32(float (&hh)[4], float (&x)[4], const 
   mma_tf32(hh, ah, b0.hi, b1.hi);
 }
 constexpr int kChain = 4;  // products of depth 8 chained in one accumulator
+constexpr int kWide = 4;   // accumulators in turn: a product does not wait for the one before it
 __device__ __forceinline__ uint32_t pack2(float x, float y, __half*) {
   const __half2 h = __floats2half2_rn(x, y);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -121,15 +122,19 @@ __device__ __forceinline__ void scores(float (&s)[NK / 8][4], const T* q, const 
         qa[i][0] = split(x[0]), qa[i][1] = split(x[8 * LD]), qa[i][2] = split(x[4]), qa[i][3] = split(x[8 * LD + 4]);
       }
 #pragma unroll
-      for (int n = 0; n < NK / 8; ++n) {
-        float hh[4] = {}, x[4] = {};
+      for (int n0 = 0; n0 < NK / 8; n0 += kWide) {
+        float hh[kWide][4] = {}, x[kWide][4] = {};
 #pragma unroll
-        for (int i = 0; i < kChain; ++i) {
-          const float* y = k + (n * 8 + r) * LD + d0 + 8 * i + c;
-          mma_3xtf32(hh, x, qa[i], split(y[0]), split(y[4]));
-        }
+        for (int i = 0; i < kChain; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[n][i] += hh[i] + x[i];
+          for (int n = 0; n < kWide && n0 + n < NK / 8; ++n) {
+            const float* y = k + ((n0 + n) * 8 + r) * LD + d0 + 8 * i + c;
+            mma_3xtf32(hh[n], x[n], qa[i], split(y[0]), split(y[4]));
+          }
+#pragma unroll
+        for (int n = 0; n < kWide && n0 + n < NK / 8; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[n0 + n][i] += hh[n][i] + x[n][i];
       }
     }
   } else {
@@ -167,15 +172,19 @@ __device__ __forceinline__ void weigh(float (&o)[DP / 8][4], const float (&p)[NK
         pa[i][0] = split(x[0]), pa[i][1] = split(x[2]), pa[i][2] = split(x[1]), pa[i][3] = split(x[3]);
       }
 #pragma unroll
-      for (int d = 0; d < DP / 8; ++d) {
-        float hh[4] = {}, x[4] = {};
+      for (int d0 = 0; d0 < DP / 8; d0 += kWide) {
+        float hh[kWide][4] = {}, x[kWide][4] = {};
 #pragma unroll
-        for (int i = 0; i < kKeys; ++i) {
-          const float* y = v + ((n0 + i) * 8 + 2 * c) * LD + d * 8 + r;
-          mma_3xtf32(hh, x, pa[i], split(y[0]), split(y[LD]));
-        }
+        for (int i = 0; i < kKeys; ++i)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[d][i] += hh[i] + x[i];
+          for (int d = 0; d < kWide; ++d) {
+            const float* y = v + ((n0 + i) * 8 + 2 * c) * LD + (d0 + d) * 8 + r;
+            mma_3xtf32(hh[d], x[d], pa[i], split(y[0]), split(y[LD]));
+          }
+#pragma unroll
+        for (int d = 0; d < kWide; ++d)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[d0 + d][i] += hh[d][i] + x[d][i];
       }
     }
   } else {
@@ -244,24 +253,29 @@ __device__ __forceinline__ void softmax_step(float (&s)[NK / 8][4], float (&o)[N
 }
 
 // ------------------------------------------------------------------ rows kernel
-// Four warps of 16 rows each share tiles of NK keys and values, double
-// buffered by cp.async.
+// Warps of 16 rows each share tiles of NK keys and values, double buffered by
+// cp.async.  fp32: eight warps, so that one CTA, which is all that shared
+// memory holds at 128 columns, fills the SM.
+template <typename T>
+constexpr int rows_warps() {
+  return sizeof(T) == 4 ? 8 : 4;
+}
 template <typename T, int DP, int NK>
 struct RowsCfg {
-  static constexpr int kRows = 64, kThreads = 128;
+  static constexpr int kWarps = rows_warps<T>(), kRows = 16 * kWarps, kThreads = 32 * kWarps;
   static constexpr int LD = DP + 16 / (int)sizeof(T);  // rows 16 bytes apart in the banks
   static constexpr size_t kSmem = sizeof(T) * LD * (kRows + 4 * NK);
 };
 
 template <typename T, int DP, int NK>
-__global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(RowsCfg<T, DP, NK>::kThreads) attn_rows_kernel(AttnArgs a) {
   using C = RowsCfg<T, DP, NK>;
   constexpr int LD = C::LD, kVec = 16 / sizeof(T), kPerRow = DP / kVec;
   extern __shared__ __align__(16) uint8_t raw[];
   T* sq = reinterpret_cast<T*>(raw);
   T* sk = sq + C::kRows * LD;
   T* sv = sk + 2 * NK * LD;
-  __shared__ int s_max[4];
+  __shared__ int s_max[C::kWarps];
   allow_next();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Item w = item_at(a, a.first_item + blockIdx.x, C::kRows);
@@ -281,7 +295,10 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
   low = __reduce_min_sync(0xffffffffu, low);
   if (lane == 0) s_max[warp] = top;
   __syncthreads();
-  const int end = min(w.k1, max(max(s_max[0], s_max[1]), max(s_max[2], s_max[3])));
+  int end = 0;
+#pragma unroll
+  for (int i = 0; i < C::kWarps; ++i) end = max(end, s_max[i]);
+  end = min(end, w.k1);
 
   const T* kp = static_cast<const T*>(a.k) + w.h * a.k_h;
   const T* vp = static_cast<const T*>(a.v) + w.h * a.v_h;
@@ -366,6 +383,7 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
       }
     }
   }
+  wait_for_previous();  // as in the keys kernel
 }
 
 // ------------------------------------------------------------------ keys kernel
@@ -373,7 +391,9 @@ __global__ void __launch_bounds__(128) attn_rows_kernel(AttnArgs a) {
 // a ring of its own filled by cp.async (no barrier until the end), and its own
 // running softmax; the four are joined in shared memory.  This is the shape of
 // decoding: a few query heads per key head against a sequence's own keys,
-// bound by the bytes of the cache.
+// bound by the bytes of the cache.  Two stages at 128 columns: three CTAs per
+// SM rather than two with three (64 sequences of up to 1000 keys: 42 against
+// 47 us).
 template <typename T, int DP, int NK, int STAGES>
 struct KeysCfg {
   static constexpr int kRows = 16, kWarps = 4, kThreads = 128;
@@ -503,6 +523,9 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
   __syncthreads();
   // eight threads a row
   const int r = tid >> 3;
+  // Where this launch began before the prefix's had ended: it ends after it, so
+  // that the join, which waits for this one, has both.
+  if (tid == 127) wait_for_previous();
   if (r >= w.rows) return;
   float m = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
   const float base = m == -INFINITY ? 0.0f : m;
@@ -611,7 +634,7 @@ struct Plan {
 // One axis of keys for `sets` sets of `rows` query rows each: the kernel by
 // the number of rows, and ranges of keys that give every SM a few CTAs but no
 // CTA less than one block of keys.
-Part plan_part(int64_t sets, int64_t rows, int64_t keys, bool tensor) {
+Part plan_part(int64_t sets, int64_t rows, int64_t keys, int dtype, bool tensor) {
   Part p;
   if (keys <= 0) return p;
   p.kind = rows <= 16 ? kKeys : tensor ? kTensor : kRows;
@@ -630,8 +653,9 @@ Part plan_part(int64_t sets, int64_t rows, int64_t keys, bool tensor) {
     }
     return p;
   }
-  p.tiles = (int)ceil_div(rows, p.kind == kKeys ? 16 : 64);
-  const int64_t block = 64, least = p.kind == kKeys ? block : 4 * block;
+  const int tile = p.kind == kKeys ? 16 : 16 * (dtype == KB_F32 ? rows_warps<float>() : rows_warps<__half>());
+  p.tiles = (int)ceil_div(rows, tile);
+  const int64_t block = 64, least = p.kind == kKeys ? block : 2 * block;
   const int64_t items = p.tiles * sets;
   const int64_t s = std::max<int64_t>(1, std::min(ceil_div((int64_t)4 * sm_count(), items), ceil_div(keys, least)));
   p.chunk = (int)(ceil_div(ceil_div(keys, s), block) * block);
@@ -639,9 +663,10 @@ Part plan_part(int64_t sets, int64_t rows, int64_t keys, bool tensor) {
   return p;
 }
 Plan plan(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv, int64_t prefix_keys, int64_t own_keys,
-          bool tensor) {
+          int dtype, bool tensor) {
   const int64_t rows = queries * (heads_q / heads_kv);
-  return {plan_part(heads_kv, batch * rows, prefix_keys, tensor), plan_part(heads_kv * batch, rows, own_keys, false)};
+  return {plan_part(heads_kv, batch * rows, prefix_keys, dtype, tensor),
+          plan_part(heads_kv * batch, rows, own_keys, dtype, false)};
 }
 size_t plan_bytes(const Plan& p, int64_t rows, int64_t dim) {
   return p.splits() <= 1 ? 0 : (size_t)p.splits() * rows * (dim + 1) * sizeof(float);
@@ -657,7 +682,8 @@ cudaLaunchAttribute after_start() {
 }
 
 template <typename K>
-int launch(K kern, size_t smem, AttnArgs a, int64_t first, int64_t items, uint64_t& attr_set, cudaStream_t stream) {
+int launch(K kern, int threads, size_t smem, AttnArgs a, int64_t first, int64_t items, uint64_t& attr_set,
+           cudaStream_t stream) {
   if (items == 0) return KB_OK;
   int dev = 0;
   KB_CUDA(cudaGetDevice(&dev));
@@ -666,30 +692,37 @@ int launch(K kern, size_t smem, AttnArgs a, int64_t first, int64_t items, uint64
     if (dev < 64) attr_set |= 1ull << dev;
   }
   a.first_item = first;
-  kern<<<(unsigned)items, 128, smem, stream>>>(a);
-  return check_launch("kb_shared_prefix_attention");
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute attr = after_start();
+  config.gridDim = dim3((unsigned)items), config.blockDim = dim3(threads), config.dynamicSmemBytes = smem;
+  config.stream = stream, config.attrs = &attr;
+  // the sequences' own keys need nothing of the prefix: their CTAs fill the SMs that it leaves
+  config.numAttrs = first > 0 ? 1 : 0;
+  KB_CUDA(cudaLaunchKernelEx(&config, kern, a));
+  return KB_OK;
 }
 template <typename T, int DP, int NK>
 int launch_rows(const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {
   static uint64_t attr_set = 0;
-  return launch(attn_rows_kernel<T, DP, NK>, RowsCfg<T, DP, NK>::kSmem, a, first, items, attr_set, stream);
+  using C = RowsCfg<T, DP, NK>;
+  return launch(attn_rows_kernel<T, DP, NK>, C::kThreads, C::kSmem, a, first, items, attr_set, stream);
 }
 template <typename T, int DP, int NK, int STAGES>
 int launch_keys(const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {
   static uint64_t attr_set = 0;
-  return launch(attn_keys_kernel<T, DP, NK, STAGES>, KeysCfg<T, DP, NK, STAGES>::kSmem, a, first, items, attr_set,
-                stream);
+  return launch(attn_keys_kernel<T, DP, NK, STAGES>, 128, KeysCfg<T, DP, NK, STAGES>::kSmem, a, first, items,
+                attr_set, stream);
 }
 template <typename T>
 int launch_kind(Kind kind, const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {
   constexpr bool f32 = sizeof(T) == 4;
   if (kind == kKeys) {
     if (a.dim <= 64) return launch_keys<T, 64, 16, 4>(a, first, items, stream);
-    if (a.dim <= 128) return launch_keys<T, 128, 16, 3>(a, first, items, stream);
+    if (a.dim <= 128) return launch_keys<T, 128, 16, 2>(a, first, items, stream);
     return launch_keys<T, 256, f32 ? 8 : 16, 3>(a, first, items, stream);
   }
   if (a.dim <= 64) return launch_rows<T, 64, 64>(a, first, items, stream);
-  if (a.dim <= 128) return launch_rows<T, 128, 64>(a, first, items, stream);
+  if (a.dim <= 128) return launch_rows<T, 128, f32 ? 32 : 64>(a, first, items, stream);
   return launch_rows<T, 256, f32 ? 32 : 64>(a, first, items, stream);
 }
 
@@ -707,7 +740,7 @@ size_t kb_shared_prefix_attention_workspace_size(int64_t batch, int64_t queries,
   if (heads_q % heads_kv) return 0;
   auto bytes = [&](bool tensor) {
     return plan_bytes(plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size,
-                           std::max<int64_t>(0, width - prefix_pages) * page_size, tensor),
+                           std::max<int64_t>(0, width - prefix_pages) * page_size, dtype, tensor),
                       batch * queries * heads_q, dim);
   };
   // strides decide whether the tensor-core kernel can take the prefix
@@ -763,7 +796,7 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
   a.k_p = k_stride_page, a.k_s = k_stride_slot, a.k_h = k_stride_head;
   a.v_p = v_stride_page, a.v_s = v_stride_slot, a.v_h = v_stride_head;
   a.scale_log2 = scale * kLog2e;
-  const Plan p = plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size, own_pages * page_size,
+  const Plan p = plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size, own_pages * page_size, dtype,
                       tc_fits(a, dtype));
   a.splits = p.splits();
   a.prefix_tiles = p.prefix.tiles, a.prefix_splits = p.prefix.splits, a.prefix_chunk = p.prefix.chunk;

@@ -21,7 +21,7 @@ __device__ __forceinline__ float ex2(float x) {
 // down to 2^-14 only, so its weights are held 2^kShift higher (far below its
 // largest), and small ones do not lose bits; bf16 has fp32's range.
 template <typename T>
-constexpr float kShift = std::is_same_v<T, __half> ? 10.0f : 0.0f;
+constexpr float kShift = std::is_same_v<T, __half> ? 7.0f : 0.0f;
 
 // Lets the next launch begin where it was made with programmatic stream
 // serialisation; it waits for this one's results by itself.

@@ -12,14 +12,17 @@
 // moves when the maximum has grown past it by more than 2^kSlack, and then the
 // row's O is scaled in TMEM (rare after the first tiles); l and O carry the
 // same m, so it cancels in O / l.  l sums the unrounded exponentials in fp32.
+// (kSlack 4 scaled some row of nearly every warp in the first ten key tiles of
+// scores of deviation 2, a thousand cycles each; 8 scales almost none.)
 //
 // Roles (10 warps): warps 0-3 and 4-7 are the softmax of the two row tiles,
 // warp 8 loads K and V tiles by TMA, one copy per page and 64 columns (the
 // page table is the gather), warp 9 issues the products in the order
 //   O_0 += P_0 V_j, S_0 = Q_0 K_j+1, O_1 += P_1 V_j, S_1 = Q_1 K_j+1
-// so that one row tile's products run during the other's softmax.  The
-// products of a thread are executed in order, so S_t(j + 1) may overwrite the
-// P_t(j) that the product before it reads.
+// so that one row tile's products run during the other's softmax; O += P V
+// begins with the first 64 keys while the others' exponentials are computed.
+// The products of a thread are executed in order, so S_t(j + 1) may overwrite
+// the P_t(j) that the product before it reads.
 //
 // TMEM (512 columns): S_0, S_1 (P_t in the first 64 columns of S_t), O_0, O_1.
 // Shared memory: Q 64 KB, two stages of K and of V, 32 KB each, all in rows of
@@ -29,7 +32,14 @@
 //
 // Bound: 4 rows keys dim operations on the tensor cores, and as many cycles
 // again of exponentials (16 per clock and SM against 128 x 128 x 128 products
-// in 512 cycles), which overlap.
+// in 512 cycles), which overlap.  What it measured: per key tile and row tile a
+// softmax takes 2400 cycles (85 for the load, 320 for the maximum, 1800 for the
+// exponentials, 170 for the store), O 520, S 820 (both operands from shared
+// memory: 8 KB per 64 cycles of product), and this chain, not a unit, sets the
+// pace.  256 samples x 32 heads x 128 over 32768 keys, bf16: 0.16 ms,
+// 850 TFLOP/s, 52 % of a large library product's 1650.  Tried and slower: steps
+// of 64 keys with two buffers for S (a product of 128 x 64 takes as long as one
+// of 128 x 128), two threads per row (spills at 96 registers).
 //
 // Every wait is bounded: one that runs out raises the CTA's abort flag and the
 // device's fault word, every role leaves, copies in flight are waited for
@@ -56,7 +66,7 @@ constexpr int kThreads = 320;
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
 constexpr int kSmemBytes = (2 + 2 * kStages) * kTileBytes + 256 + 1024;  // + barriers, alignment
 constexpr uint64_t kWaitLimitNs = 2000000000ull;
-constexpr float kSlack = 4.0f;                  // log2 of how far a maximum may pass the reference
+constexpr float kSlack = 8.0f;                  // log2 of how far a maximum may pass the reference
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -87,10 +97,11 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
 }
 // False once this or another CTA has given up, or after kWaitLimitNs.
 __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
-  const uint64_t t0 = globaltimer();
+  uint64_t t0 = 0;
   for (uint32_t n = 1;; ++n) {
     if (mbar_try_wait(bar, parity)) return true;
     if ((n & 63) == 0) {
+      if (t0 == 0) t0 = globaltimer();  // most waits end before the first look at the clock
       if (*abort_flag || *(volatile int*)&g_fault) {
         *abort_flag = 1;
         return false;
@@ -192,6 +203,10 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 // elements of the contraction per row; a step of 16 advances 32 bytes.
 // MN-major (V): 64 columns per row, one row per key; the next 64 columns lie
 // LBO = kHalfBytes further; a step of 16 keys advances 2048 bytes.
+// Addresses in it count 16 bytes: advanced(d, bytes) moves a descriptor on
+// with one addition, which matters to the one thread that issues a product
+// every 32 to 64 cycles.
+__device__ __forceinline__ uint64_t advanced(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
 __device__ __forceinline__ uint64_t make_desc(uint32_t saddr, uint32_t lbo) {
   return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)((lbo >> 4) & 0x3FFFu) << 16 | (uint64_t)(1024 >> 4) << 32 |
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
@@ -213,7 +228,32 @@ __device__ __forceinline__ uint32_t pack(float x, float y, __nv_bfloat16*) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-template <typename T>
+// Two fp32 values in a 64-bit register, and operations on both at once.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
+template <typename T, int HALVES>
 __global__ void __launch_bounds__(kThreads, 1)
 attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, AttnArgs a,
                    int row_tiles) {
@@ -230,9 +270,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   auto v_full = [&](int s) { return bar(6 + s); };
   auto v_empty = [&](int s) { return bar(8 + s); };
   auto s_full = [&](int t) { return bar(10 + t); };
-  auto p_full = [&](int t) { return bar(12 + t); };
-  auto o_full = [&](int t) { return bar(14 + t); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  auto p_full = [&](int t, int half) { return bar(12 + 2 * t + half); };
+  auto o_full = [&](int t) { return bar(16 + t); };
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_end = reinterpret_cast<int*>(tmem_slot + 2);
   allow_next();
@@ -244,7 +284,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     for (int t = 0; t < 2; ++t) {
       mbar_init(q_full + 8 * t, kTile);
       mbar_init(s_full(t), 1);
-      mbar_init(p_full(t), kTile);
+      mbar_init(p_full(t, 0), kTile);
+      mbar_init(p_full(t, 1), kTile);
       mbar_init(o_full(t), 1);
     }
     for (int s = 0; s < kStages; ++s) {
@@ -277,7 +318,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   const uint32_t tmem = *tmem_slot;
   const int end = min(w.k1, *s_end);
   const int n = end > w.k0 ? (end - w.k0 + kTile - 1) / kTile : 0;
-  const int halves = a.dim > 64 ? 2 : 1;
+  constexpr int halves = HALVES;  // of 64 columns; columns past dim are zeros
   const uint32_t o_col = row_tiles == 2 ? 256 : 128;
 
   if (warp == kLoadWarp) {
@@ -322,13 +363,16 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   } else if (warp == kMmaWarp) {
     // ---------------- products
     if (lane == 0 && n > 0) {
-      const int depth = (a.dim + 15) / 16;  // steps of 16 columns of Q and K
-      const uint32_t idesc_s = make_idesc<T>(kTile, false), idesc_o = make_idesc<T>(depth * 16, true);
+      constexpr int kDepth = HALVES * 4;
+      constexpr uint32_t idesc_s = make_idesc<T>(kTile, false), idesc_o = make_idesc<T>(HALVES * 64, true);
+      const uint64_t q_desc = make_desc(smem_u32(s_q), 16), k_desc = make_desc(smem_u32(s_k), 16),
+                     v_desc = make_desc(smem_u32(s_v), kHalfBytes);
       auto scores = [&](int i, int s) {
-        for (int k = 0; k < depth; ++k) {
+        const uint64_t q = advanced(q_desc, i * kTileBytes), kd = advanced(k_desc, s * kTileBytes);
+#pragma unroll
+        for (int k = 0; k < kDepth; ++k) {
           const uint32_t off = (k >> 2) * kHalfBytes + (k & 3) * 32;
-          mma_ss(tmem + i * kTile, make_desc(smem_u32(s_q + i * kTileBytes) + off, 16),
-                 make_desc(smem_u32(s_k + s * kTileBytes) + off, 16), idesc_s, k > 0);
+          mma_ss(tmem + i * kTile, advanced(q, off), advanced(kd, off), idesc_s, k > 0);
         }
         mma_commit(s_full(i));
       };
@@ -344,13 +388,18 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         const int s = j % kStages, next = (j + 1) % kStages;
         const uint32_t parity = (j / kStages) & 1, next_parity = ((j + 1) / kStages) & 1;
         for (int i = 0; i < row_tiles && alive; ++i) {
-          alive = mbar_wait(p_full(i), j & 1, abort_flag) && (i > 0 || mbar_wait(v_full(s), parity, abort_flag));
-          if (!alive) break;
-          tc_fence_after();
+          alive = i > 0 || mbar_wait(v_full(s), parity, abort_flag);
 #pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            mma_ts(tmem + o_col + i * kTile, tmem + i * kTile + k * 8,
-                   make_desc(smem_u32(s_v + s * kTileBytes) + k * 2048, kHalfBytes), idesc_o, j > 0 || k > 0);
+          for (int half = 0; half < 2; ++half) {  // each half of P as soon as it is there
+            alive = alive && mbar_wait(p_full(i, half), j & 1, abort_flag);
+            if (!alive) break;
+            tc_fence_after();
+#pragma unroll
+            for (int k = half * 4; k < half * 4 + 4; ++k)
+              mma_ts(tmem + o_col + i * kTile, tmem + i * kTile + k * 8,
+                     advanced(v_desc, s * kTileBytes + k * 2048), idesc_o, j > 0 || k > 0);
+          }
+          if (!alive) break;
           mma_commit(o_full(i));
           if (i == row_tiles - 1) mma_commit(v_empty(s));
           if (j + 1 < n) {
@@ -406,7 +455,11 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       }
       float top[4] = {f(0), f(1), f(2), f(3)};
 #pragma unroll
-      for (int i = 4; i < kTile; ++i) top[i & 3] = fmaxf(top[i & 3], f(i));
+      for (int i = 4; i < kTile - 4; i += 8)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top[k] = max3(top[k], f(i + k), f(i + k + 4));
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], f(kTile - 4 + k));
       const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
       // move the reference where the maximum has outgrown it
       const bool move = now > m + kSlack;  // also from -inf; not for a NaN
@@ -431,30 +484,38 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         }
       }
       const float base = (m == -INFINITY ? 0.0f : m) - kShift<T>;
-      float sum[4] = {};
+      const uint64_t cc = pair(c, c), bb = pair(-base, -base);
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int i = 0; i < kTile; i += 2) {
-        const float p0 = ex2(fmaf(f(i), c, -base)), p1 = ex2(fmaf(f(i + 1), c, -base));
-        sum[i & 2] += p0;
-        sum[(i & 2) + 1] += p1;
-        x[i >> 1] = pack(p0, p1, (T*)nullptr);
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int i = half * kTile / 2; i < (half + 1) * kTile / 2; i += 2) {
+          float p0, p1;
+          unpair(fma2(pair(f(i), f(i + 1)), cc, bb), p0, p1);
+          p0 = ex2(p0);
+          p1 = ex2(p1);
+          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair(p0, p1));
+          x[i >> 1] = pack(p0, p1, (T*)nullptr);
+        }
+        tmem_st(s_addr + half * 32, x + half * 32);
+        tmem_st_wait();
+        // V rows that nobody sees, in a page that is partly seen: zeros, for 0 x NaN
+        if (half == 0 && j == n - 1 && t == 0 && end < w.k0 + n * kTile && end % a.page_size != 0) {
+          ok = warp_wait(v_full(j % kStages), (j / kStages) & 1, abort_flag);
+          if (!ok) break;
+          if (w.k0 + j * kTile + row >= end)
+            for (int i = 0; i < halves * 8; ++i)
+              *reinterpret_cast<uint4*>(s_v + (j % kStages) * kTileBytes + (i >> 3) * kHalfBytes + row * 128 +
+                                        ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async();
+        }
+        tc_fence_before();
+        mbar_arrive(p_full(t, half));
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st(s_addr, x);
-      tmem_st(s_addr + 32, x + 32);
-      tmem_st_wait();
-      // V rows that nobody sees, in a page that is partly seen: zeros, for 0 x NaN
-      if (j == n - 1 && t == 0 && end < w.k0 + n * kTile && end % a.page_size != 0) {
-        ok = warp_wait(v_full(j % kStages), (j / kStages) & 1, abort_flag);
-        if (!ok) break;
-        if (w.k0 + j * kTile + row >= end)
-          for (int i = 0; i < halves * 8; ++i)
-            *reinterpret_cast<uint4*>(s_v + (j % kStages) * kTileBytes + (i >> 3) * kHalfBytes + row * 128 +
-                                      ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async();
-      }
-      tc_fence_before();
-      mbar_arrive(p_full(t));
+      if (!ok) break;
+      float l0, l1;
+      unpair(add2(sum[0], sum[1]), l0, l1);
+      l += l0 + l1;
     }
     if (ok && n > 0) ok = warp_wait(o_full(t), (n - 1) & 1, abort_flag);
     tc_fence_after();
@@ -532,7 +593,7 @@ int make_map(CUtensorMap* tm, const void* base, const AttnArgs& a, int dtype, in
   return KB_OK;
 }
 
-template <typename T>
+template <typename T, int HALVES>
 int launch_as(const AttnArgs& a, int dtype, int row_tiles, cudaStream_t stream) {
   CUtensorMap tk, tv;
   if (int st = make_map(&tk, a.k, a, dtype, a.k_p, a.k_s, a.k_h)) return st;
@@ -541,10 +602,10 @@ int launch_as(const AttnArgs& a, int dtype, int row_tiles, cudaStream_t stream) 
   int dev = 0;
   KB_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !(attr_set >> dev & 1)) {
-    KB_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
+    KB_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<T, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
     if (dev < 64) attr_set |= 1ull << dev;
   }
-  attn_prefix_kernel<T><<<(unsigned)a.prefix_items, kThreads, kSmemBytes, stream>>>(tk, tv, a, row_tiles);
+  attn_prefix_kernel<T, HALVES><<<(unsigned)a.prefix_items, kThreads, kSmemBytes, stream>>>(tk, tv, a, row_tiles);
   return check_launch("kb_shared_prefix_attention");
 }
 
@@ -562,8 +623,11 @@ bool tc_fits(const AttnArgs& a, int dtype) {
 
 int tc_launch(const AttnArgs& a, int dtype, cudaStream_t stream) {
   const int row_tiles = tc_tile_rows((int64_t)a.batch * a.queries * a.group) / kTile;
-  return dtype == KB_F16 ? launch_as<__half>(a, dtype, row_tiles, stream)
-                         : launch_as<__nv_bfloat16>(a, dtype, row_tiles, stream);
+  if (a.dim <= 64)
+    return dtype == KB_F16 ? launch_as<__half, 1>(a, dtype, row_tiles, stream)
+                           : launch_as<__nv_bfloat16, 1>(a, dtype, row_tiles, stream);
+  return dtype == KB_F16 ? launch_as<__half, 2>(a, dtype, row_tiles, stream)
+                         : launch_as<__nv_bfloat16, 2>(a, dtype, row_tiles, stream);
 }
 
 int tc_read_fault(bool clear, int* value) {
