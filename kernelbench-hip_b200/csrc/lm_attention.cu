@@ -36,6 +36,9 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool vali
   const int bytes = valid ? 16 : 0;
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
@@ -232,17 +235,22 @@ __device__ __forceinline__ void softmax_step(float (&s)[NK / 8][4], float (&o)[N
   for (int r = 0; r < 2; ++r) {
     top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
     top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-    const float base = top[r] == -INFINITY ? 0.0f : top[r];
-    const float keep = ex2(st.m[r] - base);
-    st.m[r] = top[r];
-    st.l[r] *= keep;
-#pragma unroll
-    for (int d = 0; d < ND; ++d) {
-      o[d][2 * r] *= keep;
-      o[d][2 * r + 1] *= keep;
-    }
-    top[r] = base - kShift<T>;
   }
+  if (__any_sync(0xffffffffu, top[0] != st.m[0] || top[1] != st.m[1])) {  // a maximum has moved
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float keep = ex2(st.m[r] - (top[r] == -INFINITY ? 0.0f : top[r]));
+      st.m[r] = top[r];
+      st.l[r] *= keep;
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        o[d][2 * r] *= keep;
+        o[d][2 * r + 1] *= keep;
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 2; ++r) top[r] = (top[r] == -INFINITY ? 0.0f : top[r]) - kShift<T>;
 #pragma unroll
   for (int n = 0; n < NK / 8; ++n)
 #pragma unroll
@@ -451,7 +459,20 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
   auto load = [&](int key0, const Place& p, int stage) {
     T* sk = mine + stage * C::kStage;
     T* sv = sk + NK * LD;
+    if (alike && key0 + NK <= end && a.dim == DP && kPerRow <= 32) {
+      // a whole block: every copy of a lane has the same column
+      constexpr int kRowsAt = kPerRow <= 32 ? 32 / kPerRow : 1;
+      const int n0 = lane / kPerRow, c = lane % kPerRow * kVec;
+      const uint32_t dst = smem_addr(sk + n0 * LD + c);
 #pragma unroll
+      for (int i = 0; i < NK / kRowsAt; ++i) {
+        const int64_t at = __shfl_sync(0xffffffffu, p.k, i * kRowsAt + n0) + c;
+        copy16(dst + i * kRowsAt * LD * (int)sizeof(T), kp + at);
+        copy16(dst + (NK + i * kRowsAt) * LD * (int)sizeof(T), vp + at);
+      }
+      return;
+    }
+#pragma unroll 1
     for (int i = 0; i < NK * kPerRow / 32; ++i) {
       const int at = i * 32 + lane, n = at / kPerRow, c = at % kPerRow * kVec;
       const int64_t k = __shfl_sync(0xffffffffu, p.k, n);
