@@ -182,6 +182,42 @@ struct Pairs {
       b[0] = t0, b[2] = b[1], b[1] = t1;
     }
   }
+  // the same in pairs of fp32: (a0, a1), (a2, a3)
+  template <typename T>
+  __device__ void get(const Raw8<T>& r, uint64_t (&a)[2], uint64_t (&b)[2]) const {
+    float x[4], y[4];
+    get(r, x, y);
+    a[0] = pair(x[0], x[1]), a[1] = pair(x[2], x[3]), b[0] = pair(y[0], y[1]), b[1] = pair(y[2], y[3]);
+  }
+  template <typename T>
+  __device__ void store(T* x, const uint64_t (&a)[2], const uint64_t (&b)[2]) const {
+    float u[4], v[4];
+    unpair(a[0], u[0], u[1]), unpair(a[1], u[2], u[3]), unpair(b[0], v[0], v[1]), unpair(b[1], v[2], v[3]);
+    store(x, u, v);
+  }
+  // (u, v) = (a uc + b us, b vc + a vs); a pair that does not turn takes no product with its partner, which may
+  // be infinite
+  __device__ void turned(const uint64_t (&a)[2], const uint64_t (&b)[2], const uint64_t (&uc)[2], const uint64_t (&us)[2],
+                         const uint64_t (&vc)[2], const uint64_t (&vs)[2], uint64_t (&u)[2], uint64_t (&v)[2]) const {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) u[i] = mul2(a[i], uc[i]), v[i] = mul2(b[i], vc[i]);
+    if (turns(3)) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) u[i] = fma2(b[i], us[i], u[i]), v[i] = fma2(a[i], vs[i], v[i]);
+    } else if (turns(0)) {
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        if (!turns(j)) continue;
+        float x[2], y[2], p[2], q[2], s[2], t[2];
+        unpair(u[j >> 1], x[0], x[1]), unpair(v[j >> 1], y[0], y[1]);
+        unpair(a[j >> 1], p[0], p[1]), unpair(b[j >> 1], q[0], q[1]);
+        unpair(us[j >> 1], s[0], s[1]), unpair(vs[j >> 1], t[0], t[1]);
+        x[j & 1] += q[j & 1] * s[j & 1];
+        y[j & 1] += p[j & 1] * t[j & 1];
+        u[j >> 1] = pair(x[0], x[1]), v[j >> 1] = pair(y[0], y[1]);
+      }
+    }
+  }
   template <typename T>
   __device__ void store(T* x, float (&a)[4], float (&b)[4]) const {
     if (LAYOUT == kNeighbours) {
@@ -262,8 +298,8 @@ __global__ void __launch_bounds__(kVecThreads, 8) rope_forward(RopeArgs a, uint3
   const int last = min(h - group + a.unit_heads, heads);
   const T* x = static_cast<const T*>(a.x[which]) + (int64_t)t * a.stride_t[which];
   T* z = static_cast<T*>(a.out[which]) + (int64_t)t * heads * a.dim;
-  // z_a = r (x_a aa - x_b ab), z_b = r (x_b bb + x_a ba): the weights times cos and sin
-  float aa[4], ab[4], bb[4], ba[4];
+  // z_a = r (x_a aa + x_b ab), z_b = r (x_b bb + x_a ba): the weights times cos and sin
+  uint64_t aa[2], ab[2], bb[2], ba[2];
   bool ready = false;
   for (; h - group < last; h += kBatch * kGroups) {
     Raw8<T> xr[kBatch] = {};
@@ -275,30 +311,27 @@ __global__ void __launch_bounds__(kVecThreads, 8) rope_forward(RopeArgs a, uint3
       pr.table(a, t, c, s);
       pr.template weights<T>(a.w[which], a.weight32, wa, wb);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) aa[j] = wa[j] * c[j], ab[j] = wb[j] * s[j], bb[j] = wb[j] * c[j], ba[j] = wa[j] * s[j];
+      for (int i = 0; i < 2; ++i) {
+        const uint64_t ci = pair(c[2 * i], c[2 * i + 1]), si = pair(s[2 * i], s[2 * i + 1]);
+        const uint64_t wai = pair(wa[2 * i], wa[2 * i + 1]), wbi = pair(wb[2 * i], wb[2 * i + 1]);
+        aa[i] = mul2(wai, ci), ab[i] = mul2(mul2(wbi, si), pair(-1.0f, -1.0f));
+        bb[i] = mul2(wbi, ci), ba[i] = mul2(wai, si);
+      }
       ready = true;
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int at = h + k * kGroups;
       if (at - group >= last) break;
-      float xa[4], xb[4], ss = 0.0f;
+      uint64_t xa[2], xb[2], za[2], zb[2];
       pr.get(xr[k], xa, xb);
+      float s0, s1;
+      unpair(fma2(xa[0], xa[0], fma2(xa[1], xa[1], fma2(xb[0], xb[0], mul2(xb[1], xb[1])))), s0, s1);
+      const float r = rsqrtf(group_sum<L>(s0 + s1) * a.inv_dim + a.eps);
+      pr.turned(xa, xb, aa, ab, bb, ba, za, zb);
+      const uint64_t rr = pair(r, r);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) ss += xa[j] * xa[j] + xb[j] * xb[j];
-      const float r = rsqrtf(group_sum<L>(ss) * a.inv_dim + a.eps);
-      float za[4], zb[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        za[j] = xa[j] * aa[j];
-        zb[j] = xb[j] * bb[j];
-        if (pr.turns(j)) {  // not a product with 0: the partner may be infinite
-          za[j] -= xb[j] * ab[j];
-          zb[j] += xa[j] * ba[j];
-        }
-        za[j] *= r;
-        zb[j] *= r;
-      }
+      for (int i = 0; i < 2; ++i) za[i] = mul2(za[i], rr), zb[i] = mul2(zb[i], rr);
       if (at < last && pr.on) pr.store(z + at * a.dim, za, zb);
     }
   }
@@ -321,15 +354,25 @@ __global__ void __launch_bounds__(kVecThreads, 4) rope_backward(RopeArgs a) {
     const int64_t stride = a.stride_h[which];
     const uint32_t per_token = which ? a.units_token - a.units_q : a.units_q;
     const uint32_t units = (uint32_t)a.tokens * per_token;
-    float wa[4], wb[4], ga[4] = {}, gb[4] = {};
-    pr.template weights<T>(a.w[which], a.weight32, wa, wb);
+    uint64_t wa[2], wb[2], ga[2] = {}, gb[2] = {};
+    {
+      float u[4], v[4];
+      pr.template weights<T>(a.w[which], a.weight32, u, v);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) wa[i] = pair(u[2 * i], u[2 * i + 1]), wb[i] = pair(v[2 * i], v[2 * i + 1]);
+    }
     int terms = 0;
     auto flush = [&] {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        acc[warp][which * 8 + j][lane] += (double)ga[j];
-        acc[warp][which * 8 + 4 + j][lane] += (double)gb[j];
-        ga[j] = gb[j] = 0.0f;
+      for (int i = 0; i < 2; ++i) {
+        float u[2], v[2];
+        unpair(ga[i], u[0], u[1]), unpair(gb[i], v[0], v[1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          acc[warp][which * 8 + 2 * i + j][lane] += (double)u[j];
+          acc[warp][which * 8 + 4 + 2 * i + j][lane] += (double)v[j];
+        }
+        ga[i] = gb[i] = 0;
       }
       terms = 0;
     };
@@ -340,7 +383,7 @@ __global__ void __launch_bounds__(kVecThreads, 4) rope_backward(RopeArgs a) {
       const T* x = static_cast<const T*>(a.x[which]) + (int64_t)t * a.stride_t[which];
       const T* dz = static_cast<const T*>(a.dz[which]) + (int64_t)t * heads * a.dim;
       T* dx = static_cast<T*>(a.out[which]) + (int64_t)t * heads * a.dim;
-      float c[4], s[4];
+      uint64_t cc[2], sn[2], ns[2];
       Raw8<T> xr[kBatch] = {}, dr[kBatch] = {};
       auto fetch = [&](int k, int at) {
         if (at < last && pr.on) {
@@ -350,46 +393,48 @@ __global__ void __launch_bounds__(kVecThreads, 4) rope_backward(RopeArgs a) {
       };
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) fetch(k, h + k * kGroups);
-      pr.table(a, t, c, s);
+      {
+        float c[4], s[4];
+        pr.table(a, t, c, s);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          cc[i] = pair(c[2 * i], c[2 * i + 1]), sn[i] = pair(s[2 * i], s[2 * i + 1]);
+          ns[i] = pair(-s[2 * i], -s[2 * i + 1]);
+        }
+      }
       for (; h - group < last; h += kBatch * kGroups) {
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           const int at = h + k * kGroups;
           if (at - group >= last) break;
-          float xa[4], xb[4], da[4], db[4], ya[4], yb[4], ss = 0.0f, dot = 0.0f;
+          uint64_t xa[2], xb[2], da[2], db[2], ya[2], yb[2], ta[2], tb[2];
           pr.get(xr[k], xa, xb);
           pr.get(dr[k], da, db);
           fetch(k, at + kBatch * kGroups);  // the head that takes this one's place
-          float ta[4], tb[4];  // dy x
+          pr.turned(da, db, cc, sn, cc, ns, ya, yb);  // dy
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            ya[j] = da[j] * c[j];
-            yb[j] = db[j] * c[j];
-            if (pr.turns(j)) {
-              ya[j] += db[j] * s[j];
-              yb[j] -= da[j] * s[j];
-            }
-            ta[j] = ya[j] * xa[j];
-            tb[j] = yb[j] * xb[j];
-            ss += xa[j] * xa[j] + xb[j] * xb[j];
-            dot += ta[j] * wa[j] + tb[j] * wb[j];
-          }
+          for (int i = 0; i < 2; ++i) ta[i] = mul2(ya[i], xa[i]), tb[i] = mul2(yb[i], xb[i]);
+          float ss, dot, s1, d1;
+          unpair(fma2(xa[0], xa[0], fma2(xa[1], xa[1], fma2(xb[0], xb[0], mul2(xb[1], xb[1])))), ss, s1);
+          unpair(fma2(ta[0], wa[0], fma2(ta[1], wa[1], fma2(tb[0], wb[0], mul2(tb[1], wb[1])))), dot, d1);
+          ss += s1;
+          dot += d1;
 #pragma unroll
           for (int o = L / 2; o > 0; o >>= 1) {
             ss += __shfl_xor_sync(0xffffffffu, ss, o);
             dot += __shfl_xor_sync(0xffffffffu, dot, o);
           }
           const float r = rsqrtf(ss * a.inv_dim + a.eps);
-          const float m = r * dot * a.inv_dim * r;  // r mean(dy w xh)
+          const float m = -(r * dot * a.inv_dim * r);  // - r mean(dy w xh)
           const bool mine = at < last && pr.on;
+          const float rg = mine ? r : 0.0f;
+          const uint64_t rr = pair(r, r), mm = pair(m, m), rrg = pair(rg, rg);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (mine) {
-              ga[j] += ta[j] * r;
-              gb[j] += tb[j] * r;
-            }
-            ya[j] = r * (ya[j] * wa[j] - xa[j] * m);
-            yb[j] = r * (yb[j] * wb[j] - xb[j] * m);
+          for (int i = 0; i < 2; ++i) {
+            ga[i] = fma2(ta[i], rrg, ga[i]);
+            gb[i] = fma2(tb[i], rrg, gb[i]);
+            ya[i] = mul2(rr, fma2(xa[i], mm, mul2(ya[i], wa[i])));
+            yb[i] = mul2(rr, fma2(xb[i], mm, mul2(yb[i], wb[i])));
           }
           if (mine) pr.store(dx + at * a.dim, ya, yb);
         }
@@ -540,12 +585,12 @@ int backward_grid(int64_t tokens, int heads) {
 // Lanes per head: the power of two that holds dim / 8 of them.
 int lanes_for(int64_t dim) { return dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
 // Fills in the layout of the register kernels; returns the units of work.  A
-// unit takes up to 16 heads per group of lanes (cos, sin and weights are
-// prepared once for them), fewer while that leaves SMs without work.
-int64_t lay_out(RopeArgs& a) {
+// unit takes up to 4 * `most` heads per group of lanes (cos, sin and weights
+// are prepared once for them), fewer while that leaves SMs without work.
+int64_t lay_out(RopeArgs& a, int most) {
   const int step = 32 / lanes_for(a.dim) * 4;
   auto units = [&](int64_t heads) { return ceil_div(a.heads[0], heads) + ceil_div(a.heads[1], heads); };
-  a.unit_heads = step * 4;
+  a.unit_heads = step * most;
   while (a.unit_heads > step && a.tokens * units(a.unit_heads) < (int64_t)sm_count() * 64) a.unit_heads /= 2;
   a.units_q = (uint32_t)ceil_div(a.heads[0], a.unit_heads);
   a.units_token = (uint32_t)units(a.unit_heads);
@@ -630,7 +675,8 @@ int kb_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
   a.dim = (int)dim, a.rotary = (int)rotary, a.interleaved = interleaved, a.pos64 = positions_64, a.eps = eps;
   a.weight32 = weight_dtype == KB_F32;
   if (dim <= kVecDim) {
-    const int64_t units = lay_out(a), blocks = kb::ceil_div(units, kVecWarps);
+    // 16-bit, 16384 x 40 x 128: 66 us with 2, 68 with 4, 70 with 1; fp32, half the tokens: 57, 60, 55
+    const int64_t units = lay_out(a, dtype == KB_F32 ? 1 : 2), blocks = kb::ceil_div(units, kVecWarps);
     KB_REQUIRE(units <= kMaxUnits, KB_ERR_UNSUPPORTED, "%s: too many tokens", name);
     return with_dtype(dtype, [&](auto* x) {
       using T = std::remove_pointer_t<decltype(x)>;
@@ -696,7 +742,7 @@ int kb_qk_norm_rope_backward(const void* dq_out, const void* dk_out, const void*
     using T = std::remove_pointer_t<decltype(x)>;
     using W = std::remove_pointer_t<decltype(w)>;
     if (any && dim <= kVecDim) {
-      const int64_t units = lay_out(a);
+      const int64_t units = lay_out(a, dtype == KB_F32 ? 1 : 4);  // as above: 112 us with 4, 118 with 1; fp32 99, 92
       KB_REQUIRE(units <= kMaxUnits, KB_ERR_UNSUPPORTED, "%s: too many tokens", name);
       grid = (int)std::min<int64_t>(kb::ceil_div(units, kVecWarps), (int64_t)kb::sm_count() * 4);  // four per SM
       if (int st = with_layout(a, vector_ok(a, sizeof(T), true), [&](auto l, auto v) {
