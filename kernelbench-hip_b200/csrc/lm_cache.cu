@@ -20,6 +20,14 @@
 // including it are there: results do not depend on timing.  Page ids and
 // slots read from device memory are checked before use; one out of range is
 // passed over.
+//
+// The decisions are one CTA's (a chain of a few latencies, 5-7 us); the copies
+// run at HBM speed (64 children of one parent in 64 planes of 32 KB pages: 27
+// us for 134 MB written, the parent's page from L2).  The launches of a call
+// start while the one before ends (programmatic dependent launch), each waiting
+// for its results.  Rows of children that share their pages meet in refs: a
+// thread takes one column of 16 rows and adds a page's changes up before its
+// atomic.
 #include "lm_common.cuh"
 
 namespace kb {
@@ -28,6 +36,41 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxPages = 1 << 20, kMaxSlots = 1 << 20;
+
+// Programmatic dependent launch: the next launch may start once all CTAs have
+// passed allow_next(); it waits for this one's results in wait_for_previous().
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 blocks, unsigned threads, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.gridDim = blocks, config.blockDim = dim3(threads), config.stream = stream;
+  config.attrs = &attr, config.numAttrs = 1;
+  KB_CUDA(cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...));
+  return KB_OK;
+}
+
+// Changes of pages' counts that a thread meets one after the other, added up
+// while the page stays the same.
+struct Run {
+  int* refs;
+  int pages, page = -1, by = 0;
+  __device__ Run(int* r, int n) : refs(r), pages(n) {}
+  __device__ void flush() {
+    if (by) atomicAdd(&refs[page], by);
+    by = 0;
+  }
+  __device__ void add(int p, int v) {
+    if (p < 0 || p >= pages) return;
+    if (p != page) flush();
+    page = p;
+    by += v;
+  }
+};
+constexpr int kColumns = 128, kRowsAtOnce = 16;  // of a table: a CTA's part where rows share pages
 
 // Exclusive prefix sum over the block, and the total.
 __device__ __forceinline__ int block_scan(int v, int* red, int& total) {
@@ -83,6 +126,7 @@ struct ForkArgs {
 
 __global__ void __launch_bounds__(kPlanThreads) fork_plan(ForkArgs a) {
   __shared__ int red[32];
+  allow_next();
   for (int i = threadIdx.x; i < a.slots; i += kPlanThreads) a.owner[i] = a.n;
   __syncthreads();
   for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
@@ -120,55 +164,92 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan(ForkArgs a) {
 }
 
 // The children's new rows, from the parents' before any of them is replaced.
-__global__ void fork_rows(ForkArgs a) {
-  const int i = blockIdx.x, len = a.len[i];
+__device__ void fork_row(const ForkArgs& a, int i) {
+  const int len = a.len[i];
   if (len < 0) return;
-  const int held = (len + a.page_size - 1) / a.page_size;
+  const int held = (len + a.page_size - 1) / a.page_size, dst = a.dst[i];
   const int* from = a.table + (int64_t)a.parents[i] * a.width;
   int* to = a.rows + (int64_t)i * a.width;
   for (int j = threadIdx.x; j < a.width; j += blockDim.x)
-    to[j] = j >= held ? -1 : (a.dst[i] >= 0 && j == held - 1) ? a.dst[i] : from[j];
+    to[j] = j >= held ? -1 : (dst >= 0 && j == held - 1) ? dst : from[j];
 }
 
-__global__ void fork_commit(ForkArgs a) {
-  const int i = blockIdx.x, len = a.len[i];
-  if (len < 0) return;
-  const int c = a.children[i];
-  int* row = a.table + (int64_t)c * a.width;
-  const int* to = a.rows + (int64_t)i * a.width;
-  for (int j = threadIdx.x; j < a.width; j += blockDim.x) {
-    const int before = row[j], after = to[j];
-    if (before >= 0 && before < a.pages) atomicSub(&a.refs[before], 1);
-    if (after >= 0 && after < a.pages) atomicAdd(&a.refs[after], 1);
-    row[j] = after;
+__global__ void __launch_bounds__(kColumns) fork_commit(ForkArgs a) {
+  wait_for_previous();
+  const int j = blockIdx.x * kColumns + threadIdx.x, first = blockIdx.y * kRowsAtOnce;
+  __shared__ int child[kRowsAtOnce];  // or -1 where nothing changes
+  if (threadIdx.x < kRowsAtOnce) {
+    const int i = first + threadIdx.x, len = i < a.n ? a.len[i] : -1;
+    child[threadIdx.x] = len >= 0 ? a.children[i] : -1;
+    if (len >= 0 && blockIdx.x == 0) a.lens[a.children[i]] = len;
   }
-  if (threadIdx.x == 0) a.lens[c] = len;
+  __syncthreads();
+  if (j >= a.width) return;
+  int before[kRowsAtOnce], after[kRowsAtOnce];  // all in flight at once
+#pragma unroll
+  for (int k = 0; k < kRowsAtOnce; ++k) {
+    before[k] = child[k] >= 0 ? a.table[(int64_t)child[k] * a.width + j] : -1;
+    after[k] = child[k] >= 0 ? a.rows[(int64_t)(first + k) * a.width + j] : -1;
+  }
+  Run gone(a.refs, a.pages), come(a.refs, a.pages);
+#pragma unroll
+  for (int k = 0; k < kRowsAtOnce; ++k) {
+    gone.add(before[k], -1);
+    come.add(after[k], 1);
+    if (child[k] >= 0) a.table[(int64_t)child[k] * a.width + j] = after[k];
+  }
+  gone.flush();
+  come.flush();
 }
 
 // ------------------------------------------------------------------ copy
-// plane-wise copies of pages src[i] -> dst[i]; `count` (device) where it is
-// not null, else n, pairs.  Pairs with an id out of range are passed over.
-__global__ void __launch_bounds__(256) copy_pages(const char* __restrict__ from, char* __restrict__ to,
-                                                  const int* __restrict__ src, const int* __restrict__ dst,
-                                                  const int* __restrict__ count, int n, int64_t planes,
-                                                  int64_t page_bytes, int64_t from_pages, int64_t to_pages) {
-  const int64_t pairs = count ? min(*count, n) : n;
-  const bool wide = page_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(from) & 15) == 0 &&
-                    (reinterpret_cast<uintptr_t>(to) & 15) == 0;
-  for (int64_t it = blockIdx.x; it < pairs * planes; it += gridDim.x) {
-    const int64_t i = it / planes, plane = it - i * planes;
-    const int s = src[i], d = dst[i];
-    if (s < 0 || s >= from_pages || d < 0 || d >= to_pages) continue;
-    const char* x = from + (plane * from_pages + s) * page_bytes;
-    char* y = to + (plane * to_pages + d) * page_bytes;
+struct CopyArgs {
+  const char* from;
+  char* to;
+  const int *src, *dst;
+  const int* count;  // device, or null: n pairs
+  int n;
+  int64_t planes, page_bytes, from_pages, to_pages;
+};
+// Copies pages src[i] -> dst[i] of every plane, shared out over `blocks` CTAs.
+// Pairs with an id out of range are passed over.
+__device__ void copy_pages(const CopyArgs& a, int64_t block, int64_t blocks) {
+  const int64_t pairs = a.count ? min(*a.count, a.n) : a.n;
+  const bool wide = a.page_bytes % 16 == 0 && (reinterpret_cast<uintptr_t>(a.from) & 15) == 0 &&
+                    (reinterpret_cast<uintptr_t>(a.to) & 15) == 0;
+  for (int64_t it = block; it < pairs * a.planes; it += blocks) {
+    const int64_t i = it / a.planes, plane = it - i * a.planes;
+    const int s = a.src[i], d = a.dst[i];
+    if (s < 0 || s >= a.from_pages || d < 0 || d >= a.to_pages) continue;
+    const char* x = a.from + (plane * a.from_pages + s) * a.page_bytes;
+    char* y = a.to + (plane * a.to_pages + d) * a.page_bytes;
     if (wide) {
-      const int64_t vecs = page_bytes / 16;
-      for (int64_t j = threadIdx.x; j < vecs; j += blockDim.x)
-        reinterpret_cast<uint4*>(y)[j] = reinterpret_cast<const uint4*>(x)[j];
+      const int64_t vecs = a.page_bytes / 16;
+      const uint4* xv = reinterpret_cast<const uint4*>(x);
+      uint4* yv = reinterpret_cast<uint4*>(y);
+      int64_t j = threadIdx.x;
+      for (; j + 3 * blockDim.x < vecs; j += 4 * blockDim.x) {
+        uint4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = xv[j + k * blockDim.x];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) yv[j + k * blockDim.x] = v[k];
+      }
+      for (; j < vecs; j += blockDim.x) yv[j] = xv[j];
     } else {
-      for (int64_t j = threadIdx.x; j < page_bytes; j += blockDim.x) y[j] = x[j];
+      for (int64_t j = threadIdx.x; j < a.page_bytes; j += blockDim.x) y[j] = x[j];
     }
   }
+}
+__global__ void __launch_bounds__(256) copy_kernel(CopyArgs a) { copy_pages(a, blockIdx.x, gridDim.x); }
+// The first n CTAs write the children's new rows, the others copy the pages.
+__global__ void __launch_bounds__(256) fork_rows(ForkArgs a, CopyArgs copy) {
+  allow_next();
+  wait_for_previous();
+  if ((int)blockIdx.x < a.n)
+    fork_row(a, blockIdx.x);
+  else
+    copy_pages(copy, blockIdx.x - a.n, gridDim.x - a.n);
 }
 
 // ------------------------------------------------------------------ reserve
@@ -288,6 +369,7 @@ struct CompactArgs {
 
 __global__ void __launch_bounds__(kPlanThreads) compact_plan(CompactArgs a) {
   __shared__ int red[32];
+  allow_next();
   int mine = 0, live;
   for (int p = threadIdx.x; p < a.pages; p += kPlanThreads) mine += a.refs[p] > 0;
   block_scan(mine, red, live);
@@ -320,9 +402,15 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan(CompactArgs a) {
   }
 }
 
-__global__ void compact_table(CompactArgs a) {
+// The first `table_blocks` CTAs rewrite the table, the others move the pages.
+__global__ void __launch_bounds__(256) compact_moves(CompactArgs a, CopyArgs copy, int table_blocks) {
+  wait_for_previous();
+  if ((int)blockIdx.x >= table_blocks) {
+    copy_pages(copy, blockIdx.x - table_blocks, gridDim.x - table_blocks);
+    return;
+  }
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < a.entries;
-       i += (int64_t)gridDim.x * blockDim.x) {
+       i += (int64_t)table_blocks * blockDim.x) {
     const int p = a.table[i];
     if (p >= 0 && p < a.pages && a.map[p] >= 0) a.table[i] = a.map[p];
   }
@@ -379,16 +467,13 @@ int kb_cache_fork(void* pool, int32_t* table, int32_t* lens, int32_t* refs, cons
   a.owner = take(slots), a.list = take(n), a.src = take(n), a.dst = take(n), a.len = take(n), a.rows = take(n * width);
   fork_plan<<<1, kPlanThreads, 0, stream>>>(a);
   if (int st = kb::check_launch(name)) return st;
-  fork_rows<<<(unsigned)n, 256, 0, stream>>>(a);
-  if (int st = kb::check_launch(name)) return st;
-  if (planes && page_bytes && pages) {
-    copy_pages<<<copy_grid(n * planes), 256, 0, stream>>>(static_cast<const char*>(pool), static_cast<char*>(pool),
-                                                          a.src, a.dst, nullptr, (int)n, planes, page_bytes, pages,
-                                                          pages);
-    if (int st = kb::check_launch(name)) return st;
-  }
-  fork_commit<<<(unsigned)n, 256, 0, stream>>>(a);
-  return kb::check_launch(name);
+  CopyArgs copy{static_cast<const char*>(pool), static_cast<char*>(pool), a.src, a.dst, nullptr, (int)n, planes,
+                page_bytes, pages, pages};
+  const unsigned copies = planes && page_bytes && pages ? copy_grid(n * planes) : 0;
+  if (int st = launch_after(fork_rows, dim3((unsigned)n + copies), 256u, stream, a, copy)) return st;
+  return launch_after(fork_commit, dim3((unsigned)std::max<int64_t>(1, kb::ceil_div(width, kColumns)),
+                                        (unsigned)kb::ceil_div(n, kRowsAtOnce)),
+                      (unsigned)kColumns, stream, a);
 }
 
 size_t kb_cache_reserve_workspace_size(int64_t n, int64_t tokens, int64_t slots, int64_t width, int64_t pages,
@@ -471,17 +556,12 @@ int kb_cache_compact(void* pool, int32_t* table, int32_t* refs, int32_t* live, i
   compact_plan<<<1, kPlanThreads, 0, stream>>>(a);
   if (int st = kb::check_launch(name)) return st;
   if (pages == 0) return KB_OK;
-  if (a.entries) {
-    compact_table<<<copy_grid(kb::ceil_div(a.entries, 256)), 256, 0, stream>>>(a);
-    if (int st = kb::check_launch(name)) return st;
-  }
-  if (planes && page_bytes) {
-    copy_pages<<<copy_grid(pages * planes), 256, 0, stream>>>(static_cast<const char*>(pool), static_cast<char*>(pool),
-                                                              a.src, a.dst, a.count, (int)pages, planes, page_bytes,
-                                                              pages, pages);
-    return kb::check_launch(name);
-  }
-  return KB_OK;
+  CopyArgs copy{static_cast<const char*>(pool), static_cast<char*>(pool), a.src, a.dst, a.count, (int)pages, planes,
+                page_bytes, pages, pages};
+  const unsigned copies = planes && page_bytes ? copy_grid(pages * planes) : 0;
+  const unsigned rows = a.entries ? copy_grid(kb::ceil_div(a.entries, 1024)) : 0;
+  if (copies + rows == 0) return KB_OK;
+  return launch_after(compact_moves, dim3(rows + copies), 256u, stream, a, copy, (int)rows);
 }
 
 int kb_cache_copy(const void* src_pool, const int32_t* src, void* dst_pool, const int32_t* dst, int64_t n,
@@ -493,9 +573,9 @@ int kb_cache_copy(const void* src_pool, const int32_t* src, void* dst_pool, cons
   KB_REQUIRE(n <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many pages", name);
   if (n == 0 || planes == 0 || page_bytes == 0 || src_pages == 0 || dst_pages == 0) return KB_OK;
   KB_REQUIRE(src_pool && dst_pool && src && dst, KB_ERR_INVALID_ARG, "%s: null pointer", name);
-  copy_pages<<<copy_grid(n * planes), 256, 0, stream>>>(static_cast<const char*>(src_pool),
-                                                        static_cast<char*>(dst_pool), src, dst, nullptr, (int)n,
-                                                        planes, page_bytes, src_pages, dst_pages);
+  const CopyArgs copy{static_cast<const char*>(src_pool), static_cast<char*>(dst_pool), src, dst, nullptr, (int)n,
+                      planes, page_bytes, src_pages, dst_pages};
+  copy_kernel<<<copy_grid(n * planes), 256, 0, stream>>>(copy);
   return kb::check_launch(name);
 }
 
