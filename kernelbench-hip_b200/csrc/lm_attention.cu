@@ -758,7 +758,9 @@ size_t kb_shared_prefix_attention_workspace_size(int64_t batch, int64_t queries,
                                                  int64_t dim, int64_t prefix_pages, int64_t width,
                                                  int64_t page_size, int dtype) {
   using namespace kb::lm::attn;
-  if (heads_q % heads_kv) return 0;
+  if (batch <= 0 || queries <= 0 || heads_q <= 0 || heads_kv <= 0 || dim <= 0 || page_size <= 0 || prefix_pages < 0 ||
+      heads_q % heads_kv)
+    return 0;
   auto bytes = [&](bool tensor) {
     return plan_bytes(plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size,
                            std::max<int64_t>(0, width - prefix_pages) * page_size, dtype, tensor),

@@ -22,7 +22,7 @@ from functools import lru_cache
 import torch
 
 from ._lib import LIB, KbError
-from .ops import _get_raw_stream, _ptr, _workspace
+from .ops import _get_raw_stream, _ptr
 from .ops import _stream as _stream_of
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_backward", "rope_tables", "shared_prefix_attention", "cache_reserve",
@@ -36,12 +36,24 @@ _POOLS = (torch.float32, torch.float16, torch.bfloat16, torch.uint8, torch.int8)
 # host counts: each function first asks one compact question that all right
 # arguments answer with yes, and only on a no goes through the checks one by
 # one, to say what is wrong.
-_empty = torch.empty
+_empty, _empty_like = torch.empty, torch.empty_like
 _F32, _I32 = torch.float32, torch.int32
 
 
 def _stream(dev: int, t: torch.Tensor) -> int:
     return _get_raw_stream(dev) if _get_raw_stream is not None else _stream_of(t)
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A new contiguous tensor of x's shape and type (empty_like costs half of empty; it keeps another order of
+    memory than the contiguous one where x has one)."""
+    y = _empty_like(x)
+    return y if y.is_contiguous() else _empty(x.shape, device=x.device, dtype=x.dtype)
+
+
+def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
+    """Workspace of nbytes, made of `like`'s 32-bit elements."""
+    return like.new_empty((nbytes + 3) // 4 if nbytes > 16 else 4)
 
 
 def check(fn: str, status: int) -> None:
@@ -181,7 +193,8 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps: float = 1e-
     and k."""
     fn = "kb_qk_norm_rope"
     shape, kinds, dev = _rope_args(fn, q, k, q_weight, k_weight, cos, sin, positions)
-    qo, ko = _out(fn, q_out, q, shape[0:2] + shape[3:4]), _out(fn, k_out, k, (shape[0], shape[2], shape[3]))
+    qo = _like(q) if q_out is None else _out(fn, q_out, q, q.shape)
+    ko = _like(k) if k_out is None else _out(fn, k_out, k, k.shape)
     check(fn, LIB.kb_qk_norm_rope(q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight), cos.data_ptr(),
                                   sin.data_ptr(), positions.data_ptr(), qo.data_ptr(), ko.data_ptr(), *shape,
                                   *kinds, 1 if interleaved else 0, eps, _stream(dev, q)))
@@ -203,12 +216,13 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, po
     dq, dk = torch.empty_like(dq_out), torch.empty_like(dk_out)
     dqw = None if q_weight is None else torch.empty_like(q_weight)
     dkw = None if k_weight is None else torch.empty_like(k_weight)
-    ws = _workspace(q, _rope_backward_bytes(*shape[:4]))
+    need = _rope_backward_bytes(shape[0], shape[1], shape[2], shape[3])
+    ws = _scratch(need, cos)
     check(fn, LIB.kb_qk_norm_rope_backward(dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(),
                                            _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
                                            positions.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(dqw), _ptr(dkw),
                                            *shape, *kinds, 1 if interleaved else 0, eps, ws.data_ptr(),
-                                           ws.shape[0], _stream(dev, q)))
+                                           need, _stream(dev, q)))
     return dq, dk, dqw, dkw
 
 
@@ -229,11 +243,11 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix, table, lens, scale: flo
     if sizes is None:
         sizes = _attention_checks(fn, q, k_pages, v_pages, prefix, table, lens)
     B, Q, hq, hkv, d, n_pre, width, pages, page_size, qs, ks, vs = sizes
-    dev, code = q.device, _DTYPES[q.dtype]
-    o = _empty((B, Q, hq, d), device=dev, dtype=q.dtype) if out is None else _out(fn, out, q, q.shape)
-    lse = _empty((B, Q, hq), device=dev, dtype=_F32)
+    code = _DTYPES[q.dtype]
+    o = _like(q) if out is None else _out(fn, out, q, q.shape)
+    lse = q.new_empty((B, Q, hq), dtype=_F32)
     need = _attention_bytes(B, Q, hq, hkv, d, n_pre, width, page_size, code)
-    ws = _empty(need, device=dev, dtype=torch.uint8) if need else None
+    ws = _scratch(need, lens) if need else None
     check(fn, LIB.kb_shared_prefix_attention(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), prefix.data_ptr(), table.data_ptr(), lens.data_ptr(),
         o.data_ptr(), lse.data_ptr(), B, Q, hq, hkv, d, n_pre, width, pages, page_size, qs[0], qs[1], qs[2],
@@ -331,11 +345,12 @@ def cache_reserve(table, lens, refs, seqs, tokens: int, page_size: int):
     fn = "kb_cache_reserve"
     dev = _state(fn, table, lens, refs)
     n = _slots(fn, "seqs", seqs, dev).shape[0]
-    granted = torch.empty(n, device=dev, dtype=torch.int32)
+    granted = _empty_like(seqs)
     sizes = (table.shape[0], table.shape[1], refs.shape[0], int(page_size))
-    ws = _workspace(table, _reserve_bytes(n, int(tokens), *sizes))
+    need = _reserve_bytes(n, int(tokens), *sizes)
+    ws = _scratch(need, refs)
     check(fn, LIB.kb_cache_reserve(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(),
-                                   granted.data_ptr(), n, int(tokens), *sizes, ws.data_ptr(), ws.numel(),
+                                   granted.data_ptr(), n, int(tokens), *sizes, ws.data_ptr(), need,
                                    _stream(table.get_device(), table)))
     return granted
 
@@ -402,12 +417,13 @@ def cache_fork(pool, table, lens, refs, parents, children):
     page_bytes = _pool(fn, "pool", pool, dev, refs.shape[0])
     n = _slots(fn, "parents", parents, dev).shape[0]
     _slots(fn, "children", children, dev, n)
-    granted = torch.empty(n, device=dev, dtype=torch.int32)
+    granted = _empty_like(parents)
     slots, width = table.shape
-    ws = _workspace(table, _fork_bytes(n, slots, width))
+    need = _fork_bytes(n, slots, width)
+    ws = _scratch(need, refs)
     check(fn, LIB.kb_cache_fork(pool.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
                                 parents.data_ptr(), children.data_ptr(), granted.data_ptr(), n, slots, width,
-                                pool.shape[0], pool.shape[1], pool.shape[2], page_bytes, ws.data_ptr(), ws.numel(),
+                                *pool.shape[:3], page_bytes, ws.data_ptr(), need,
                                 _stream(table.get_device(), table)))
     return granted
 
@@ -427,11 +443,12 @@ def cache_compact(pool, table, refs):
     fn = "kb_cache_compact"
     dev = _state(fn, table, None, refs)
     page_bytes = _pool(fn, "pool", pool, dev, refs.shape[0])
-    live = torch.empty(1, device=dev, dtype=torch.int32)
-    ws = _workspace(table, LIB.kb_cache_compact_workspace_size(refs.shape[0]))
+    live = refs.new_empty(1)
+    need = LIB.kb_cache_compact_workspace_size(refs.shape[0])
+    ws = _scratch(need, refs)
     check(fn, LIB.kb_cache_compact(pool.data_ptr(), table.data_ptr(), refs.data_ptr(), live.data_ptr(),
                                    table.shape[0], table.shape[1], pool.shape[0], pool.shape[1], page_bytes,
-                                   ws.data_ptr(), ws.numel(), _stream(table.get_device(), table)))
+                                   ws.data_ptr(), need, _stream(table.get_device(), table)))
     return live
 
 
@@ -502,7 +519,7 @@ def penalize_logits(logits, prompt=None, output=None, repetition=None, presence=
             raise RuntimeError(f"{fn}: mask has shape {tuple(mask.shape)}, expected ({B} or 1, {words})")
         _contiguous(fn, "mask", mask)
         mask_stride = words if mask.shape[0] == B else 0
-    y = _out(fn, out, logits, logits.shape)
+    y = _like(logits) if out is None else _out(fn, out, logits, logits.shape)
     check(fn, LIB.kb_penalize_logits(logits.data_ptr(), y.data_ptr(), _ptr(prompt), _ptr(output), _ptr(repetition),
                                      _ptr(presence), _ptr(frequency), _ptr(bias_ids), _ptr(bias_values), _ptr(mask),
                                      B, V, logits.stride(0), *lengths, mask_stride, _DTYPES[logits.dtype],
