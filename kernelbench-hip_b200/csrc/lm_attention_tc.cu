@@ -398,19 +398,28 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const uint32_t s_addr = tmem + lanes + t * kTile, o_addr = tmem + lanes + o_col + t * kTile;
     const float c = fabsf(a.scale_log2);
     if (n > 0) {
-      // the row of Q into the swizzled tile, its sign turned where the scale is negative
-      const uint4* src = static_cast<const uint4*>(query_of(a, w, r < w.rows ? r : 0, 2));
-      const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-      uint8_t* dst = s_q + t * kTileBytes + row * 128;
+      // the row of Q into the swizzled tile, all copies in flight at once
+      const char* src = static_cast<const char*>(query_of(a, w, r < w.rows ? r : 0, 2));
+      const uint32_t dst = smem_u32(s_q + t * kTileBytes + row * 128);
+      auto at = [&](int i) { return dst + (i >> 3) * kHalfBytes + (((i & 7) ^ (row & 7)) << 4); };
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (i >= halves * 8) break;
-        if (r < w.rows && i * 8 < a.dim) {
-          x = src[i];
-          x.x ^= flip, x.y ^= flip, x.z ^= flip, x.w ^= flip;
+      for (int i = 0; i < halves * 8; ++i) {
+        const bool in = r < w.rows && i * 8 < a.dim;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at(i)), "l"(src + (in ? i * 16 : 0)),
+                     "r"(in ? 16 : 0)
+                     : "memory");
+      }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      if (a.scale_log2 < 0.0f) {  // scores are multiplied by |c|
+        for (int i = 0; i < halves * 8; ++i) {
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                       : "r"(at(i)));
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at(i)), "r"(x[0] ^ 0x80008000u),
+                       "r"(x[1] ^ 0x80008000u), "r"(x[2] ^ 0x80008000u), "r"(x[3] ^ 0x80008000u)
+                       : "memory");
         }
-        *reinterpret_cast<uint4*>(dst + (i >> 3) * kHalfBytes + (((i & 7) ^ (row & 7)) << 4)) = x;
       }
       fence_proxy_async();
       mbar_arrive(q_full + 8 * t);
@@ -506,7 +515,13 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     const float lse = none ? -INFINITY : (m == -INFINITY ? 0.0f : base) * kLn2 + logf(l);
     if (r < w.rows) (a.part_o ? a.part_lse[at * a.splits + w.split] : a.lse[at]) = lse;
     if (ok) {
+      // Out through shared memory, 32 columns at a time, so that a warp writes
+      // whole 128-byte pieces of rows (a thread's own row straight from its
+      // registers took 5 us per CTA).  The row tile's Q, whose last product is
+      // done, makes room: one buffer per warp, rows 144 bytes apart.
       const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
+      float* buf = reinterpret_cast<float*>(s_q + t * kTileBytes) + (warp & 3) * 32 * 36;
+      const int row0 = t * kTile + (warp & 3) * 32;  // the warp's rows
 #pragma unroll 1
       for (int i = 0; i < a.dim; i += 32) {
         uint32_t y[32];
@@ -514,21 +529,28 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           tmem_ld(o_addr + i, y);
           tmem_ld_wait(y);
         }
-        if (r >= w.rows || (none && a.part_o)) continue;  // a part without keys is not read
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
-          if (i + k >= a.dim) break;
           float z[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) z[e] = none ? 0.0f : __uint_as_float(y[k + e]) * inv;
-          if (a.part_o) {
-            *reinterpret_cast<float4*>(a.part_o + ((int64_t)w.split * n_rows + at) * a.dim + i + k) =
-                make_float4(z[0], z[1], z[2], z[3]);
+          *reinterpret_cast<float4*>(buf + lane * 36 + k) = make_float4(z[0], z[1], z[2], z[3]);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int p = 0; p < 8; ++p) {
+          const int q = p * 4 + (lane >> 3), col = i + (lane & 7) * 4;
+          const float4 z = *reinterpret_cast<const float4*>(buf + q * 36 + (lane & 7) * 4);
+          const int64_t at_row = __shfl_sync(0xffffffffu, at, q);
+          if (row0 + q >= w.rows || col >= a.dim) continue;
+          if (a.part_o) {  // a part without keys is not read: its zeros do no harm
+            *reinterpret_cast<float4*>(a.part_o + ((int64_t)w.split * n_rows + at_row) * a.dim + col) = z;
           } else {
-            T* out = static_cast<T*>(a.out) + at * a.dim + i + k;
-            *reinterpret_cast<uint2*>(out) = make_uint2(pack(z[0], z[1], (T*)nullptr), pack(z[2], z[3], (T*)nullptr));
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at_row * a.dim + col) =
+                make_uint2(pack(z.x, z.y, (T*)nullptr), pack(z.z, z.w, (T*)nullptr));
           }
         }
+        __syncwarp();
       }
     }
   }
