@@ -424,6 +424,40 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Item w = item_at(a, a.first_item + blockIdx.x, C::kRows);
   const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
+  const T* kp = static_cast<const T*>(a.k) + w.h * a.k_h;
+  const T* vp = static_cast<const T*>(a.v) + w.h * a.v_h;
+  T* mine = ring + warp * STAGES * C::kStage;
+  // A CTA lives for a few blocks, so its start counts: the queries, the pages
+  // and the lengths are read at once, and the keys as soon as those are there
+  // (one after the other they took 5 us until the first keys).
+  for (int i = tid; i < C::kRows * kPerRow; i += C::kThreads) {
+    const int r = i / kPerRow, c = (i - r * kPerRow) * kVec;
+    const bool in = r < w.rows && c < a.dim;
+    cp_async16(sq + r * LD + c, static_cast<const T*>(query_of(a, w, in ? r : 0, sizeof(T))) + (in ? c : 0), in);
+  }
+  // Where this lane's key of the block at key0 lies (lanes past NK repeat):
+  // looked up once per key, before it is known whether any row sees it.
+  const bool alike = a.k_p == a.v_p && a.k_s == a.v_s;
+  struct Place {
+    int64_t k, v;
+  };
+  auto place = [&](int key0) {
+    const int j = key0 + lane % NK;
+    Place p{0, 0};
+    if (j < w.k1) {
+      const int pj = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
+      const int slot = j - pj * a.page_size;
+      const int64_t page = min(max(w.pages[pj], 0), a.pages - 1);
+      p.k = page * a.k_p + slot * a.k_s;
+      p.v = alike ? p.k : page * a.v_p + slot * a.v_s;
+    }
+    return p;
+  };
+  constexpr int kStep = C::kWarps * NK;
+  const int begin = w.k0 + warp * NK;
+  Place first[STAGES];
+#pragma unroll
+  for (int i = 0; i < STAGES; ++i) first[i] = place(begin + i * kStep);
   const int row[2] = {lane >> 2, (lane >> 2) + 8};
   int vis[2], top = 0, low = 0x7fffffff;
 #pragma unroll
@@ -435,27 +469,6 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
   const int end = min(w.k1, __reduce_max_sync(0xffffffffu, top));
   low = __reduce_min_sync(0xffffffffu, low);
 
-  const T* kp = static_cast<const T*>(a.k) + w.h * a.k_h;
-  const T* vp = static_cast<const T*>(a.v) + w.h * a.v_h;
-  T* mine = ring + warp * STAGES * C::kStage;
-  // Where this lane's key of the block at key0 lies (lanes past NK repeat):
-  // looked up once per key, a block before its copies are issued.
-  const bool alike = a.k_p == a.v_p && a.k_s == a.v_s;
-  struct Place {
-    int64_t k, v;
-  };
-  auto place = [&](int key0) {
-    const int j = key0 + lane % NK;
-    Place p{0, 0};
-    if (j < end) {
-      const int pj = a.page_shift >= 0 ? j >> a.page_shift : j / a.page_size;
-      const int slot = j - pj * a.page_size;
-      const int64_t page = min(max(w.pages[pj], 0), a.pages - 1);
-      p.k = page * a.k_p + slot * a.k_s;
-      p.v = alike ? p.k : page * a.v_p + slot * a.v_s;
-    }
-    return p;
-  };
   auto load = [&](int key0, const Place& p, int stage) {
     T* sk = mine + stage * C::kStage;
     T* sv = sk + NK * LD;
@@ -483,24 +496,12 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
       cp_async16(sv + n * LD + c, vp + v + cc, in);
     }
   };
-  constexpr int kStep = C::kWarps * NK;
-  const int begin = w.k0 + warp * NK;
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) {
-    if (begin + i * kStep < end) load(begin + i * kStep, place(begin + i * kStep), i);
+    if (begin + i * kStep < end) load(begin + i * kStep, first[i], i);
     cp_async_commit();
   }
-  Place next = place(begin + (STAGES - 1) * kStep);
-  // the queries, while the first keys are on their way
-  for (int i = tid; i < C::kRows * kPerRow; i += C::kThreads) {
-    const int r = i / kPerRow, c = (i - r * kPerRow) * kVec;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (r < w.rows && c < a.dim) {
-      x = *reinterpret_cast<const uint4*>(static_cast<const T*>(query_of(a, w, r, sizeof(T))) + c);
-    }
-    *reinterpret_cast<uint4*>(sq + r * LD + c) = x;
-  }
-  __syncthreads();
+  Place next = first[STAGES - 1];
 
   float o[DP / 8][4];
 #pragma unroll
@@ -509,6 +510,12 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
     for (int i = 0; i < 4; ++i) o[d][i] = 0.0f;
   Running st{{-INFINITY, -INFINITY}, {0.0f, 0.0f}};
   const int seen[2] = {min(vis[0], end), min(vis[1], end)};
+  // The queries came with each warp's first copies; a warp without a block meets the others here, too.
+  auto queries_there = [&] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+  if (begin >= end) {
+    cp_async_wait<0>();
+    queries_there();
+  }
   int stage = 0;
   for (int key0 = begin; key0 < end; key0 += kStep) {
     const int ahead = key0 + (STAGES - 1) * kStep;
@@ -516,6 +523,7 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
     cp_async_commit();
     next = place(ahead + kStep);
     cp_async_wait<STAGES - 1>();
+    if (key0 == begin) queries_there();
     __syncwarp();
     const T* sk = mine + stage * C::kStage;
     float s[NK / 8][4];
