@@ -76,7 +76,8 @@ namespace kb {
 
 namespace lm {
 namespace attn {
-int tc_read_fault(bool clear, int* value);  // the attention kernel's fault word
+int tc_read_fault(bool clear, int* value);  // the attention kernels' fault words
+int tc32_read_fault(bool clear, int* value);
 }
 }  // namespace lm
 
@@ -1068,6 +1069,8 @@ int kb_read_fault(int clear, int* value) {
   }
   int attention = 0;
   if (int st = kb::lm::attn::tc_read_fault(clear != 0, &attention)) return st;
+  *value |= attention;
+  if (int st = kb::lm::attn::tc32_read_fault(clear != 0, &attention)) return st;
   *value |= attention;
   return KB_OK;
 }

@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(RowsCfg<T, DP, NK>::kThreads) attn_rows_kernel
 }
 
 // ------------------------------------------------------------------ keys kernel
-// Up to 16 rows: each of four warps takes every fourth block of NK keys, with
+// Tiles of 16 rows: each of four warps takes every fourth block of NK keys, with
 // a ring of its own filled by cp.async (no barrier until the end), and its own
 // running softmax; the four are joined in shared memory.  This is the shape of
 // decoding: a few query heads per key head against a sequence's own keys,
@@ -666,13 +666,17 @@ struct Plan {
 Part plan_part(int64_t sets, int64_t rows, int64_t keys, int dtype, bool tensor) {
   Part p;
   if (keys <= 0) return p;
-  p.kind = rows <= 16 ? kKeys : tensor ? kTensor : kRows;
+  // Up to a few row tiles the keys kernel reads the keys again for each (from
+  // L2) and is still faster than a wider tile that stays half empty: fp32, 24
+  // rows over 32000 keys 188 against 300 us, 64 rows 111 against 119; 16-bit, 32
+  // rows 44 against 76, 64 rows 38 against 34.
+  p.kind = rows <= (dtype == KB_F32 ? 64 : tensor ? 16 : 48) ? kKeys : tensor ? kTensor : kRows;
   if (p.kind == kTensor) {
     // One CTA per SM, equal ranges of whole 128-key tiles: the number of
     // ranges that makes the last wave end first, a range's fixed cost (the
     // queries, the first scores, the way out) counted as kFixed tiles.
     constexpr int64_t kFixed = 3;
-    p.tiles = (int)ceil_div(rows, (int64_t)tc_tile_rows(rows));
+    p.tiles = (int)ceil_div(rows, (int64_t)(dtype == KB_F32 ? kTc32Rows : tc_tile_rows(rows)));
     const int64_t items = p.tiles * sets, tiles = ceil_div(keys, 128), most = std::min<int64_t>(tiles, 64);
     int64_t best = 0;
     for (int64_t s = 1; s <= most; ++s) {
@@ -697,8 +701,9 @@ Plan plan(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv, int
   return {plan_part(heads_kv, batch * rows, prefix_keys, dtype, tensor),
           plan_part(heads_kv * batch, rows, own_keys, dtype, false)};
 }
-size_t plan_bytes(const Plan& p, int64_t rows, int64_t dim) {
-  return p.splits() <= 1 ? 0 : (size_t)p.splits() * rows * (dim + 1) * sizeof(float);
+// Parts, then (fp32 on the tensor cores) the prefix in halves.
+size_t part_bytes(const Plan& p, int64_t rows, int64_t dim) {
+  return p.splits() <= 1 ? 0 : (size_t)ceil_div(p.splits() * rows * (dim + 1), 4) * 16;
 }
 
 // The launch may begin once every CTA of the one before it has begun; the
@@ -769,13 +774,18 @@ size_t kb_shared_prefix_attention_workspace_size(int64_t batch, int64_t queries,
   if (batch <= 0 || queries <= 0 || heads_q <= 0 || heads_kv <= 0 || dim <= 0 || page_size <= 0 || prefix_pages < 0 ||
       heads_q % heads_kv)
     return 0;
+  const int64_t keys = prefix_pages * page_size;
   auto bytes = [&](bool tensor) {
-    return plan_bytes(plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size,
+    return part_bytes(plan(batch, queries, heads_q, heads_kv, keys,
                            std::max<int64_t>(0, width - prefix_pages) * page_size, dtype, tensor),
                       batch * queries * heads_q, dim);
   };
+  if (dtype == KB_F32) {
+    const bool tensor = tc32_pays(batch * queries * (heads_q / heads_kv), heads_kv, dim, keys);
+    return bytes(tensor) + (tensor ? tc32_bytes(heads_kv, dim, keys) : 0);
+  }
   // strides decide whether the tensor-core kernel can take the prefix
-  return dtype == KB_F32 ? bytes(false) : std::max(bytes(false), bytes(true));
+  return std::max(bytes(false), bytes(true));
 }
 
 int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v_pages, const int32_t* prefix,
@@ -827,21 +837,27 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
   a.k_p = k_stride_page, a.k_s = k_stride_slot, a.k_h = k_stride_head;
   a.v_p = v_stride_page, a.v_s = v_stride_slot, a.v_h = v_stride_head;
   a.scale_log2 = scale * kLog2e;
-  const Plan p = plan(batch, queries, heads_q, heads_kv, prefix_pages * page_size, own_pages * page_size, dtype,
-                      tc_fits(a, dtype));
+  const int64_t keys = prefix_pages * page_size;
+  const bool tensor = dtype == KB_F32 ? tc32_pays(batch * queries * a.group, heads_kv, dim, keys) : tc_fits(a, dtype);
+  const Plan p = plan(batch, queries, heads_q, heads_kv, keys, own_pages * page_size, dtype, tensor);
   a.splits = p.splits();
   a.prefix_tiles = p.prefix.tiles, a.prefix_splits = p.prefix.splits, a.prefix_chunk = p.prefix.chunk;
   a.own_tiles = p.own.tiles, a.own_splits = p.own.splits, a.own_chunk = p.own.chunk;
   a.prefix_items = (int64_t)p.prefix.tiles * p.prefix.splits * heads_kv;
   const int64_t items = a.prefix_items + (int64_t)p.own.tiles * p.own.splits * heads_kv * batch;
   KB_REQUIRE(items <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many work items", name);
-  if (p.splits() > 1) {
-    const size_t need = plan_bytes(p, rows, dim);
+  const bool halves = dtype == KB_F32 && p.prefix.kind == kTensor;
+  void* scratch = nullptr;
+  if (p.splits() > 1 || halves) {
+    const size_t parts = part_bytes(p, rows, dim), need = parts + (halves ? tc32_bytes(heads_kv, dim, keys) : 0);
     KB_REQUIRE(workspace && workspace_bytes >= need, KB_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", name, need, workspace_bytes);
     KB_REQUIRE(kb::aligned16(workspace), KB_ERR_INVALID_ARG, "%s: workspace must be 16-byte aligned", name);
-    a.part_o = static_cast<float*>(workspace);
-    a.part_lse = a.part_o + (int64_t)p.splits() * rows * dim;
+    if (p.splits() > 1) {
+      a.part_o = static_cast<float*>(workspace);
+      a.part_lse = a.part_o + (int64_t)p.splits() * rows * dim;
+    }
+    scratch = static_cast<char*>(workspace) + parts;
   }
   return with_dtype(dtype, [&](auto* x) {
     using T = std::remove_pointer_t<decltype(x)>;
@@ -849,8 +865,9 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
       if (p.prefix.kind == p.own.kind) {
         if (int st = launch_kind<T>(p.own.kind, a, 0, items, stream)) return st;
       } else {
-        if (int st = p.prefix.kind == kTensor ? tc_launch(a, dtype, stream)
-                                              : launch_kind<T>(p.prefix.kind, a, 0, a.prefix_items, stream))
+        if (int st = halves                      ? tc32_launch(a, scratch, stream)
+                     : p.prefix.kind == kTensor ? tc_launch(a, dtype, stream)
+                                                : launch_kind<T>(p.prefix.kind, a, 0, a.prefix_items, stream))
           return st;
         if (int st = launch_kind<T>(p.own.kind, a, a.prefix_items, items - a.prefix_items, stream)) return st;
       }

@@ -105,6 +105,13 @@ int tc_launch(const AttnArgs& a, int dtype, cudaStream_t stream);
 // The device's fault word: nonzero after a wait ran out.
 int tc_read_fault(bool clear, int* value);
 
+// ------------------------------------------------------------------ fp32 prefix in halves (lm_attention_tc32.cu)
+constexpr int kTc32Rows = 128;  // rows of a row tile
+bool tc32_pays(int64_t rows, int64_t heads_kv, int64_t dim, int64_t keys);
+size_t tc32_bytes(int64_t heads_kv, int64_t dim, int64_t keys);  // scratch, 16-byte aligned
+int tc32_launch(const AttnArgs& a, void* scratch, cudaStream_t stream);
+int tc32_read_fault(bool clear, int* value);
+
 }  // namespace attn
 }  // namespace lm
 }  // namespace kb

@@ -205,6 +205,39 @@ def test_shared_prefix_attention(shape, dt, cuda_device):
     check_attention(attention_inputs(cuda_device, dt, *shape, seed=sum(shape)), dt)
 
 
+LARGE = [  # past 1.2e9 operations over the prefix: fp32 in halves on the tensor cores
+    (40, 1, 16, 4, 64, 16, 460, 30), (33, 2, 8, 2, 80, 24, 300, 50), (18, 1, 32, 4, 128, 32, 140, 0),
+]
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", LARGE)
+def test_attention_long_prefix(shape, dt, cuda_device):
+    check_attention(attention_inputs(cuda_device, dt, *shape, seed=sum(shape)), dt)
+
+
+def test_attention_long_prefix_in_fp32_of_uneven_magnitudes(cuda_device):
+    """Keys and values over six orders of magnitude, short and ended sequences, NaN where nobody looks, a negative
+    scale."""
+    shape = (40, 1, 16, 4, 64, 16, 460, 30)
+    q, k, v, prefix, table, lens = attention_inputs(cuda_device, torch.float32, *shape, seed=3)
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    q, k, v = (x * 10 ** (3 * torch.rand(x.shape[:-1] + (1,), device=cuda_device, generator=g) - 2.5) for x in (q, k, v * 1e5))
+    lens = 7000 + torch.arange(40, device=cuda_device, dtype=torch.int32)
+    lens[5], lens[6], lens[7] = 0, 1, 130
+    args = (q, k, v, prefix, table, lens)
+    out, lse = check_attention(args, torch.float32)
+    assert (out[5] == 0).all()
+    check_attention(args, torch.float32, scale=-0.05)
+    last = prefix[7039 // 16:].long()
+    for t in (k, v):
+        t[last[1:]] = float("nan")
+        t[last[0], 7039 % 16:] = float("inf")
+    from kbb200 import lm
+    again = lm.shared_prefix_attention(*args)
+    assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
 @pytest.mark.parametrize("dt", TYPES)
 def test_attention_empty_and_short_rows(dt, cuda_device):
     """Ended slots, sequences with fewer keys than queries, and shorter than the prefix."""
