@@ -2,8 +2,10 @@
 
 Each csrc/*.cu is compiled by nvcc into _build/*.o in parallel, then linked
 into kbb200/libkbb200.so with the CUDA runtime linked statically, so the
-library needs only the driver at run time.  Rebuilds only what changed
-(object older than its source or any header).
+library needs only the driver at run time.  csrc/lm_host.cpp, the host side
+of kbb200.lm's calls, becomes the Python module kbb200/_lm_host.so, against the
+installed torch.  Rebuilds only what changed (object older than its source or
+any header).
 
     python kernelbench-hip_b200/build.py [--clean] [-j N] [--verbose]
 """
@@ -23,6 +25,8 @@ BUILD = PKG_ROOT / "_build"
 REPO = PKG_ROOT.parent
 INCLUDE = REPO / "include"
 LIB = PKG_ROOT / "kbb200" / "libkbb200.so"
+HOST_SRC = CSRC / "lm_host.cpp"
+HOST_MODULE = PKG_ROOT / "kbb200" / "_lm_host.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -56,9 +60,31 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _build_host_module(verbose: bool) -> None:
+    import importlib.util
+    import sysconfig
+
+    torch = Path(importlib.util.find_spec("torch").origin).parent  # not imported: only its headers and libraries
+    newest = max(f.stat().st_mtime for f in (HOST_SRC, INCLUDE / "kbb200.h", torch / "version.py"))
+    if HOST_MODULE.exists() and HOST_MODULE.stat().st_mtime >= newest and not verbose:
+        return
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = HOST_MODULE.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", str(HOST_SRC), "-o", str(tmp),
+           "-I", sysconfig.get_paths()["include"], "-I", str(torch / "include"),
+           "-I", str(torch / "include" / "torch" / "csrc" / "api" / "include"), "-I", str(cuda / "include"),
+           "-L", str(torch / "lib"), "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on {HOST_SRC.name}:\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, HOST_MODULE)
+
+
 def build(jobs: int | None = None, clean: bool = False, verbose: bool = False) -> Path:
-    if clean and BUILD.exists():
-        shutil.rmtree(BUILD)
+    if clean:
+        if BUILD.exists():
+            shutil.rmtree(BUILD)
+        HOST_MODULE.unlink(missing_ok=True)
     BUILD.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.cu"))
     hdr = _headers_mtime()
@@ -68,8 +94,10 @@ def build(jobs: int | None = None, clean: bool = False, verbose: bool = False) -
         if verbose or not o.exists() or o.stat().st_mtime < max(s.stat().st_mtime, hdr):
             stale.append(s)
     jobs = jobs or min(len(stale) or 1, os.cpu_count() or 4)
-    with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+    with cf.ThreadPoolExecutor(max_workers=jobs + 1) as ex:
+        host = ex.submit(_build_host_module, verbose)
         list(ex.map(lambda s: _compile(s, verbose), stale))
+        host.result()
     objs = [BUILD / (s.stem + ".o") for s in sources]
     if stale or not LIB.exists() or LIB.stat().st_mtime < max(o.stat().st_mtime for o in objs):
         tmp = LIB.with_suffix(".so.tmp")

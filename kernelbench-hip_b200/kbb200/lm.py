@@ -14,16 +14,28 @@ Tensors are fp32, fp16 or bf16 on one CUDA device.  Every function checks its
 tensors, allocates outputs and scratch through torch's caching allocator and
 launches on torch's current stream; it never waits for the GPU.  A C-ABI error
 raises KbError.
+
+Decoding makes these calls once per layer and token, so the way of right
+arguments is native (csrc/lm_host.cpp): it checks them, allocates and calls the
+C ABI, and answers None where anything is not plainly right.  Then the checks
+here run one by one and say what is wrong, or the call is made from here.
 """
 from __future__ import annotations
 
-from functools import lru_cache
+import ctypes
 
 import torch
 
-from ._lib import LIB, KbError
-from .ops import _get_raw_stream, _ptr
-from .ops import _stream as _stream_of
+from ._lib import LIB, SIGNATURES, check
+from .ops import _ptr, _stream, _workspace
+
+try:
+    from . import _lm_host as _host
+except ImportError as e:
+    raise ImportError("kbb200/_lm_host.so is missing or was built for another torch: build it with "
+                      "`python kernelbench-hip_b200/build.py`") from e
+
+_host.init({name: ctypes.cast(getattr(LIB, name), ctypes.c_void_p).value for name in SIGNATURES})
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_backward", "rope_tables", "shared_prefix_attention", "cache_reserve",
            "cache_append", "cache_fork", "cache_free", "cache_compact", "cache_copy", "penalize_logits"]
@@ -31,65 +43,6 @@ __all__ = ["qk_norm_rope", "qk_norm_rope_backward", "rope_tables", "shared_prefi
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _INTS = {torch.int32: 0, torch.int64: 1}
 _POOLS = (torch.float32, torch.float16, torch.bfloat16, torch.uint8, torch.int8)
-
-# Decoding makes these calls once per layer and token, so a call's time on the
-# host counts: each function first asks one compact question that all right
-# arguments answer with yes, and only on a no goes through the checks one by
-# one, to say what is wrong.
-_empty, _empty_like = torch.empty, torch.empty_like
-_F32, _I32 = torch.float32, torch.int32
-
-
-def _stream(dev: int, t: torch.Tensor) -> int:
-    return _get_raw_stream(dev) if _get_raw_stream is not None else _stream_of(t)
-
-
-def _like(x: torch.Tensor) -> torch.Tensor:
-    """A new contiguous tensor of x's shape and type (empty_like costs half of empty; it keeps another order of
-    memory than the contiguous one where x has one)."""
-    y = _empty_like(x)
-    return y if y.is_contiguous() else _empty(x.shape, device=x.device, dtype=x.dtype)
-
-
-def _scratch(nbytes: int, like: torch.Tensor) -> torch.Tensor:
-    """Workspace of nbytes, made of `like`'s 32-bit elements."""
-    return like.new_empty((nbytes + 3) // 4 if nbytes > 16 else 4)
-
-
-def check(fn: str, status: int) -> None:
-    if status != 0:
-        raise KbError(fn, status, LIB.kb_last_error().decode(errors="replace"))
-
-
-def _is(t, dtype, dev, dims) -> bool:
-    return isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.dim() == dims
-
-
-def _is_row(t, dtype, dev, n) -> bool:
-    """A contiguous tensor [n]."""
-    return (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == dev and t.dim() == 1
-            and t.shape[0] == n and t.is_contiguous())
-
-
-@lru_cache(maxsize=4096)
-def _attention_bytes(*sizes) -> int:
-    return LIB.kb_shared_prefix_attention_workspace_size(*sizes)
-
-
-@lru_cache(maxsize=4096)
-def _rope_backward_bytes(*sizes) -> int:
-    return LIB.kb_qk_norm_rope_backward_workspace_size(*sizes)
-
-
-@lru_cache(maxsize=4096)
-def _reserve_bytes(*sizes) -> int:
-    return LIB.kb_cache_reserve_workspace_size(*sizes)
-
-
-@lru_cache(maxsize=4096)
-def _fork_bytes(*sizes) -> int:
-    return LIB.kb_cache_fork_workspace_size(*sizes)
-
 
 def _tensor(name: str, what: str, t, dev: torch.device | None, dtypes, dims: int | None = None) -> torch.Tensor:
     if not isinstance(t, torch.Tensor):
@@ -123,7 +76,7 @@ def _vectors(name: str, what: str, t: torch.Tensor) -> torch.Tensor:
 def _out(name: str, t: torch.Tensor | None, like: torch.Tensor, shape, dtype=None) -> torch.Tensor:
     dtype = like.dtype if dtype is None else dtype
     if t is None:
-        return _empty(shape, device=like.device, dtype=dtype)
+        return torch.empty(shape, device=like.device, dtype=dtype)
     _tensor(name, "out", t, like.device, (dtype,))
     return _contiguous(name, "out", t, shape)
 
@@ -138,21 +91,6 @@ def rope_tables(length: int, rotary: int, base: float = 10000.0, device="cuda"):
 
 
 def _rope_args(name, q, k, q_weight, k_weight, cos, sin, positions):
-    if isinstance(q, torch.Tensor) and q.dim() == 3 and q.is_cuda:
-        T, hq, d = q.shape
-        dt, dev = q.dtype, q.get_device()
-        qs, ps = q.stride(), None
-        if (_is(k, dt, dev, 3) and dt in _DTYPES and isinstance(positions, torch.Tensor)
-                and (q_weight is None) == (k_weight is None) and T and hq and d > 1 and qs[2] == 1):
-            ks, wt, ps = k.stride(), _F32 if q_weight is None else q_weight.dtype, positions.dtype
-            n = k.shape
-            if (n[0] == T and n[2] == d and n[1] and ks[2] == 1 and (wt is dt or wt is _F32)
-                    and (q_weight is None or (_is_row(q_weight, wt, dev, d) and _is_row(k_weight, wt, dev, d)))
-                    and _is(cos, _F32, dev, 2) and _is(sin, _F32, dev, 2) and cos.shape == sin.shape
-                    and cos.is_contiguous() and sin.is_contiguous() and ps in _INTS and _is_row(positions, ps, dev, T)):
-                rows, half = cos.shape
-                return ((T, hq, n[1], d, 2 * half, rows, qs[0], qs[1], ks[0], ks[1]),
-                        (_DTYPES[dt], _DTYPES[wt], _INTS[ps]), dev)
     _tensor(name, "q", q, None, _DTYPES, 3)
     dev, dt = q.device, q.dtype
     _tensor(name, "k", k, dev, (dt,), 3)
@@ -179,7 +117,7 @@ def _rope_args(name, q, k, q_weight, k_weight, cos, sin, positions):
     _contiguous(name, "positions", positions, (T,))
     shape = (T, hq, hkv, d, 2 * cos.shape[1], cos.shape[0], q.stride(0), q.stride(1), k.stride(0), k.stride(1))
     kinds = (_DTYPES[dt], _DTYPES[wt if wt is not None else torch.float32], _INTS[positions.dtype])
-    return shape, kinds, q.get_device()
+    return shape, kinds
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps: float = 1e-6, interleaved: bool = False,
@@ -192,12 +130,15 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps: float = 1e-
     position outside the tables gives NaN in the rotated elements.  Returns new (or the given, contiguous) q
     and k."""
     fn = "kb_qk_norm_rope"
-    shape, kinds, dev = _rope_args(fn, q, k, q_weight, k_weight, cos, sin, positions)
-    qo = _like(q) if q_out is None else _out(fn, q_out, q, q.shape)
-    ko = _like(k) if k_out is None else _out(fn, k_out, k, k.shape)
+    if q_out is None and k_out is None:
+        out = _host.rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+        if out is not None:
+            return out
+    shape, kinds = _rope_args(fn, q, k, q_weight, k_weight, cos, sin, positions)
+    qo, ko = _out(fn, q_out, q, q.shape), _out(fn, k_out, k, k.shape)
     check(fn, LIB.kb_qk_norm_rope(q.data_ptr(), k.data_ptr(), _ptr(q_weight), _ptr(k_weight), cos.data_ptr(),
                                   sin.data_ptr(), positions.data_ptr(), qo.data_ptr(), ko.data_ptr(), *shape,
-                                  *kinds, 1 if interleaved else 0, eps, _stream(dev, q)))
+                                  *kinds, 1 if interleaved else 0, float(eps), _stream(q)))
     return qo, ko
 
 
@@ -207,22 +148,22 @@ def qk_norm_rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, po
     (contiguous).  A weight that is None has None.  Weight gradients have the weights' type; they are summed in
     fp64 in a fixed order."""
     fn = "kb_qk_norm_rope_backward"
-    shape, kinds, dev = _rope_args(fn, q, k, q_weight, k_weight, cos, sin, positions)
-    dt = q.dtype
+    out = _host.rope_backward(dq_out, dk_out, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if out is not None:
+        return out
+    shape, kinds = _rope_args(fn, q, k, q_weight, k_weight, cos, sin, positions)
     for what, g, x in (("dq_out", dq_out, q), ("dk_out", dk_out, k)):
-        if not (_is(g, dt, dev, 3) and g.shape == x.shape and g.is_contiguous()):
-            _tensor(fn, what, g, q.device, (dt,))
-            _contiguous(fn, what, g, x.shape)
+        _tensor(fn, what, g, q.device, (q.dtype,))
+        _contiguous(fn, what, g, x.shape)
     dq, dk = torch.empty_like(dq_out), torch.empty_like(dk_out)
     dqw = None if q_weight is None else torch.empty_like(q_weight)
     dkw = None if k_weight is None else torch.empty_like(k_weight)
-    need = _rope_backward_bytes(shape[0], shape[1], shape[2], shape[3])
-    ws = _scratch(need, cos)
+    ws = _workspace(q, LIB.kb_qk_norm_rope_backward_workspace_size(*shape[:4]))
     check(fn, LIB.kb_qk_norm_rope_backward(dq_out.data_ptr(), dk_out.data_ptr(), q.data_ptr(), k.data_ptr(),
                                            _ptr(q_weight), _ptr(k_weight), cos.data_ptr(), sin.data_ptr(),
                                            positions.data_ptr(), dq.data_ptr(), dk.data_ptr(), _ptr(dqw), _ptr(dkw),
-                                           *shape, *kinds, 1 if interleaved else 0, eps, ws.data_ptr(),
-                                           need, _stream(dev, q)))
+                                           *shape, *kinds, 1 if interleaved else 0, float(eps), ws.data_ptr(),
+                                           ws.numel(), _stream(q)))
     return dq, dk, dqw, dkw
 
 
@@ -239,43 +180,10 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix, table, lens, scale: flo
     Returns (out, lse): out like q, contiguous, and lse [batch, queries, heads_q] fp32, the logarithm of the sum
     of the exponentials; a query without keys (a slot whose lens is 0) gets zeros and -inf."""
     fn = "kb_shared_prefix_attention"
-    sizes = _attention_sizes(q, k_pages, v_pages, prefix, table, lens)
-    if sizes is None:
-        sizes = _attention_checks(fn, q, k_pages, v_pages, prefix, table, lens)
-    B, Q, hq, hkv, d, n_pre, width, pages, page_size, qs, ks, vs = sizes
-    code = _DTYPES[q.dtype]
-    o = _like(q) if out is None else _out(fn, out, q, q.shape)
-    lse = q.new_empty((B, Q, hq), dtype=_F32)
-    need = _attention_bytes(B, Q, hq, hkv, d, n_pre, width, page_size, code)
-    ws = _scratch(need, lens) if need else None
-    check(fn, LIB.kb_shared_prefix_attention(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), prefix.data_ptr(), table.data_ptr(), lens.data_ptr(),
-        o.data_ptr(), lse.data_ptr(), B, Q, hq, hkv, d, n_pre, width, pages, page_size, qs[0], qs[1], qs[2],
-        ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], d ** -0.5 if scale is None else scale, code,
-        _ptr(ws), need, _stream(q.get_device(), q)))
-    return o, lse
-
-
-def _attention_sizes(q, k_pages, v_pages, prefix, table, lens):
-    """The sizes of right arguments, else None."""
-    if not (isinstance(q, torch.Tensor) and q.dim() == 4 and q.is_cuda):
-        return None
-    dt, dev = q.dtype, q.get_device()
-    if not (dt in _DTYPES and _is(k_pages, dt, dev, 4) and _is(v_pages, dt, dev, 4) and _is(table, _I32, dev, 2)
-            and _is(prefix, _I32, dev, 1)):
-        return None
-    B, Q, hq, d = q.shape
-    n = k_pages.shape
-    pages, page_size, hkv, dk = n
-    qs, ks, vs = q.stride(), k_pages.stride(), v_pages.stride()
-    rows, width = table.shape
-    if (dk != d or d < 2 or n != v_pages.shape or qs[3] != 1 or ks[3] != 1 or vs[3] != 1 or rows != B
-            or not prefix.is_contiguous() or not table.is_contiguous() or not _is_row(lens, _I32, dev, B)):
-        return None
-    return B, Q, hq, hkv, d, prefix.shape[0], width, pages, page_size, qs, ks, vs
-
-
-def _attention_checks(fn, q, k_pages, v_pages, prefix, table, lens):
+    if out is None:
+        made = _host.attention(q, k_pages, v_pages, prefix, table, lens, scale)
+        if made is not None:
+            return made
     _tensor(fn, "q", q, None, _DTYPES, 4)
     dev, dt = q.device, q.dtype
     _tensor(fn, "k_pages", k_pages, dev, (dt,), 4)
@@ -295,17 +203,20 @@ def _attention_checks(fn, q, k_pages, v_pages, prefix, table, lens):
     _contiguous(fn, "lens", lens, (B,))
     if table.shape[0] != B:
         raise RuntimeError(f"{fn}: table has {table.shape[0]} rows for {B} sequences")
-    return (B, Q, hq, hkv, d, prefix.shape[0], table.shape[1], pages, page_size, q.stride(), k_pages.stride(),
-            v_pages.stride())
+    n_pre, width, code = prefix.shape[0], table.shape[1], _DTYPES[dt]
+    o = _out(fn, out, q, q.shape)
+    lse = torch.empty((B, Q, hq), device=dev, dtype=torch.float32)
+    ws = _workspace(q, LIB.kb_shared_prefix_attention_workspace_size(B, Q, hq, hkv, d, n_pre, width, page_size, code))
+    check(fn, LIB.kb_shared_prefix_attention(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), prefix.data_ptr(), table.data_ptr(), lens.data_ptr(),
+        o.data_ptr(), lse.data_ptr(), B, Q, hq, hkv, d, n_pre, width, pages, page_size, *q.stride()[:3],
+        *k_pages.stride()[:3], *v_pages.stride()[:3], float(d ** -0.5 if scale is None else scale), code,
+        ws.data_ptr(), ws.numel(), _stream(q)))
+    return o, lse
 
 
 # ------------------------------------------------------------------ the paged cache
 def _state(fn, table, lens, refs):
-    if isinstance(table, torch.Tensor) and table.is_cuda and table.dtype is _I32 and table.dim() == 2 and table.is_contiguous():
-        dev = table.get_device()
-        if ((lens is None or _is_row(lens, _I32, dev, table.shape[0]))
-                and (refs is None or (_is(refs, _I32, dev, 1) and refs.is_contiguous()))):
-            return table.device
     _tensor(fn, "table", table, None, (torch.int32,), 2)
     dev = table.device
     _contiguous(fn, "table", table)
@@ -319,17 +230,13 @@ def _state(fn, table, lens, refs):
 
 
 def _slots(fn, what, t, dev, n=None):
-    if (isinstance(t, torch.Tensor) and t.dtype is _I32 and t.device == dev and t.dim() == 1 and t.is_contiguous()
-            and (n is None or t.shape[0] == n)):
-        return t
     _tensor(fn, what, t, dev, (torch.int32,), 1)
     return _contiguous(fn, what, t, None if n is None else (n,))
 
 
 def _pool(fn, what, pool, dev, pages=None):
-    if not (isinstance(pool, torch.Tensor) and pool.dtype in _POOLS and pool.device == dev and pool.is_contiguous()):
-        _tensor(fn, what, pool, dev, _POOLS)
-        _contiguous(fn, what, pool)
+    _tensor(fn, what, pool, dev, _POOLS)
+    _contiguous(fn, what, pool)
     if pool.dim() < 3:
         raise RuntimeError(f"{fn}: {what} must be [planes, pages, page_size, ...], got {tuple(pool.shape)}")
     if pages is not None and pool.shape[1] != pages:
@@ -343,15 +250,17 @@ def cache_reserve(table, lens, refs, seqs, tokens: int, page_size: int):
     changed in place.  Returns granted [n] int32: 0 for a request that got nothing (the row or the pool is
     full, or the slot is out of range or listed again)."""
     fn = "kb_cache_reserve"
+    granted = _host.reserve(table, lens, refs, seqs, tokens, page_size)
+    if granted is not None:
+        return granted
     dev = _state(fn, table, lens, refs)
     n = _slots(fn, "seqs", seqs, dev).shape[0]
-    granted = _empty_like(seqs)
+    granted = torch.empty_like(seqs)
     sizes = (table.shape[0], table.shape[1], refs.shape[0], int(page_size))
-    need = _reserve_bytes(n, int(tokens), *sizes)
-    ws = _scratch(need, refs)
+    ws = _workspace(table, LIB.kb_cache_reserve_workspace_size(n, int(tokens), *sizes))
     check(fn, LIB.kb_cache_reserve(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(),
-                                   granted.data_ptr(), n, int(tokens), *sizes, ws.data_ptr(), need,
-                                   _stream(table.get_device(), table)))
+                                   granted.data_ptr(), n, int(tokens), *sizes, ws.data_ptr(), ws.numel(),
+                                   _stream(table)))
     return granted
 
 
@@ -359,51 +268,28 @@ def cache_append(k, v, k_pages, v_pages, table, lens, seqs) -> None:
     """Writes k, v [n, tokens, heads, dim] into the last `tokens` places of the slots seqs [n] int32 (which
     cache_reserve has made), in one layer's planes k_pages, v_pages [pages, page_size, heads, dim]."""
     fn = "kb_cache_append"
+    if _host.append(k, v, k_pages, v_pages, table, lens, seqs):
+        return
     dev = _state(fn, table, lens, None)
     n = _slots(fn, "seqs", seqs, dev).shape[0]
-    ks = _append_strides(k, v, k_pages, v_pages, dev, n)
-    if ks is None:
-        _append_checks(fn, k, v, k_pages, v_pages, dev, n)
-        ks = k.stride(), v.stride()
-    (ksn, kst, *_), (vsn, vst, *_) = ks
-    pages, page_size, h, d = k_pages.shape
-    e = k_pages.element_size()
-    check(fn, LIB.kb_cache_append(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                                  table.data_ptr(), lens.data_ptr(), seqs.data_ptr(), n, k.shape[1], table.shape[0],
-                                  table.shape[1], pages, page_size, page_size * h * d * e, h * d * e,
-                                  ksn * e, kst * e, vsn * e, vst * e,
-                                  _stream(table.get_device(), table)))
-
-
-def _append_strides(k, v, k_pages, v_pages, dev, n):
-    """The strides of right arguments, else None."""
-    if not (isinstance(k_pages, torch.Tensor) and k_pages.dim() == 4 and k_pages.device == dev):
-        return None
-    dt, i = k_pages.dtype, k_pages.get_device()
-    if not (dt in _DTYPES and _is(v_pages, dt, i, 4) and _is(k, dt, i, 4) and _is(v, dt, i, 4)
-            and k_pages.is_contiguous() and v_pages.is_contiguous()):
-        return None
-    size, kv, ks, vs = k_pages.shape, k.shape, k.stride(), v.stride()
-    d = size[3]
-    if (v_pages.shape != size or v.shape != kv or kv[0] != n or kv[2] != size[2] or kv[3] != d
-            or ks[2:] != (d, 1) or vs[2:] != (d, 1)):
-        return None
-    return ks, vs
-
-
-def _append_checks(fn, k, v, k_pages, v_pages, dev, n):
     _tensor(fn, "k_pages", k_pages, dev, _DTYPES, 4)
     dt = (k_pages.dtype,)
     _tensor(fn, "v_pages", v_pages, dev, dt, 4)
     _contiguous(fn, "k_pages", k_pages)
     _contiguous(fn, "v_pages", v_pages, k_pages.shape)
     pages, page_size, h, d = k_pages.shape
+    e = k_pages.element_size()
     for what, t in (("k", k), ("v", v)):
         _tensor(fn, what, t, dev, dt, 4)
         if t.shape[0] != n or t.shape[2:] != k_pages.shape[2:] or t.shape[1] != k.shape[1]:
             raise RuntimeError(f"{fn}: {what} has shape {tuple(t.shape)}, expected ({n}, {k.shape[1]}, {h}, {d})")
         if t.numel() and ((d > 1 and t.stride(3) != 1) or (h > 1 and t.stride(2) != d)):
             raise RuntimeError(f"{fn}: the heads of a token of {what} must be contiguous")
+    check(fn, LIB.kb_cache_append(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                  table.data_ptr(), lens.data_ptr(), seqs.data_ptr(), n, k.shape[1], table.shape[0],
+                                  table.shape[1], pages, page_size, page_size * h * d * e, h * d * e,
+                                  k.stride(0) * e, k.stride(1) * e, v.stride(0) * e, v.stride(1) * e,
+                                  _stream(table)))
 
 
 def cache_fork(pool, table, lens, refs, parents, children):
@@ -413,42 +299,48 @@ def cache_fork(pool, table, lens, refs, parents, children):
     permuted), and pages are taken before those of replaced children are given back.  Returns granted [n] int32
     as cache_reserve does."""
     fn = "kb_cache_fork"
+    granted = _host.fork(pool, table, lens, refs, parents, children)
+    if granted is not None:
+        return granted
     dev = _state(fn, table, lens, refs)
     page_bytes = _pool(fn, "pool", pool, dev, refs.shape[0])
     n = _slots(fn, "parents", parents, dev).shape[0]
     _slots(fn, "children", children, dev, n)
-    granted = _empty_like(parents)
+    granted = torch.empty_like(parents)
     slots, width = table.shape
-    need = _fork_bytes(n, slots, width)
-    ws = _scratch(need, refs)
+    ws = _workspace(table, LIB.kb_cache_fork_workspace_size(n, slots, width))
     check(fn, LIB.kb_cache_fork(pool.data_ptr(), table.data_ptr(), lens.data_ptr(), refs.data_ptr(),
                                 parents.data_ptr(), children.data_ptr(), granted.data_ptr(), n, slots, width,
-                                *pool.shape[:3], page_bytes, ws.data_ptr(), need,
-                                _stream(table.get_device(), table)))
+                                *pool.shape[:3], page_bytes, ws.data_ptr(), ws.numel(),
+                                _stream(table)))
     return granted
 
 
 def cache_free(table, lens, refs, seqs) -> None:
     """Empties the slots seqs [n] int32: their pages are given back, lens = 0, rows = -1."""
     fn = "kb_cache_free"
+    if _host.release(table, lens, refs, seqs):
+        return
     dev = _state(fn, table, lens, refs)
     n = _slots(fn, "seqs", seqs, dev).shape[0]
     check(fn, LIB.kb_cache_free(table.data_ptr(), lens.data_ptr(), refs.data_ptr(), seqs.data_ptr(), n,
-                                table.shape[0], table.shape[1], refs.shape[0], _stream(table.get_device(), table)))
+                                table.shape[0], table.shape[1], refs.shape[0], _stream(table)))
 
 
 def cache_compact(pool, table, refs):
     """Moves the live pages to the low end of pool [planes, pages, ...]: with n live pages, the i-th live page at
     or above n goes to the i-th free one below; table and refs follow.  Returns n as an int32 tensor [1]."""
     fn = "kb_cache_compact"
+    live = _host.compact(pool, table, refs)
+    if live is not None:
+        return live
     dev = _state(fn, table, None, refs)
     page_bytes = _pool(fn, "pool", pool, dev, refs.shape[0])
-    live = refs.new_empty(1)
-    need = LIB.kb_cache_compact_workspace_size(refs.shape[0])
-    ws = _scratch(need, refs)
+    live = torch.empty(1, device=dev, dtype=torch.int32)
+    ws = _workspace(table, LIB.kb_cache_compact_workspace_size(refs.shape[0]))
     check(fn, LIB.kb_cache_compact(pool.data_ptr(), table.data_ptr(), refs.data_ptr(), live.data_ptr(),
                                    table.shape[0], table.shape[1], pool.shape[0], pool.shape[1], page_bytes,
-                                   ws.data_ptr(), need, _stream(table.get_device(), table)))
+                                   ws.data_ptr(), ws.numel(), _stream(table)))
     return live
 
 
@@ -466,7 +358,7 @@ def cache_copy(src_pool, src, dst_pool, dst) -> None:
     _slots(fn, "dst", dst, dev, n)
     check(fn, LIB.kb_cache_copy(src_pool.data_ptr(), src.data_ptr(), dst_pool.data_ptr(), dst.data_ptr(), n,
                                 src_pool.shape[0], page_bytes, src_pool.shape[1], dst_pool.shape[1],
-                                _stream(src_pool.get_device(), src_pool)))
+                                _stream(src_pool)))
 
 
 # ------------------------------------------------------------------ logits
@@ -484,11 +376,13 @@ def penalize_logits(logits, prompt=None, output=None, repetition=None, presence=
     [rows or 1, ceil(vocab / 32)], token v at bit v % 32 of word v // 32.  All may be None.  `out` may be logits
     itself (contiguous)."""
     fn = "kb_penalize_logits"
-    if not (isinstance(logits, torch.Tensor) and logits.is_cuda and logits.dtype in _DTYPES and logits.dim() == 2
-            and logits.stride(1) == 1):
-        _tensor(fn, "logits", logits, None, _DTYPES, 2)
-        _vectors(fn, "logits", logits)
-    dev, index = logits.device, logits.get_device()
+    if out is None:
+        made = _host.logits(logits, prompt, output, repetition, presence, frequency, bias_ids, bias_values, mask)
+        if made is not None:
+            return made
+    _tensor(fn, "logits", logits, None, _DTYPES, 2)
+    _vectors(fn, "logits", logits)
+    dev = logits.device
     B, V = logits.shape
     ids = None
     lengths = []
@@ -496,19 +390,17 @@ def penalize_logits(logits, prompt=None, output=None, repetition=None, presence=
         if t is None:
             lengths.append(0)
             continue
-        if not (_is(t, ids if ids is not None else torch.int64, index, 2) and t.is_contiguous() and t.shape[0] == B):
-            _tensor(fn, what, t, dev, _INTS if ids is None else (ids,), 2)
-            _contiguous(fn, what, t, (B, t.shape[1]))
+        _tensor(fn, what, t, dev, _INTS if ids is None else (ids,), 2)
         ids = t.dtype
+        _contiguous(fn, what, t, (B, t.shape[1]))
         lengths.append(t.shape[1])
     for what, t in (("repetition", repetition), ("presence", presence), ("frequency", frequency)):
-        if t is not None and not _is_row(t, _F32, index, B):
+        if t is not None:
             _tensor(fn, what, t, dev, (torch.float32,), 1)
             _contiguous(fn, what, t, (B,))
     if (bias_ids is None) != (bias_values is None):
         raise RuntimeError(f"{fn}: bias_ids and bias_values go together")
-    if bias_values is not None and not (_is(bias_values, _F32, index, 2) and bias_values.is_contiguous()
-                                        and bias_values.shape == bias_ids.shape):
+    if bias_values is not None:
         _tensor(fn, "bias_values", bias_values, dev, (torch.float32,), 2)
         _contiguous(fn, "bias_values", bias_values, bias_ids.shape)
     mask_stride = 0
@@ -519,9 +411,9 @@ def penalize_logits(logits, prompt=None, output=None, repetition=None, presence=
             raise RuntimeError(f"{fn}: mask has shape {tuple(mask.shape)}, expected ({B} or 1, {words})")
         _contiguous(fn, "mask", mask)
         mask_stride = words if mask.shape[0] == B else 0
-    y = _like(logits) if out is None else _out(fn, out, logits, logits.shape)
+    y = _out(fn, out, logits, logits.shape)
     check(fn, LIB.kb_penalize_logits(logits.data_ptr(), y.data_ptr(), _ptr(prompt), _ptr(output), _ptr(repetition),
                                      _ptr(presence), _ptr(frequency), _ptr(bias_ids), _ptr(bias_values), _ptr(mask),
                                      B, V, logits.stride(0), *lengths, mask_stride, _DTYPES[logits.dtype],
-                                     1 if ids is torch.int64 else 0, _stream(index, logits)))
+                                     1 if ids is torch.int64 else 0, _stream(logits)))
     return y
