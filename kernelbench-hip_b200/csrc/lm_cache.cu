@@ -36,6 +36,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxPages = 1 << 20, kMaxSlots = 1 << 20;
+constexpr int kSharedSlots = 4096;  // slots whose owners shared memory holds
 
 // Programmatic dependent launch: the next launch may start once all CTAs have
 // passed allow_next(); it waits for this one's results in wait_for_previous().
@@ -96,12 +97,13 @@ __device__ __forceinline__ int block_scan(int v, int* red, int& total) {
 }
 
 // list[r] = the r-th lowest page with refs == 0, for r < want; returns how
-// many there are, at most `want`.
-__device__ int free_pages(const int* refs, int pages, int want, int* list, int* red) {
+// many there are, at most `want`.  `first`: refs[threadIdx.x], loaded ahead
+// (nonzero past the pages).
+__device__ int free_pages(const int* refs, int pages, int want, int* list, int* red, int first) {
   int found = 0;
   for (int base = 0; base < pages && found < want; base += kPlanThreads) {
     const int p = base + threadIdx.x;
-    const int is_free = p < pages && refs[p] == 0;
+    const int is_free = p < pages && (base == 0 ? first : refs[p]) == 0;
     int total;
     const int at = found + block_scan(is_free, red, total);
     if (is_free && at < want) list[at] = p;
@@ -124,26 +126,36 @@ struct ForkArgs {
   int *rows;    // [n][width] the children's new rows
 };
 
+// A chain of latencies: what does not depend on another load is loaded at the
+// start, and the slots' owners and the free pages stay in shared memory where
+// they fit.
 __global__ void __launch_bounds__(kPlanThreads) fork_plan(ForkArgs a) {
   __shared__ int red[32];
+  __shared__ int s_owner[kSharedSlots], s_list[kPlanThreads];
   allow_next();
-  for (int i = threadIdx.x; i < a.slots; i += kPlanThreads) a.owner[i] = a.n;
+  int* owner = a.slots <= kSharedSlots ? s_owner : a.owner;
+  int* list = a.n <= kPlanThreads ? s_list : a.list;
+  const int mine = threadIdx.x;
+  const int first = mine < a.pages ? a.refs[mine] : 1;
+  const int parent0 = mine < a.n ? a.parents[mine] : -1, child0 = mine < a.n ? a.children[mine] : -1;
+  const int len0 = parent0 >= 0 && parent0 < a.slots ? a.lens[parent0] : 0;
+  for (int i = mine; i < a.slots; i += kPlanThreads) owner[i] = a.n;
   __syncthreads();
-  for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
-    const int c = a.children[i];
-    if (c >= 0 && c < a.slots) atomicMin(&a.owner[c], i);
+  for (int i = mine; i < a.n; i += kPlanThreads) {
+    const int c = i == mine ? child0 : a.children[i];
+    if (c >= 0 && c < a.slots) atomicMin(&owner[c], i);
   }
-  __syncthreads();
-  const int have = free_pages(a.refs, a.pages, a.n, a.list, red);
+  const int have = free_pages(a.refs, a.pages, a.n, list, red, first);  // ends with a barrier
+  __syncthreads();                                                      // where there was no page to look at
   int asked = 0;
   for (int base = 0; base < a.n; base += kPlanThreads) {
-    const int i = base + threadIdx.x;
+    const int i = base + mine;
     int need = 0, len = -1, ok = 0, src = -1;
     if (i < a.n) {
-      const int p = a.parents[i], c = a.children[i];
-      ok = p >= 0 && p < a.slots && c >= 0 && c < a.slots && a.owner[c] == i;
+      const int p = base ? a.parents[i] : parent0, c = base ? a.children[i] : child0;
+      ok = p >= 0 && p < a.slots && c >= 0 && c < a.slots && owner[c] == i;
       if (ok && p != c) {
-        len = max(0, min(a.lens[p], a.width * a.page_size));
+        len = max(0, min(base ? a.lens[p] : len0, a.width * a.page_size));
         if (len % a.page_size) {
           src = a.table[(int64_t)p * a.width + len / a.page_size];
           need = src >= 0 && src < a.pages;
@@ -158,7 +170,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan(ForkArgs a) {
       a.granted[i] = ok;
       a.len[i] = len;
       a.src[i] = need ? src : -1;
-      a.dst[i] = need ? a.list[rank] : -1;
+      a.dst[i] = need ? list[rank] : -1;
     }
   }
 }
@@ -263,25 +275,32 @@ struct ReserveArgs {
 
 __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(ReserveArgs a) {
   __shared__ int red[32];
-  for (int i = threadIdx.x; i < a.slots; i += kPlanThreads) a.owner[i] = a.n;
-  __syncthreads();
-  for (int i = threadIdx.x; i < a.n; i += kPlanThreads) {
-    const int c = a.seqs[i];
-    if (c >= 0 && c < a.slots) atomicMin(&a.owner[c], i);
-  }
-  __syncthreads();
+  __shared__ int s_owner[kSharedSlots], s_list[kPlanThreads];
   // no slot takes more pages than its row is wide, nor all more than there are
   const int most = (int)min((int64_t)a.pages, (int64_t)a.n * min(a.width, a.tokens / a.page_size + 1));
-  const int have = free_pages(a.refs, a.pages, most, a.list, red);
+  int* owner = a.slots <= kSharedSlots ? s_owner : a.owner;
+  int* list = most <= kPlanThreads ? s_list : a.list;
+  const int mine = threadIdx.x;
+  const int first = mine < a.pages ? a.refs[mine] : 1;
+  const int seq0 = mine < a.n ? a.seqs[mine] : -1;
+  const int len0 = seq0 >= 0 && seq0 < a.slots ? a.lens[seq0] : 0;
+  for (int i = mine; i < a.slots; i += kPlanThreads) owner[i] = a.n;
+  __syncthreads();
+  for (int i = mine; i < a.n; i += kPlanThreads) {
+    const int c = i == mine ? seq0 : a.seqs[i];
+    if (c >= 0 && c < a.slots) atomicMin(&owner[c], i);
+  }
+  const int have = free_pages(a.refs, a.pages, most, list, red, first);
+  __syncthreads();
   int asked = 0;
   for (int base = 0; base < a.n; base += kPlanThreads) {
-    const int i = base + threadIdx.x;
+    const int i = base + mine;
     int need = 0, ok = 0, held = 0, len = 0, c = -1;
     if (i < a.n) {
-      c = a.seqs[i];
-      ok = c >= 0 && c < a.slots && a.owner[c] == i;
+      c = base ? a.seqs[i] : seq0;
+      ok = c >= 0 && c < a.slots && owner[c] == i;
       if (ok) {
-        len = a.lens[c];
+        len = base ? a.lens[c] : len0;
         ok = len >= 0 && (int64_t)len + a.tokens <= (int64_t)a.width * a.page_size;
       }
       if (ok) {
@@ -298,7 +317,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(ReserveArgs a) {
       a.granted[i] = ok;
       if (ok) {
         for (int j = 0; j < need; ++j) {
-          const int p = a.list[rank + j];
+          const int p = list[rank + j];
           a.table[(int64_t)c * a.width + held + j] = p;
           a.refs[p] = 1;
         }

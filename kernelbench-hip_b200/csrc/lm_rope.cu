@@ -344,6 +344,7 @@ template <typename T, int L, int LAYOUT>
 __global__ void __launch_bounds__(kVecThreads, 4) rope_backward(RopeArgs a) {
   constexpr int kGroups = 32 / L, kBatch = 2;
   __shared__ double acc[kVecWarps][16][32];  // [warp][which * 8 + a0..3 b0..3][lane]
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / L;
   const Pairs<LAYOUT> pr(a, lane % L);
 #pragma unroll
@@ -559,21 +560,29 @@ __global__ void __launch_bounds__(kThreads) rope_backward_any(RopeArgs a) {
   }
 }
 
-// dw[e] = the sum of the CTAs' partials in their order.
+// dw[e] = the sum of the CTAs' partials, in an order that the sizes fix.
 template <typename W>
-__global__ void rope_weight_grads(const double* __restrict__ partial, int parts, int dim, W* __restrict__ dqw,
-                                  W* __restrict__ dkw) {
-  __shared__ double red[32][33];
-  const int lane = threadIdx.x, row = threadIdx.y;  // 32 x 32: a column of the partials per lane
-  const int e = blockIdx.x * 32 + lane;
+__global__ void __launch_bounds__(1024) rope_weight_grads(const double* __restrict__ partial, int parts, int dim,
+                                                          W* __restrict__ dqw, W* __restrict__ dkw) {
+  __shared__ double red[128][9];
+  const int col = threadIdx.x & 7, row = threadIdx.x >> 3;  // 8 columns of the partials x 128 of their rows
+  const int e = blockIdx.x * 8 + col;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the partials
   double s = 0.0;
   if (e < 2 * dim)
 #pragma unroll 8
-    for (int i = row; i < parts; i += 32) s += partial[(int64_t)i * 2 * dim + e];
-  red[row][lane] = s;
+    for (int i = row; i < parts; i += 128) s += partial[(int64_t)i * 2 * dim + e];
+  red[row][col] = s;
+  __syncthreads();
+  if (row < 16) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += red[row + 16 * i][col];
+    red[row][col] = s;
+  }
   __syncthreads();
   if (row || e >= 2 * dim) return;
-  for (int i = 1; i < 32; ++i) s += red[i][lane];
+#pragma unroll
+  for (int i = 1; i < 16; ++i) s += red[i][col];
   W* out = e < dim ? dqw : dkw;
   if (out) out[e < dim ? e : e - dim] = from_f32<W>((float)s);
 }
@@ -756,9 +765,15 @@ int kb_qk_norm_rope_backward(const void* dq_out, const void* dk_out, const void*
       if (int st = kb::check_launch(name)) return st;
     }
     if (!dq_weight && !dk_weight) return (int)KB_OK;
-    rope_weight_grads<W><<<(unsigned)kb::ceil_div(2 * dim, 32), dim3(32, 32), 0, stream>>>(
-        partial, grid, (int)dim, static_cast<W*>(dq_weight), static_cast<W*>(dk_weight));
-    return kb::check_launch(name);
+    cudaLaunchConfig_t config{};
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    config.gridDim = dim3((unsigned)kb::ceil_div(2 * dim, 8)), config.blockDim = dim3(1024), config.stream = stream;
+    config.attrs = &attr, config.numAttrs = 1;
+    KB_CUDA(cudaLaunchKernelEx(&config, rope_weight_grads<W>, (const double*)partial, grid, (int)dim,
+                               static_cast<W*>(dq_weight), static_cast<W*>(dk_weight)));
+    return (int)KB_OK;
   });
 }
 
