@@ -399,9 +399,12 @@ __global__ void __launch_bounds__(RowsCfg<T, DP, NK>::kThreads) attn_rows_kernel
 // a ring of its own filled by cp.async (no barrier until the end), and its own
 // running softmax; the four are joined in shared memory.  This is the shape of
 // decoding: a few query heads per key head against a sequence's own keys,
-// bound by the bytes of the cache.  Two stages at 128 columns: three CTAs per
-// SM rather than two with three (64 sequences of up to 1000 keys: 42 against
-// 47 us).
+// bound by the bytes of the cache.  Two stages, and blocks of 8 keys for 128
+// columns of fp32: what they leave of shared memory goes to more CTAs per SM.
+// Against one more stage (128 columns), 64 sequences of up to 1000 keys: 42
+// against 47 us; against four (64 columns): 60 against 89 us for 100 sequences
+// of 8 queries in fp32, 26 against 32 us for 64 of one query in fp16; blocks of
+// 8 against 16 (fp32, 16 sequences of up to 1024 keys): 27 against 37 us.
 template <typename T, int DP, int NK, int STAGES>
 struct KeysCfg {
   static constexpr int kRows = 16, kWarps = 4, kThreads = 128;
@@ -751,8 +754,8 @@ template <typename T>
 int launch_kind(Kind kind, const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {
   constexpr bool f32 = sizeof(T) == 4;
   if (kind == kKeys) {
-    if (a.dim <= 64) return launch_keys<T, 64, 16, 4>(a, first, items, stream);
-    if (a.dim <= 128) return launch_keys<T, 128, 16, 2>(a, first, items, stream);
+    if (a.dim <= 64) return launch_keys<T, 64, 16, 2>(a, first, items, stream);
+    if (a.dim <= 128) return launch_keys<T, 128, f32 ? 8 : 16, 2>(a, first, items, stream);
     return launch_keys<T, 256, f32 ? 8 : 16, 3>(a, first, items, stream);
   }
   if (a.dim <= 64) return launch_rows<T, 64, 64>(a, first, items, stream);
