@@ -45,6 +45,15 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+// Start of a kernel over keys.  The launch over the sequences' own keys needs
+// nothing of the one over the prefix, and its CTAs fill the SMs that that one
+// leaves: it reads on without a wait.  So the launch that comes first waits for
+// those before it first, and only then lets the next one begin.
+__device__ __forceinline__ void begin(const AttnArgs& a) {
+  if (a.first_item == 0) wait_for_previous();
+  allow_next();
+}
+
 // ------------------------------------------------------------------ products
 // Fragments of mma.sync: 16 rows x 8 columns of fp32 accumulators per warp.
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -284,7 +293,7 @@ __global__ void __launch_bounds__(RowsCfg<T, DP, NK>::kThreads) attn_rows_kernel
   T* sk = sq + C::kRows * LD;
   T* sv = sk + 2 * NK * LD;
   __shared__ int s_max[C::kWarps];
-  allow_next();
+  begin(a);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Item w = item_at(a, a.first_item + blockIdx.x, C::kRows);
   const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
@@ -423,7 +432,7 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
   T* sq = reinterpret_cast<T*>(raw);
   T* ring = sq + C::kRows * LD;
   __shared__ float s_m[4][16], s_l[4][16];
-  allow_next();
+  begin(a);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Item w = item_at(a, a.first_item + blockIdx.x, C::kRows);
   const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
@@ -600,11 +609,11 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
 // read (nothing was written there).
 constexpr int kJoin = 8;
 template <typename T>
-__global__ void __launch_bounds__(128) attn_join_kernel(const float* __restrict__ part_o,
-                                                        const float* __restrict__ part_lse, int splits, int64_t rows,
-                                                        int dim, T* __restrict__ out, float* __restrict__ lse) {
+__global__ void __launch_bounds__(128) attn_join_kernel(const float* part_o, const float* part_lse, int splits,
+                                                        int64_t rows, int dim, T* out, float* lse) {
   const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
+  allow_next();
   wait_for_previous();  // for the parts
   if (row >= rows) return;
   part_lse += row * splits;
@@ -709,15 +718,6 @@ size_t part_bytes(const Plan& p, int64_t rows, int64_t dim) {
   return p.splits() <= 1 ? 0 : (size_t)ceil_div(p.splits() * rows * (dim + 1), 4) * 16;
 }
 
-// The launch may begin once every CTA of the one before it has begun; the
-// kernel itself waits for that one's results (griddepcontrol.wait).
-cudaLaunchAttribute after_start() {
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  return attr;
-}
-
 template <typename K>
 int launch(K kern, int threads, size_t smem, AttnArgs a, int64_t first, int64_t items, uint64_t& attr_set,
            cudaStream_t stream) {
@@ -729,14 +729,7 @@ int launch(K kern, int threads, size_t smem, AttnArgs a, int64_t first, int64_t 
     if (dev < 64) attr_set |= 1ull << dev;
   }
   a.first_item = first;
-  cudaLaunchConfig_t config{};
-  cudaLaunchAttribute attr = after_start();
-  config.gridDim = dim3((unsigned)items), config.blockDim = dim3(threads), config.dynamicSmemBytes = smem;
-  config.stream = stream, config.attrs = &attr;
-  // the sequences' own keys need nothing of the prefix: their CTAs fill the SMs that it leaves
-  config.numAttrs = first > 0 ? 1 : 0;
-  KB_CUDA(cudaLaunchKernelEx(&config, kern, a));
-  return KB_OK;
+  return launch_after(kern, dim3((unsigned)items), (unsigned)threads, smem, stream, a);
 }
 template <typename T, int DP, int NK>
 int launch_rows(const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {
@@ -877,13 +870,9 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
       if (p.splits() == 1) return (int)KB_OK;
     }
     // also where there are no keys at all: zeros and -inf
-    cudaLaunchConfig_t config{};
-    cudaLaunchAttribute attr = after_start();
-    config.gridDim = dim3((unsigned)kb::ceil_div(rows, 4)), config.blockDim = dim3(128), config.stream = stream;
-    config.attrs = &attr, config.numAttrs = 1;
-    KB_CUDA(cudaLaunchKernelEx(&config, attn_join_kernel<T>, (const float*)a.part_o, (const float*)a.part_lse,
-                               p.splits(), rows, (int)dim, static_cast<T*>(out), lse));
-    return (int)KB_OK;
+    return launch_after(attn_join_kernel<T>, dim3((unsigned)kb::ceil_div(rows, 4)), 128u, 0, stream,
+                        (const float*)a.part_o, (const float*)a.part_lse, p.splits(), rows, dim, static_cast<T*>(out),
+                        lse);
   });
 }
 

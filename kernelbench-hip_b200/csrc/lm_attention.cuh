@@ -23,11 +23,6 @@ __device__ __forceinline__ float ex2(float x) {
 template <typename T>
 constexpr float kShift = std::is_same_v<T, __half> ? 7.0f : 0.0f;
 
-// Lets the next launch begin where it was made with programmatic stream
-// serialisation; it waits for this one's results by itself.
-__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 struct AttnArgs {
   const void *q, *k, *v;
   void* out;

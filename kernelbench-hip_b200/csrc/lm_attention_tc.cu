@@ -80,7 +80,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_end = reinterpret_cast<int*>(tmem_slot + 2);
-  allow_next();
+  // first of all, so that no CTA holds TMEM while a launch before it has to take its own
+  wait_for_previous();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Item w = item_at(a, blockIdx.x, row_tiles * kTile);
@@ -108,6 +109,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     tmem_relinquish();
   }
   __syncthreads();
+  allow_next();  // the sequences' own keys are read without a wait, and TMEM is taken
   // the keys that any row of this CTA sees
   const int t = warp >> 2, row = threadIdx.x & (kTile - 1);  // softmax warps: row tile, row in it
   const int r = t * kTile + row;
@@ -416,8 +418,8 @@ int launch_as(const AttnArgs& a, int dtype, int row_tiles, cudaStream_t stream) 
     KB_CUDA(cudaFuncSetAttribute(attn_prefix_kernel<T, HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
     if (dev < 64) attr_set |= 1ull << dev;
   }
-  attn_prefix_kernel<T, HALVES><<<(unsigned)a.prefix_items, kThreads, kSmemBytes, stream>>>(tk, tv, a, row_tiles);
-  return check_launch("kb_shared_prefix_attention");
+  return launch_after(attn_prefix_kernel<T, HALVES>, dim3((unsigned)a.prefix_items), (unsigned)kThreads, kSmemBytes,
+                      stream, tk, tv, a, row_tiles);
 }
 
 }  // namespace

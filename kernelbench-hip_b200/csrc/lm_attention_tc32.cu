@@ -175,7 +175,6 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_end = reinterpret_cast<int*>(tmem_slot + 2);
-  allow_next();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Item w = item_at(a, blockIdx.x, kTile);
@@ -201,6 +200,7 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
     tmem_relinquish();
   }
   __syncthreads();
+  allow_next();
   const int row = threadIdx.x & (kTile - 1);
   int vis = 0;
   if (warp < 4) {
@@ -465,17 +465,9 @@ int launch_as(const SplitArgs& s, cudaStream_t stream) {
                                                       (int64_t)sm_count() * 8);
   largest_kernel<<<blocks, 256, 0, stream>>>(s);
   if (int st = check_launch("kb_shared_prefix_attention")) return st;
-  cudaLaunchConfig_t config{};
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  config.gridDim = dim3(blocks), config.blockDim = dim3(256), config.stream = stream;
-  config.attrs = &attr, config.numAttrs = 1;
-  KB_CUDA(cudaLaunchKernelEx(&config, halves_kernel, s));
-  config.gridDim = dim3((unsigned)s.a.prefix_items), config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = kSmemBytes;
-  KB_CUDA(cudaLaunchKernelEx(&config, attn_prefix32_kernel<HALVES>, tm, s));
-  return KB_OK;
+  if (int st = launch_after(halves_kernel, dim3(blocks), 256u, 0, stream, s)) return st;
+  return launch_after(attn_prefix32_kernel<HALVES>, dim3((unsigned)s.a.prefix_items), (unsigned)kThreads, kSmemBytes,
+                      stream, tm, s);
 }
 
 }  // namespace

@@ -23,9 +23,11 @@
 //
 // The decisions are one CTA's (a chain of a few latencies, 5-7 us); the copies
 // run at HBM speed (64 children of one parent in 64 planes of 32 KB pages: 27
-// us for 134 MB written, the parent's page from L2).  The launches of a call
-// start while the one before ends (programmatic dependent launch), each waiting
-// for its results.  Rows of children that share their pages meet in refs: a
+// us for 134 MB written, the parent's page from L2).  Each launch starts while
+// the one before ends.  A fork of few table entries is two launches, the plan's
+// CTA writing the rows as well (4 children of 68 pages, with the reserve and the
+// append that follow: 12.4 against 14.4 us; 32 of 101 pages: 16.4 against 14.4).
+// Rows of children that share their pages meet in refs: a
 // thread takes one column of 16 rows and adds a page's changes up before its
 // atomic.
 #include "lm_common.cuh"
@@ -37,22 +39,7 @@ namespace {
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxPages = 1 << 20, kMaxSlots = 1 << 20;
 constexpr int kSharedSlots = 4096;  // slots whose owners shared memory holds
-
-// Programmatic dependent launch: the next launch may start once all CTAs have
-// passed allow_next(); it waits for this one's results in wait_for_previous().
-__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-template <typename... P, typename... A>
-int launch_after(void (*kernel)(P...), dim3 blocks, unsigned threads, cudaStream_t stream, A... args) {
-  cudaLaunchConfig_t config{};
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  config.gridDim = blocks, config.blockDim = dim3(threads), config.stream = stream;
-  config.attrs = &attr, config.numAttrs = 1;
-  KB_CUDA(cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...));
-  return KB_OK;
-}
+constexpr int kWholeRows = 2048;    // table entries that the fork's planning CTA writes itself
 
 // Changes of pages' counts that a thread meets one after the other, added up
 // while the page stays the same.
@@ -124,7 +111,14 @@ struct ForkArgs {
   int *src, *dst;  // [n] page to copy and where to, or -1
   int *len;     // [n] the child's new length, or -1 where nothing changes
   int *rows;    // [n][width] the children's new rows
+  bool whole;   // the plan's CTA writes the rows, too
 };
+
+// Entry j of the row of a child of `len` keys whose last page, if it was copied, is `dst`.
+__device__ __forceinline__ int new_entry(const ForkArgs& a, int len, int dst, int parent, int j) {
+  const int held = (len + a.page_size - 1) / a.page_size;
+  return j >= held ? -1 : (dst >= 0 && j == held - 1) ? dst : a.table[(int64_t)parent * a.width + j];
+}
 
 // A chain of latencies: what does not depend on another load is loaded at the
 // start, and the slots' owners and the free pages stay in shared memory where
@@ -132,7 +126,9 @@ struct ForkArgs {
 __global__ void __launch_bounds__(kPlanThreads) fork_plan(ForkArgs a) {
   __shared__ int red[32];
   __shared__ int s_owner[kSharedSlots], s_list[kPlanThreads];
+  __shared__ int s_child[kPlanThreads], s_len[kPlanThreads], s_dst[kPlanThreads];  // of the one-CTA case
   allow_next();
+  wait_for_previous();
   int* owner = a.slots <= kSharedSlots ? s_owner : a.owner;
   int* list = a.n <= kPlanThreads ? s_list : a.list;
   const int mine = threadIdx.x;
@@ -171,7 +167,34 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan(ForkArgs a) {
       a.len[i] = len;
       a.src[i] = need ? src : -1;
       a.dst[i] = need ? list[rank] : -1;
+      if (a.whole) s_child[i] = child0, s_len[i] = len, s_dst[i] = need ? list[rank] : -1;
     }
+  }
+  if (!a.whole) return;
+  // the rows as well: all are read before any is written
+  __shared__ int s_parent[kPlanThreads];
+  s_parent[mine] = parent0;
+  __syncthreads();
+  constexpr int kEach = kWholeRows / kPlanThreads;
+  const int entries = a.n * a.width;
+  int before[kEach], after[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int at = mine + k * kPlanThreads, i = at / max(a.width, 1), j = at - i * a.width;
+    before[k] = after[k] = -1;
+    if (at >= entries || s_len[i] < 0) continue;
+    before[k] = a.table[(int64_t)s_child[i] * a.width + j];
+    after[k] = new_entry(a, s_len[i], s_dst[i], s_parent[i], j);
+  }
+  __syncthreads();
+  if (mine < a.n && s_len[mine] >= 0) a.lens[child0] = s_len[mine];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int at = mine + k * kPlanThreads, i = at / max(a.width, 1), j = at - i * a.width;
+    if (at >= entries || s_len[i] < 0) continue;
+    a.table[(int64_t)s_child[i] * a.width + j] = after[k];
+    if (before[k] >= 0 && before[k] < a.pages) atomicSub(&a.refs[before[k]], 1);
+    if (after[k] >= 0 && after[k] < a.pages) atomicAdd(&a.refs[after[k]], 1);
   }
 }
 
@@ -179,14 +202,13 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan(ForkArgs a) {
 __device__ void fork_row(const ForkArgs& a, int i) {
   const int len = a.len[i];
   if (len < 0) return;
-  const int held = (len + a.page_size - 1) / a.page_size, dst = a.dst[i];
-  const int* from = a.table + (int64_t)a.parents[i] * a.width;
+  const int dst = a.dst[i], parent = a.parents[i];
   int* to = a.rows + (int64_t)i * a.width;
-  for (int j = threadIdx.x; j < a.width; j += blockDim.x)
-    to[j] = j >= held ? -1 : (dst >= 0 && j == held - 1) ? dst : from[j];
+  for (int j = threadIdx.x; j < a.width; j += blockDim.x) to[j] = new_entry(a, len, dst, parent, j);
 }
 
 __global__ void __launch_bounds__(kColumns) fork_commit(ForkArgs a) {
+  allow_next();
   wait_for_previous();
   const int j = blockIdx.x * kColumns + threadIdx.x, first = blockIdx.y * kRowsAtOnce;
   __shared__ int child[kRowsAtOnce];  // or -1 where nothing changes
@@ -253,7 +275,11 @@ __device__ void copy_pages(const CopyArgs& a, int64_t block, int64_t blocks) {
     }
   }
 }
-__global__ void __launch_bounds__(256) copy_kernel(CopyArgs a) { copy_pages(a, blockIdx.x, gridDim.x); }
+__global__ void __launch_bounds__(256) copy_kernel(CopyArgs a) {
+  allow_next();
+  wait_for_previous();
+  copy_pages(a, blockIdx.x, gridDim.x);
+}
 // The first n CTAs write the children's new rows, the others copy the pages.
 __global__ void __launch_bounds__(256) fork_rows(ForkArgs a, CopyArgs copy) {
   allow_next();
@@ -276,6 +302,8 @@ struct ReserveArgs {
 __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(ReserveArgs a) {
   __shared__ int red[32];
   __shared__ int s_owner[kSharedSlots], s_list[kPlanThreads];
+  allow_next();
+  wait_for_previous();
   // no slot takes more pages than its row is wide, nor all more than there are
   const int most = (int)min((int64_t)a.pages, (int64_t)a.n * min(a.width, a.tokens / a.page_size + 1));
   int* owner = a.slots <= kSharedSlots ? s_owner : a.owner;
@@ -338,6 +366,8 @@ struct AppendArgs {
 };
 
 __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
+  allow_next();
+  wait_for_previous();
   const int64_t i = blockIdx.x / a.tokens;
   const int t = (int)(blockIdx.x - i * a.tokens);
   const int c = a.seqs[i];
@@ -363,6 +393,8 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
 // ------------------------------------------------------------------ free
 __global__ void free_kernel(int* table, int* lens, int* refs, const int* seqs, int slots, int width, int pages) {
   __shared__ int len;
+  allow_next();
+  wait_for_previous();
   const int c = seqs[blockIdx.x];
   if (c < 0 || c >= slots) return;
   if (threadIdx.x == 0) len = atomicExch(&lens[c], 0);  // a slot that is listed twice is emptied once
@@ -389,6 +421,7 @@ struct CompactArgs {
 __global__ void __launch_bounds__(kPlanThreads) compact_plan(CompactArgs a) {
   __shared__ int red[32];
   allow_next();
+  wait_for_previous();
   int mine = 0, live;
   for (int p = threadIdx.x; p < a.pages; p += kPlanThreads) mine += a.refs[p] > 0;
   block_scan(mine, red, live);
@@ -423,6 +456,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan(CompactArgs a) {
 
 // The first `table_blocks` CTAs rewrite the table, the others move the pages.
 __global__ void __launch_bounds__(256) compact_moves(CompactArgs a, CopyArgs copy, int table_blocks) {
+  allow_next();
   wait_for_previous();
   if ((int)blockIdx.x >= table_blocks) {
     copy_pages(copy, blockIdx.x - table_blocks, gridDim.x - table_blocks);
@@ -477,22 +511,23 @@ int kb_cache_fork(void* pool, int32_t* table, int32_t* lens, int32_t* refs, cons
   KB_CACHE_WORKSPACE(kb_cache_fork_workspace_size(n, slots, width));
   char* w = static_cast<char*>(workspace);
   ForkArgs a{table, lens, refs, parents, children, granted, (int)n, (int)slots, (int)width, (int)pages, (int)page_size,
-             nullptr, nullptr, nullptr, nullptr, nullptr, nullptr};
+             nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, false};
   auto take = [&](int64_t m) {
     int* p = reinterpret_cast<int*>(w);
     w += ints(m);
     return p;
   };
   a.owner = take(slots), a.list = take(n), a.src = take(n), a.dst = take(n), a.len = take(n), a.rows = take(n * width);
-  fork_plan<<<1, kPlanThreads, 0, stream>>>(a);
-  if (int st = kb::check_launch(name)) return st;
+  a.whole = n <= kPlanThreads && n * width <= kWholeRows;
+  if (int st = launch_after(fork_plan, dim3(1), (unsigned)kPlanThreads, 0, stream, a)) return st;
   CopyArgs copy{static_cast<const char*>(pool), static_cast<char*>(pool), a.src, a.dst, nullptr, (int)n, planes,
                 page_bytes, pages, pages};
   const unsigned copies = planes && page_bytes && pages ? copy_grid(n * planes) : 0;
-  if (int st = launch_after(fork_rows, dim3((unsigned)n + copies), 256u, stream, a, copy)) return st;
+  if (a.whole) return copies ? launch_after(copy_kernel, dim3(copies), 256u, 0, stream, copy) : (int)KB_OK;
+  if (int st = launch_after(fork_rows, dim3((unsigned)n + copies), 256u, 0, stream, a, copy)) return st;
   return launch_after(fork_commit, dim3((unsigned)std::max<int64_t>(1, kb::ceil_div(width, kColumns)),
                                         (unsigned)kb::ceil_div(n, kRowsAtOnce)),
-                      (unsigned)kColumns, stream, a);
+                      (unsigned)kColumns, 0, stream, a);
 }
 
 size_t kb_cache_reserve_workspace_size(int64_t n, int64_t tokens, int64_t slots, int64_t width, int64_t pages,
@@ -517,8 +552,7 @@ int kb_cache_reserve(int32_t* table, int32_t* lens, int32_t* refs, const int32_t
   ReserveArgs a{table, lens, refs, seqs, granted, (int)n, (int)tokens, (int)slots, (int)width, (int)pages,
                 (int)page_size, static_cast<int*>(workspace),
                 reinterpret_cast<int*>(static_cast<char*>(workspace) + ints(slots))};
-  reserve_kernel<<<1, kPlanThreads, 0, stream>>>(a);
-  return kb::check_launch(name);
+  return launch_after(reserve_kernel, dim3(1), (unsigned)kPlanThreads, 0, stream, a);
 }
 
 int kb_cache_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
@@ -537,8 +571,7 @@ int kb_cache_append(const void* k, const void* v, void* k_pages, void* v_pages, 
                static_cast<char*>(v_pages), table, lens, seqs, k_stride_seq, k_stride_token, v_stride_seq,
                v_stride_token, page_bytes, key_bytes, (int)n, (int)tokens, (int)slots, (int)width, (int)pages,
                (int)page_size};
-  append_kernel<<<(unsigned)(n * tokens), 128, 0, stream>>>(a);
-  return kb::check_launch(name);
+  return launch_after(append_kernel, dim3((unsigned)(n * tokens)), 128u, 0, stream, a);
 }
 
 int kb_cache_free(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* seqs, int64_t n, int64_t slots,
@@ -548,8 +581,8 @@ int kb_cache_free(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* s
   KB_CACHE_COMMON(n);
   if (n == 0 || slots == 0) return KB_OK;
   KB_REQUIRE(lens && seqs && (!width || table) && (!pages || refs), KB_ERR_INVALID_ARG, "%s: null pointer", name);
-  free_kernel<<<(unsigned)n, 256, 0, stream>>>(table, lens, refs, seqs, (int)slots, (int)width, (int)pages);
-  return kb::check_launch(name);
+  return launch_after(free_kernel, dim3((unsigned)n), 256u, 0, stream, table, lens, refs, seqs, (int)slots, (int)width,
+                      (int)pages);
 }
 
 size_t kb_cache_compact_workspace_size(int64_t pages) {
@@ -572,15 +605,14 @@ int kb_cache_compact(void* pool, int32_t* table, int32_t* refs, int32_t* live, i
   a.src = reinterpret_cast<int*>(w + 16);
   a.dst = reinterpret_cast<int*>(w + 16 + ints(pages));
   a.map = reinterpret_cast<int*>(w + 16 + 2 * ints(pages));
-  compact_plan<<<1, kPlanThreads, 0, stream>>>(a);
-  if (int st = kb::check_launch(name)) return st;
+  if (int st = launch_after(compact_plan, dim3(1), (unsigned)kPlanThreads, 0, stream, a)) return st;
   if (pages == 0) return KB_OK;
   CopyArgs copy{static_cast<const char*>(pool), static_cast<char*>(pool), a.src, a.dst, a.count, (int)pages, planes,
                 page_bytes, pages, pages};
   const unsigned copies = planes && page_bytes ? copy_grid(pages * planes) : 0;
   const unsigned rows = a.entries ? copy_grid(kb::ceil_div(a.entries, 1024)) : 0;
   if (copies + rows == 0) return KB_OK;
-  return launch_after(compact_moves, dim3(rows + copies), 256u, stream, a, copy, (int)rows);
+  return launch_after(compact_moves, dim3(rows + copies), 256u, 0, stream, a, copy, (int)rows);
 }
 
 int kb_cache_copy(const void* src_pool, const int32_t* src, void* dst_pool, const int32_t* dst, int64_t n,
@@ -594,8 +626,7 @@ int kb_cache_copy(const void* src_pool, const int32_t* src, void* dst_pool, cons
   KB_REQUIRE(src_pool && dst_pool && src && dst, KB_ERR_INVALID_ARG, "%s: null pointer", name);
   const CopyArgs copy{static_cast<const char*>(src_pool), static_cast<char*>(dst_pool), src, dst, nullptr, (int)n,
                       planes, page_bytes, src_pages, dst_pages};
-  copy_kernel<<<copy_grid(n * planes), 256, 0, stream>>>(copy);
-  return kb::check_launch(name);
+  return launch_after(copy_kernel, dim3(copy_grid(n * planes)), 256u, 0, stream, copy);
 }
 
 }  // extern "C"

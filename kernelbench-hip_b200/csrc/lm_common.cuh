@@ -1,5 +1,5 @@
 // lm_common.cuh — helpers shared by the language-model operators: element
-// types, 16-byte vectors of them, and page lookups.
+// types, pairs of fp32 values, and launches that begin while the one before ends.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -64,6 +64,25 @@ int with_dtype(int dtype, F f) {
     case KB_F16: return f(static_cast<__half*>(nullptr));
     default: return f(static_cast<__nv_bfloat16*>(nullptr));
   }
+}
+
+// Programmatic dependent launch, for every launch of these operators: it may
+// begin once all CTAs of the launch before it have passed allow_next() (or
+// ended), and nothing of that launch, nor of those before it, is read or
+// written before wait_for_previous() returns.  A decoding step is a chain of
+// launches of a few microseconds each, and their starts are a good part of it.
+__device__ __forceinline__ void allow_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 blocks, unsigned threads, size_t smem, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t config{};
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  config.gridDim = blocks, config.blockDim = dim3(threads), config.dynamicSmemBytes = smem, config.stream = stream;
+  config.attrs = &attr, config.numAttrs = 1;
+  KB_CUDA(cudaLaunchKernelEx(&config, kernel, static_cast<P>(args)...));
+  return KB_OK;
 }
 
 }  // namespace lm

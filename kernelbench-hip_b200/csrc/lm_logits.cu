@@ -157,7 +157,8 @@ __device__ __forceinline__ RowTerms terms_of(const LogitsArgs& a, int64_t row) {
 template <typename T>
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(LogitsArgs a) {
   constexpr int kSlice = kCopyThreads * kFlight * 16 / sizeof(T);
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  wait_for_previous();
+  allow_next();  // after the wait: the next launch reads the histories before its own
   const int64_t first = (int64_t)blockIdx.x * kSlice;
   Slice<T, kCopyThreads> slice(a, blockIdx.y, first, (int)min((int64_t)kSlice, a.vocab - first));
   slice.fetch(threadIdx.x);
@@ -182,6 +183,7 @@ template <typename T>
 __global__ void __launch_bounds__(kRowThreads) touched_kernel(LogitsArgs a, uint32_t size) {
   extern __shared__ __align__(16) uint32_t table[];
   uint32_t *keys = table, *words = table + size;
+  allow_next();
   const int64_t row = blockIdx.x;
   const List bias(a.bias_ids, row, a.n_bias, a.ids64), prompt(a.prompt, row, a.n_prompt, a.ids64),
       output(a.output, row, a.n_output, a.ids64);
@@ -239,7 +241,7 @@ __global__ void __launch_bounds__(kRowThreads) touched_kernel(LogitsArgs a, uint
         keys[i] = kNoKey;
     }
   }
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // until the copy is done
+  wait_for_previous();  // until the copy is done
   for (uint32_t i = threadIdx.x; i < size; i += kRowThreads)  // the thread's own slots: no barrier
     if (keys[i] != kNoKey) y[keys[i]] = from_f32<T>(__uint_as_float(words[i]));
 }
@@ -251,6 +253,8 @@ __global__ void __launch_bounds__(kThreads, 2) penalize_kernel(LogitsArgs a, int
   extern __shared__ __align__(16) uint32_t word[];  // [slice_size], then the list of tokens that have one
   uint16_t* list = reinterpret_cast<uint16_t*>(word + slice_size);
   __shared__ uint32_t listed;
+  allow_next();
+  wait_for_previous();
   const int64_t row = blockIdx.y, first = (int64_t)blockIdx.x * slice_size;
   const int n = (int)min((int64_t)slice_size, a.vocab - first);
   Slice<T, kThreads> slice(a, row, first, n);
@@ -345,21 +349,13 @@ int kb_penalize_logits(const void* logits, void* out, const void* prompt, const 
     if (ids == 0 || (ids <= kMaxTable / 2 && rows * vocab * (int64_t)sizeof(T) >= kLargeBytes)) {
       constexpr int kSlice = kCopyThreads * kFlight * 16 / sizeof(T);
       const dim3 grid((unsigned)kb::ceil_div(vocab, kSlice), (unsigned)rows);
-      copy_kernel<T><<<grid, kCopyThreads, 0, stream>>>(a);
-      if (int st = kb::check_launch(name)) return st;
+      if (int st = launch_after(copy_kernel<T>, grid, (unsigned)kCopyThreads, 0, stream, a)) return st;
       if (ids == 0) return (int)KB_OK;
       static uint64_t done = 0;
       if (int st = allow_smem((const void*)touched_kernel<T>, kMaxTable * 8, done)) return st;
       uint32_t size = 32;
       while (size < 2 * ids) size *= 2;
-      cudaLaunchConfig_t config{};
-      cudaLaunchAttribute attr{};
-      attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      attr.val.programmaticStreamSerializationAllowed = 1;
-      config.gridDim = dim3((unsigned)rows), config.blockDim = dim3(kRowThreads);
-      config.dynamicSmemBytes = size * 8, config.stream = stream, config.attrs = &attr, config.numAttrs = 1;
-      KB_CUDA(cudaLaunchKernelEx(&config, touched_kernel<T>, a, size));
-      return (int)KB_OK;
+      return launch_after(touched_kernel<T>, dim3((unsigned)rows), (unsigned)kRowThreads, size * 8, stream, a, size);
     }
     // Slices: as large as shared memory allows (the histories are read once
     // for each), smaller while that leaves SMs without work.
@@ -368,8 +364,7 @@ int kb_penalize_logits(const void* logits, void* out, const void* prompt, const 
     static uint64_t done = 0;
     if (int st = allow_smem((const void*)penalize_kernel<T>, kMaxSlice * 6, done)) return st;
     const dim3 grid((unsigned)kb::ceil_div(vocab, slice), (unsigned)rows);
-    penalize_kernel<T><<<grid, kThreads, (size_t)slice * 6, stream>>>(a, slice);
-    return kb::check_launch(name);
+    return launch_after(penalize_kernel<T>, grid, (unsigned)kThreads, (size_t)slice * 6, stream, a, slice);
   });
 }
 

@@ -286,6 +286,8 @@ struct Pairs {
 template <typename T, int L, int LAYOUT>
 __global__ void __launch_bounds__(kVecThreads, 8) rope_forward(RopeArgs a, uint32_t units) {
   constexpr int kGroups = 32 / L, kBatch = sizeof(T) == 2 ? 4 : 2;
+  allow_next();
+  wait_for_previous();
   const uint32_t id = blockIdx.x * kVecWarps + (threadIdx.x >> 5);
   if (id >= units) return;
   const int lane = threadIdx.x & 31, group = lane / L;
@@ -344,7 +346,8 @@ template <typename T, int L, int LAYOUT>
 __global__ void __launch_bounds__(kVecThreads, 4) rope_backward(RopeArgs a) {
   constexpr int kGroups = 32 / L, kBatch = 2;
   __shared__ double acc[kVecWarps][16][32];  // [warp][which * 8 + a0..3 b0..3][lane]
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  allow_next();
+  wait_for_previous();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = lane / L;
   const Pairs<LAYOUT> pr(a, lane % L);
 #pragma unroll
@@ -461,6 +464,8 @@ __global__ void __launch_bounds__(kVecThreads, 4) rope_backward(RopeArgs a) {
 template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads) rope_forward_any(RopeArgs a) {
   extern __shared__ float smem[];
+  allow_next();
+  wait_for_previous();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float* y = smem + warp * a.dim;
   const int total_heads = a.heads[0] + a.heads[1];
@@ -503,6 +508,8 @@ __global__ void __launch_bounds__(kThreads) rope_forward_any(RopeArgs a) {
 template <typename T, typename W>
 __global__ void __launch_bounds__(kThreads) rope_backward_any(RopeArgs a) {
   extern __shared__ double dsmem[];
+  allow_next();
+  wait_for_previous();
   // per warp: dw of both weights (fp64), then dy
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double* acc = dsmem + (int64_t)warp * 2 * a.dim;
@@ -562,12 +569,12 @@ __global__ void __launch_bounds__(kThreads) rope_backward_any(RopeArgs a) {
 
 // dw[e] = the sum of the CTAs' partials, in an order that the sizes fix.
 template <typename W>
-__global__ void __launch_bounds__(1024) rope_weight_grads(const double* __restrict__ partial, int parts, int dim,
-                                                          W* __restrict__ dqw, W* __restrict__ dkw) {
+__global__ void __launch_bounds__(1024) rope_weight_grads(const double* partial, int parts, int dim, W* dqw, W* dkw) {
   __shared__ double red[128][9];
   const int col = threadIdx.x & 7, row = threadIdx.x >> 3;  // 8 columns of the partials x 128 of their rows
   const int e = blockIdx.x * 8 + col;
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the partials
+  allow_next();
+  wait_for_previous();  // for the partials
   double s = 0.0;
   if (e < 2 * dim)
 #pragma unroll 8
@@ -690,8 +697,8 @@ int kb_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
     return with_dtype(dtype, [&](auto* x) {
       using T = std::remove_pointer_t<decltype(x)>;
       return with_layout(a, vector_ok(a, sizeof(T), false), [&](auto l, auto v) {
-        rope_forward<T, decltype(l)::value, decltype(v)::value><<<(unsigned)blocks, kVecThreads, 0, stream>>>(a, (uint32_t)units);
-        return kb::check_launch(name);
+        return launch_after(rope_forward<T, decltype(l)::value, decltype(v)::value>, dim3((unsigned)blocks),
+                            (unsigned)kVecThreads, 0, stream, a, units);
       });
     });
   }
@@ -700,8 +707,7 @@ int kb_qk_norm_rope(const void* q, const void* k, const void* q_weight, const vo
   return with_types(dtype, weight_dtype, [&](auto* x, auto* w) {
     using T = std::remove_pointer_t<decltype(x)>;
     using W = std::remove_pointer_t<decltype(w)>;
-    rope_forward_any<T, W><<<grid, kThreads, kWarps * dim * sizeof(float), stream>>>(a);
-    return kb::check_launch(name);
+    return launch_after(rope_forward_any<T, W>, dim3(grid), (unsigned)kThreads, kWarps * dim * sizeof(float), stream, a);
   });
 }
 
@@ -755,25 +761,18 @@ int kb_qk_norm_rope_backward(const void* dq_out, const void* dk_out, const void*
       KB_REQUIRE(units <= kMaxUnits, KB_ERR_UNSUPPORTED, "%s: too many tokens", name);
       grid = (int)std::min<int64_t>(kb::ceil_div(units, kVecWarps), (int64_t)kb::sm_count() * 4);  // four per SM
       if (int st = with_layout(a, vector_ok(a, sizeof(T), true), [&](auto l, auto v) {
-            rope_backward<T, decltype(l)::value, decltype(v)::value><<<grid, kVecThreads, 0, stream>>>(a);
-            return kb::check_launch(name);
+            return launch_after(rope_backward<T, decltype(l)::value, decltype(v)::value>, dim3((unsigned)grid),
+                                (unsigned)kVecThreads, 0, stream, a);
           }))
         return st;
     } else if (any) {
       const size_t smem = (size_t)kWarps * dim * (2 * sizeof(double) + sizeof(float));
-      rope_backward_any<T, W><<<grid, kThreads, smem, stream>>>(a);
-      if (int st = kb::check_launch(name)) return st;
+      if (int st = launch_after(rope_backward_any<T, W>, dim3((unsigned)grid), (unsigned)kThreads, smem, stream, a))
+        return st;
     }
     if (!dq_weight && !dk_weight) return (int)KB_OK;
-    cudaLaunchConfig_t config{};
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    config.gridDim = dim3((unsigned)kb::ceil_div(2 * dim, 8)), config.blockDim = dim3(1024), config.stream = stream;
-    config.attrs = &attr, config.numAttrs = 1;
-    KB_CUDA(cudaLaunchKernelEx(&config, rope_weight_grads<W>, (const double*)partial, grid, (int)dim,
-                               static_cast<W*>(dq_weight), static_cast<W*>(dk_weight)));
-    return (int)KB_OK;
+    return launch_after(rope_weight_grads<W>, dim3((unsigned)kb::ceil_div(2 * dim, 8)), 1024u, 0, stream,
+                        (const double*)partial, grid, dim, static_cast<W*>(dq_weight), static_cast<W*>(dk_weight));
   });
 }
 
