@@ -23,6 +23,11 @@ __device__ __forceinline__ float ex2(float x) {
 template <typename T>
 constexpr float kShift = std::is_same_v<T, __half> ? 7.0f : 0.0f;
 
+// What the tensor-core kernels multiply raw scores by after they have put -inf in
+// the masked ones' place: |c|, but the least normal number for a c of zero (a
+// scale of zero), since -inf x 0 would be a NaN.
+__device__ __forceinline__ float score_factor(float c) { return c == 0.0f ? 0x1p-126f : fabsf(c); }
+
 struct AttnArgs {
   const void *q, *k, *v;
   void* out;

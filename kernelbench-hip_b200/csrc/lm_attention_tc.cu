@@ -222,7 +222,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
     // ---------------- softmax: this thread's row
     const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
     const uint32_t s_addr = tmem + lanes + t * kTile, o_addr = tmem + lanes + o_col + t * kTile;
-    const float c = fabsf(a.scale_log2);
+    const float c = score_factor(a.scale_log2);
     if (n > 0) {
       // the row of Q into the swizzled tile, all copies in flight at once
       const char* src = static_cast<const char*>(query_of(a, w, r < w.rows ? r : 0, 2));

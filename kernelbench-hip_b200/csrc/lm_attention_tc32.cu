@@ -318,7 +318,7 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
     }
   } else if (warp < 4) {
     // ---------------- softmax
-    const float c = fabsf(a.scale_log2) * power2(min(max(-eq - ek, -126), 126));
+    const float c = score_factor(a.scale_log2 * power2(min(max(-eq - ek, -126), 126)));
     for (int j = 0; j < n; ++j) {
       ok = warp_wait(s_full(j), (j >> 1) & 1, abort_flag);
       if (!ok) break;
@@ -477,7 +477,7 @@ int launch_as(const SplitArgs& s, cudaStream_t stream) {
 // against 87 at 2.1e9, 162 against 267 at 8.6e9, 245 against 494 at 17e9 and 952
 // against 3394 at 131e9 (calls with short continuations).
 bool tc32_pays(int64_t rows, int64_t heads_kv, int64_t dim, int64_t keys) {
-  return dim <= kTile && rows > 16 && keys > 0 && 4.0 * rows * heads_kv * dim * keys >= 1.2e9;
+  return dim <= kTile && rows > 64 && keys > 0 && 4.0 * rows * heads_kv * dim * keys >= 1.2e9;
 }
 size_t tc32_bytes(int64_t heads_kv, int64_t dim, int64_t keys) {
   return 16 + (size_t)4 * heads_kv * padded_keys(keys) * (dim > 64 ? 128 : 64) * sizeof(__half);
