@@ -675,20 +675,32 @@ struct Plan {
 // One axis of keys for `sets` sets of `rows` query rows each: the kernel by
 // the number of rows, and ranges of keys that give every SM a few CTAs but no
 // CTA less than one block of keys.
-Part plan_part(int64_t sets, int64_t rows, int64_t keys, int dtype, bool tensor) {
+Part plan_part(int64_t sets, int64_t rows, int64_t keys, int64_t dim, int dtype, bool tensor) {
   Part p;
   if (keys <= 0) return p;
+  const bool f32 = dtype == KB_F32;
   // Up to a few row tiles the keys kernel reads the keys again for each (from
-  // L2) and is still faster than a wider tile that stays half empty: fp32, 24
-  // rows over 32000 keys 188 against 300 us, 64 rows 111 against 119; 16-bit, 32
-  // rows 44 against 76, 64 rows 38 against 34.
-  p.kind = rows <= (dtype == KB_F32 ? 64 : tensor ? 16 : 48) ? kKeys : tensor ? kTensor : kRows;
+  // L2) and is still faster than a wider tile that stays half empty (8 key heads
+  // x 128): fp32, 48 rows over 32000 keys 265 against 302 us (64: 342 against
+  // 300); 16-bit on mma.sync, 32 rows over 8192 keys 24 against 32, 64 rows 33
+  // against 35 (over 2048, 17 against 17).
+  const bool few = rows <= (f32 ? 64 : tensor ? 16 : 48);
+  // And where there is little to do, for it starts and ends sooner.  16-bit
+  // against tcgen05, 8 heads x 128: 64 rows over 64 keys 7.7 against 13 us, over
+  // 2048 17 against 19, over 8192 33 against 26; 512 rows over 256 keys 28
+  // against 29, over 1024 40 against 34; one head, 32 rows over 4096 keys 12
+  // against 15, over 32000 34 against 23.  fp32 against the rows kernel, 4 heads:
+  // 96 rows over 2080 keys x 128 27 against 37, x 64 18 against 22; 128 rows over
+  // 320 keys x 128 15 against 36, over 2080 39 against 37.
+  const double each = (double)rows * dim * keys;
+  const bool little = (f32 || tensor) && each <= (f32 ? 3e7 : 2e7) && 4.0 * sets * each < 1.2e9;
+  p.kind = few || little ? kKeys : tensor ? kTensor : kRows;
   if (p.kind == kTensor) {
     // One CTA per SM, equal ranges of whole 128-key tiles: the number of
     // ranges that makes the last wave end first, a range's fixed cost (the
     // queries, the first scores, the way out) counted as kFixed tiles.
     constexpr int64_t kFixed = 3;
-    p.tiles = (int)ceil_div(rows, (int64_t)(dtype == KB_F32 ? kTc32Rows : tc_tile_rows(rows)));
+    p.tiles = (int)ceil_div(rows, (int64_t)(f32 ? kTc32Rows : tc_tile_rows(rows)));
     const int64_t items = p.tiles * sets, tiles = ceil_div(keys, 128), most = std::min<int64_t>(tiles, 64);
     int64_t best = 0;
     for (int64_t s = 1; s <= most; ++s) {
@@ -698,7 +710,7 @@ Part plan_part(int64_t sets, int64_t rows, int64_t keys, int dtype, bool tensor)
     }
     return p;
   }
-  const int tile = p.kind == kKeys ? 16 : 16 * (dtype == KB_F32 ? rows_warps<float>() : rows_warps<__half>());
+  const int tile = p.kind == kKeys ? 16 : 16 * (f32 ? rows_warps<float>() : rows_warps<__half>());
   p.tiles = (int)ceil_div(rows, tile);
   const int64_t block = 64, least = p.kind == kKeys ? block : 2 * block;
   const int64_t items = p.tiles * sets;
@@ -707,11 +719,11 @@ Part plan_part(int64_t sets, int64_t rows, int64_t keys, int dtype, bool tensor)
   p.splits = (int)ceil_div(keys, p.chunk);
   return p;
 }
-Plan plan(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv, int64_t prefix_keys, int64_t own_keys,
-          int dtype, bool tensor) {
+Plan plan(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv, int64_t dim, int64_t prefix_keys,
+          int64_t own_keys, int dtype, bool tensor) {
   const int64_t rows = queries * (heads_q / heads_kv);
-  return {plan_part(heads_kv, batch * rows, prefix_keys, dtype, tensor),
-          plan_part(heads_kv * batch, rows, own_keys, dtype, false)};
+  return {plan_part(heads_kv, batch * rows, prefix_keys, dim, dtype, tensor),
+          plan_part(heads_kv * batch, rows, own_keys, dim, dtype, false)};
 }
 // Parts, then (fp32 on the tensor cores) the prefix in halves.
 size_t part_bytes(const Plan& p, int64_t rows, int64_t dim) {
@@ -772,7 +784,7 @@ size_t kb_shared_prefix_attention_workspace_size(int64_t batch, int64_t queries,
     return 0;
   const int64_t keys = prefix_pages * page_size;
   auto bytes = [&](bool tensor) {
-    return part_bytes(plan(batch, queries, heads_q, heads_kv, keys,
+    return part_bytes(plan(batch, queries, heads_q, heads_kv, dim, keys,
                            std::max<int64_t>(0, width - prefix_pages) * page_size, dtype, tensor),
                       batch * queries * heads_q, dim);
   };
@@ -835,7 +847,7 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
   a.scale_log2 = scale * kLog2e;
   const int64_t keys = prefix_pages * page_size;
   const bool tensor = dtype == KB_F32 ? tc32_pays(batch * queries * a.group, heads_kv, dim, keys) : tc_fits(a, dtype);
-  const Plan p = plan(batch, queries, heads_q, heads_kv, keys, own_pages * page_size, dtype, tensor);
+  const Plan p = plan(batch, queries, heads_q, heads_kv, dim, keys, own_pages * page_size, dtype, tensor);
   a.splits = p.splits();
   a.prefix_tiles = p.prefix.tiles, a.prefix_splits = p.prefix.splits, a.prefix_chunk = p.prefix.chunk;
   a.own_tiles = p.own.tiles, a.own_splits = p.own.splits, a.own_chunk = p.own.chunk;
