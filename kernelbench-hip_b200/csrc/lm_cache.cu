@@ -25,11 +25,10 @@
 // run at HBM speed (64 children of one parent in 64 planes of 32 KB pages: 27
 // us for 134 MB written, the parent's page from L2).  Each launch starts while
 // the one before ends.  A fork of few table entries is two launches, the plan's
-// CTA writing the rows as well (4 children of 68 pages, with the reserve and the
+// CTA writing the rows as well (4 children of 63 pages, with the reserve and the
 // append that follow: 12.4 against 14.4 us; 32 of 101 pages: 16.4 against 14.4).
-// Rows of children that share their pages meet in refs: a
-// thread takes one column of 16 rows and adds a page's changes up before its
-// atomic.
+// Else rows of children that share their pages meet in refs: a thread takes one
+// column of 16 rows and adds a page's changes up before its atomic.
 #include "lm_common.cuh"
 
 namespace kb {

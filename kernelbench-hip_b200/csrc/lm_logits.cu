@@ -29,7 +29,7 @@
 // change the result.
 //
 // 256 x 131072 bf16 with 3000 ids and 300 biases a row and a mask, on a B200:
-// 47 us, of which the copy takes 20 (142 MB, 7.1 TB/s); one launch of slices
+// 43 us, of which the copy takes 20 (142 MB, 7.1 TB/s); one launch of slices
 // took 63, and a cluster of CTAs per row that shared the histories out and
 // scattered them over distributed shared memory 112.
 #include "lm_common.cuh"

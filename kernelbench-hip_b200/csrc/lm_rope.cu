@@ -25,7 +25,9 @@
 // 16-byte loads; interleaved, eight elements in a row.  The norm's sum is
 // log2(L) shuffles, the rotation none.  A warp takes kBatch x 32 / L heads of
 // one token, all loads issued before the first use, so cos and sin are read
-// once per token and warp.
+// once per token and warp.  16384 tokens x 40 heads x 128, bf16, on a B200:
+// forward 67 us (5.0 TB/s of the 6.6 that a plain copy reaches), backward with
+// both weights' gradients 108 us (4.7 TB/s), where instruction issue is next.
 #include "lm_common.cuh"
 
 namespace kb {
