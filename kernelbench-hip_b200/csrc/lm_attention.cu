@@ -53,6 +53,8 @@ __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
+constexpr size_t kMaxSmem = 227 * 1024;  // of a block, what the kernels declare statically included
+
 // Start of a kernel over keys.  The launch over the sequences' own keys needs
 // nothing of the one over the prefix, and its CTAs fill the SMs that that one
 // leaves: it reads on without a wait.  So the launch that comes first waits for
@@ -290,6 +292,7 @@ struct RowsCfg {
   static constexpr int kWarps = rows_warps<T>(), kRows = 16 * kWarps, kThreads = 32 * kWarps;
   static constexpr int LD = DP + 16 / (int)sizeof(T);  // rows 16 bytes apart in the banks
   static constexpr size_t kSmem = sizeof(T) * LD * (kRows + 4 * NK);
+  static_assert(kSmem + 1024 <= kMaxSmem, "no block holds this");
 };
 
 template <typename T, int DP, int NK>
@@ -430,6 +433,7 @@ struct KeysCfg {
   static constexpr size_t kRing = sizeof(T) * kWarps * STAGES * kStage;
   static constexpr size_t kJoin = sizeof(float) * kWarps * kRows * (DP + 4);
   static constexpr size_t kSmem = sizeof(T) * kRows * LD + (kRing > kJoin ? kRing : kJoin);
+  static_assert(kSmem + 1024 <= kMaxSmem, "no block holds this");
 };
 
 template <typename T, int DP, int NK, int STAGES>
@@ -773,7 +777,7 @@ int launch_kind(Kind kind, const AttnArgs& a, int64_t first, int64_t items, cuda
   }
   if (a.dim <= 64) return launch_rows<T, 64, 64>(a, first, items, stream);
   if (a.dim <= 128) return launch_rows<T, 128, f32 ? 32 : 64>(a, first, items, stream);
-  return launch_rows<T, 256, f32 ? 32 : 64>(a, first, items, stream);
+  return launch_rows<T, 256, f32 ? 16 : 64>(a, first, items, stream);  // fp32: 200 KB with its 128 rows
 }
 
 }  // namespace
