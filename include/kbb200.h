@@ -452,7 +452,12 @@ KB_API int kb_shared_prefix_attention(const void* q, const void* k_pages, const 
  * requests.
  *   reserve  lens += tokens, with the pages that takes
  *   append   k, v [n, tokens, key_bytes] (strides in BYTES) into the last
- *            `tokens` places of slots seqs, of one layer's two planes
+ *            `tokens` places of slots seqs, of one layer's two planes.  A slot
+ *            whose reserve was refused has not grown: its last places hold
+ *            older keys, which other slots may share.  append_granted takes
+ *            what that reserve answered (granted[n], or NULL: all were) and
+ *            passes such a slot over; append writes wherever seqs says, so
+ *            its caller puts -1 there
  *   fork     children become copies of their parents: full pages shared, a
  *            last page that is not full copied, in every plane.  All parents
  *            are read before any child is replaced, and pages are taken
@@ -474,6 +479,14 @@ KB_API int kb_cache_append(const void* k, const void* v, void* k_pages, void* v_
                            int64_t pages, int64_t page_size, int64_t page_bytes,
                            int64_t key_bytes, int64_t k_stride_seq, int64_t k_stride_token,
                            int64_t v_stride_seq, int64_t v_stride_token, kbStream stream);
+KB_API int kb_cache_append_granted(const void* k, const void* v, void* k_pages, void* v_pages,
+                                   const int32_t* table, const int32_t* lens,
+                                   const int32_t* seqs, const int32_t* granted, int64_t n,
+                                   int64_t tokens, int64_t slots, int64_t width,
+                                   int64_t pages, int64_t page_size, int64_t page_bytes,
+                                   int64_t key_bytes, int64_t k_stride_seq,
+                                   int64_t k_stride_token, int64_t v_stride_seq,
+                                   int64_t v_stride_token, kbStream stream);
 KB_API size_t kb_cache_fork_workspace_size(int64_t n, int64_t slots, int64_t width);
 KB_API int kb_cache_fork(void* pool, int32_t* table, int32_t* lens, int32_t* refs,
                          const int32_t* parents, const int32_t* children, int32_t* granted,

@@ -8,7 +8,8 @@
 // of its row; a page that is not full belongs to one slot alone.
 //
 //   reserve  grows slots by `tokens` keys, taking pages
-//   append   writes keys and values at a slot's last `tokens` places
+//   append   writes keys and values at a slot's last `tokens` places, where
+//            the request that made them was granted
 //   fork     makes child slots copies of parent slots: full pages are
 //            shared, a last page that is not full is copied
 //   free     empties slots
@@ -359,6 +360,7 @@ struct AppendArgs {
   const char *k, *v;
   char *k_pages, *v_pages;
   const int *table, *lens, *seqs;
+  const int* granted;  // of the reserve that made the places, or null: all of them
   int64_t k_stride_seq, k_stride_tok, v_stride_seq, v_stride_tok;  // bytes
   int64_t page_bytes, key_bytes;  // a page, and one token's heads, of one plane
   int n, tokens, slots, width, pages, page_size;
@@ -370,7 +372,8 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
   const int64_t i = blockIdx.x / a.tokens;
   const int t = (int)(blockIdx.x - i * a.tokens);
   const int c = a.seqs[i];
-  if (c < 0 || c >= a.slots) return;
+  // A refused slot has not grown: its last places are older keys, which other slots may share.
+  if (c < 0 || c >= a.slots || (a.granted && !a.granted[i])) return;
   const int pos = a.lens[c] - a.tokens + t;
   if (pos < 0 || pos / a.page_size >= a.width) return;
   const int p = a.table[(int64_t)c * a.width + pos / a.page_size];
@@ -554,10 +557,11 @@ int kb_cache_reserve(int32_t* table, int32_t* lens, int32_t* refs, const int32_t
   return launch_after(reserve_kernel, dim3(1), (unsigned)kPlanThreads, 0, stream, a);
 }
 
-int kb_cache_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
-                    const int32_t* lens, const int32_t* seqs, int64_t n, int64_t tokens, int64_t slots, int64_t width,
-                    int64_t pages, int64_t page_size, int64_t page_bytes, int64_t key_bytes, int64_t k_stride_seq,
-                    int64_t k_stride_token, int64_t v_stride_seq, int64_t v_stride_token, kbStream stream) {
+int kb_cache_append_granted(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
+                            const int32_t* lens, const int32_t* seqs, const int32_t* granted, int64_t n,
+                            int64_t tokens, int64_t slots, int64_t width, int64_t pages, int64_t page_size,
+                            int64_t page_bytes, int64_t key_bytes, int64_t k_stride_seq, int64_t k_stride_token,
+                            int64_t v_stride_seq, int64_t v_stride_token, kbStream stream) {
   const char* name = "kb_cache_append";
   using namespace kb::lm;
   KB_CACHE_COMMON(n);
@@ -567,10 +571,19 @@ int kb_cache_append(const void* k, const void* v, void* k_pages, void* v_pages, 
   if (n == 0 || tokens == 0 || key_bytes == 0 || slots == 0 || width == 0 || pages == 0) return KB_OK;
   KB_REQUIRE(k && v && k_pages && v_pages && table && lens && seqs, KB_ERR_INVALID_ARG, "%s: null pointer", name);
   AppendArgs a{static_cast<const char*>(k), static_cast<const char*>(v), static_cast<char*>(k_pages),
-               static_cast<char*>(v_pages), table, lens, seqs, k_stride_seq, k_stride_token, v_stride_seq,
+               static_cast<char*>(v_pages), table, lens, seqs, granted, k_stride_seq, k_stride_token, v_stride_seq,
                v_stride_token, page_bytes, key_bytes, (int)n, (int)tokens, (int)slots, (int)width, (int)pages,
                (int)page_size};
   return launch_after(append_kernel, dim3((unsigned)(n * tokens)), 128u, 0, stream, a);
+}
+
+int kb_cache_append(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* table,
+                    const int32_t* lens, const int32_t* seqs, int64_t n, int64_t tokens, int64_t slots, int64_t width,
+                    int64_t pages, int64_t page_size, int64_t page_bytes, int64_t key_bytes, int64_t k_stride_seq,
+                    int64_t k_stride_token, int64_t v_stride_seq, int64_t v_stride_token, kbStream stream) {
+  return kb_cache_append_granted(k, v, k_pages, v_pages, table, lens, seqs, nullptr, n, tokens, slots, width, pages,
+                                 page_size, page_bytes, key_bytes, k_stride_seq, k_stride_token, v_stride_seq,
+                                 v_stride_token, stream);
 }
 
 int kb_cache_free(int32_t* table, int32_t* lens, int32_t* refs, const int32_t* seqs, int64_t n, int64_t slots,

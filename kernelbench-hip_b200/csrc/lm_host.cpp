@@ -26,7 +26,7 @@ namespace {
 #define KB_HOST_ENTRIES(X)                                                                                        \
   X(kb_qk_norm_rope) X(kb_qk_norm_rope_backward_workspace_size) X(kb_qk_norm_rope_backward)                        \
   X(kb_shared_prefix_attention_workspace_size) X(kb_shared_prefix_attention) X(kb_cache_reserve_workspace_size)    \
-  X(kb_cache_reserve) X(kb_cache_append) X(kb_cache_fork_workspace_size) X(kb_cache_fork) X(kb_cache_free)         \
+  X(kb_cache_reserve) X(kb_cache_append_granted) X(kb_cache_fork_workspace_size) X(kb_cache_fork) X(kb_cache_free)         \
   X(kb_cache_compact_workspace_size) X(kb_cache_compact) X(kb_penalize_logits)
 
 struct Abi {
@@ -248,12 +248,12 @@ PyObject* reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// k, v, k_pages, v_pages, table, lens, seqs
+// k, v, k_pages, v_pages, table, lens, seqs, granted or None
 PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  if (n != 7) Py_RETURN_NONE;
+  if (n != 8) Py_RETURN_NONE;
   const Tensor *k = tensor(args[0]), *v = tensor(args[1]), *kp = tensor(args[2]), *vp = tensor(args[3]),
-               *seqs = tensor(args[6]);
+               *seqs = tensor(args[6]), *granted = args[7] == Py_None ? nullptr : tensor(args[7]);
   const Device dev(tensor(args[4]));
   State s;
   if (!s.read(dev, args[4], args[5], nullptr) || !kp || code(kp->scalar_type()) < 0 || !dev.whole(seqs, at::kInt, 1))
@@ -261,14 +261,15 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::ScalarType type = kp->scalar_type();
   if (!dev.whole(kp, type, 4) || !dev.whole(vp, type, 4) || kp->sizes() != vp->sizes() || !dev.has(k, type, 4) ||
       !dev.has(v, type, 4) || k->sizes() != v->sizes() || k->size(0) != seqs->size(0) || k->size(2) != kp->size(2) ||
-      k->size(3) != kp->size(3))
+      k->size(3) != kp->size(3) || (args[7] != Py_None && !dev.row(granted, at::kInt, seqs->size(0))))
     Py_RETURN_NONE;
   const int64_t d = kp->size(3), h = kp->size(2), e = static_cast<int64_t>(kp->element_size());
   for (const Tensor* t : {k, v})
     if (t->stride(3) != 1 || t->stride(2) != d) Py_RETURN_NONE;
-  if (abi.kb_cache_append(ptr(k), ptr(v), ptr(kp), ptr(vp), ints(s.table), ints(s.lens), ints(seqs), seqs->size(0), k->size(1),
-                          s.table->size(0), s.table->size(1), kp->size(0), kp->size(1), kp->size(1) * h * d * e, h * d * e,
-                          k->stride(0) * e, k->stride(1) * e, v->stride(0) * e, v->stride(1) * e, dev.stream()))
+  if (abi.kb_cache_append_granted(ptr(k), ptr(v), ptr(kp), ptr(vp), ints(s.table), ints(s.lens), ints(seqs),
+                                  granted ? ints(granted) : nullptr, seqs->size(0), k->size(1), s.table->size(0),
+                                  s.table->size(1), kp->size(0), kp->size(1), kp->size(1) * h * d * e, h * d * e,
+                                  k->stride(0) * e, k->stride(1) * e, v->stride(0) * e, v->stride(1) * e, dev.stream()))
     Py_RETURN_NONE;
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS

@@ -7,7 +7,8 @@ for every sample, and each step decodes all samples together, the prompt's full 
 
 Per layer: ops.rms_norm, ops.matmul, lm.qk_norm_rope, lm.cache_append, lm.shared_prefix_attention, ops.gelu_tanh;
 per step: lm.cache_reserve, lm.penalize_logits, ops.softmax, ops.cumsum.  When a sample ends its slot is freed, and
-at the end the live pages are compacted.
+at the end the live pages are compacted.  A sample that the cache refuses a place ends there, without the host: what
+cache_reserve granted goes to cache_append, which leaves the slots of the others' requests alone.
 """
 from __future__ import annotations
 
@@ -69,9 +70,9 @@ class Cache:
         self.refs = torch.zeros(pages, device=device, dtype=torch.int32)
 
 
-def forward(model: Decoder, cache: Cache, tokens, slots, positions, prefix):
+def forward(model: Decoder, cache: Cache, tokens, slots, positions, prefix, granted):
     """Logits [sequences, queries, vocab] of the newest tokens [sequences, queries] of the slots, whose places in the
-    cache are reserved."""
+    cache are reserved where granted [sequences] is not 0."""
     s = model.s
     n, q = tokens.shape
     x = model.embedding[tokens].view(n * q, -1)
@@ -84,7 +85,7 @@ def forward(model: Decoder, cache: Cache, tokens, slots, positions, prefix):
                                         w["q_norm"], w["k_norm"], model.cos, model.sin, positions)
         values = qkv[:, (hq + hkv) * d:].view(n, q, hkv, d)
         k_pages, v_pages = cache.pool[2 * i], cache.pool[2 * i + 1]
-        lm.cache_append(keys.view(n, q, hkv, d), values, k_pages, v_pages, cache.table, cache.lens, slots)
+        lm.cache_append(keys.view(n, q, hkv, d), values, k_pages, v_pages, cache.table, cache.lens, slots, granted)
         o, _ = lm.shared_prefix_attention(queries.view(n, q, hq, d), k_pages, v_pages, prefix, rows, lens)
         x = x + ops.matmul(o.view(n * q, hq * d), w["out"])
         x = x + ops.matmul(ops.gelu_tanh(ops.matmul(ops.rms_norm(x, w["norm2"]), w["up"])), w["down"])
@@ -92,22 +93,25 @@ def forward(model: Decoder, cache: Cache, tokens, slots, positions, prefix):
 
 
 def generate(model: Decoder, prompt, samples: int, steps: int, seed: int = 0, repetition: float = 1.1,
-             frequency: float = 0.1, end_token: int | None = None):
-    """`samples` continuations [samples, steps] of the prompt [length] (-1 after an end token), and the logits of
-    every step as the model gave them [samples, steps, vocab]."""
+             frequency: float = 0.1, end_token: int | None = None, pages: int | None = None):
+    """`samples` continuations [samples, steps] of the prompt [length] (-1 after an end token, or where the cache of
+    `pages` pages, enough for all unless given, had no more room), and the logits of every step as the model gave them
+    [samples, steps, vocab]."""
     s, dev = model.s, prompt.device
     length = prompt.shape[0]
     per_sample = -(-(length % s.page + steps) // s.page) + 1
-    cache = Cache(s, samples + 1, -(-length // s.page) + samples * per_sample, dev)
+    cache = Cache(s, samples + 1, -(-length // s.page) + samples * per_sample if pages is None else pages, dev)
     root = torch.zeros(1, device=dev, dtype=torch.int32)
     none = torch.empty(0, device=dev, dtype=torch.int32)
 
     # the prompt, once
-    lm.cache_reserve(cache.table, cache.lens, cache.refs, root, length, s.page)
-    logits = forward(model, cache, prompt[None], root, torch.arange(length, device=dev), none)[:, -1].expand(samples, -1)
+    granted = lm.cache_reserve(cache.table, cache.lens, cache.refs, root, length, s.page)
+    logits = forward(model, cache, prompt[None], root, torch.arange(length, device=dev), none, granted)[:, -1].expand(samples, -1)
     # its slot for every sample; full pages are shared
     slots = torch.arange(1, samples + 1, device=dev, dtype=torch.int32)
-    lm.cache_fork(cache.pool, cache.table, cache.lens, cache.refs, root.expand(samples).contiguous(), slots)
+    forked = lm.cache_fork(cache.pool, cache.table, cache.lens, cache.refs, root.expand(samples).contiguous(), slots)
+    if not (granted.all() and forked.all()):  # the one look from the host, before the first step
+        raise RuntimeError(f"the prompt's {length} tokens and {samples} copies of it do not fit the cache")
     prefix = cache.table[0, : length // s.page].contiguous()
 
     g = torch.Generator(device=dev).manual_seed(seed)
@@ -115,21 +119,24 @@ def generate(model: Decoder, prompt, samples: int, steps: int, seed: int = 0, re
     history = prompt[None].expand(samples, -1).contiguous()
     rep, freq = (torch.full((samples,), v, device=dev) for v in (repetition, frequency))
     seen = []
+    alive = torch.ones(samples, device=dev, dtype=torch.bool)
     for step in range(steps):
         seen.append(logits)
         p = ops.softmax(lm.penalize_logits(logits.contiguous(), prompt=history, output=made, repetition=rep, frequency=freq))
         u = torch.rand(samples, 1, device=dev, generator=g)
         token = (ops.cumsum(p, 1) < u).sum(1).clamp_(max=s.vocab - 1)
-        if end_token is not None and step:
-            token = torch.where((made[:, step - 1] < 0) | (made[:, step - 1] == end_token), -1, token)
-            lm.cache_free(cache.table, cache.lens, cache.refs, torch.where(token < 0, slots, -1))
+        token = torch.where(alive, token, -1)
         made[:, step] = token
         if step + 1 == steps:
             break
-        # samples that have ended ask for nothing: slot -1 is passed over
-        lm.cache_reserve(cache.table, cache.lens, cache.refs, torch.where(token >= 0, slots, -1), 1, s.page)
+        if end_token is not None:
+            alive &= token != end_token
+        # samples that have ended give their pages back and ask for nothing: slot -1 is passed over
+        lm.cache_free(cache.table, cache.lens, cache.refs, torch.where(alive, -1, slots))
+        granted = lm.cache_reserve(cache.table, cache.lens, cache.refs, torch.where(alive, slots, -1), 1, s.page)
+        alive = granted != 0
         positions = torch.full((samples,), length + step, device=dev)
-        logits = forward(model, cache, token.clamp(min=0)[:, None], slots, positions, prefix)[:, 0]
+        logits = forward(model, cache, token.clamp(min=0)[:, None], slots, positions, prefix, granted)[:, 0]
     lm.cache_compact(cache.pool, cache.table, cache.refs)
     return made, torch.stack(seen, 1)
 

@@ -95,6 +95,7 @@ SIGNATURES: dict[str, tuple] = {
     "kb_cache_reserve_workspace_size": (_sz, [_i64] * 6),
     "kb_cache_reserve": (_int, [_p] * 5 + [_i64] * 6 + [_p, _sz, _p]),
     "kb_cache_append": (_int, [_p] * 7 + [_i64] * 12 + [_p]),
+    "kb_cache_append_granted": (_int, [_p] * 8 + [_i64] * 12 + [_p]),
     "kb_cache_fork_workspace_size": (_sz, [_i64] * 3),
     "kb_cache_fork": (_int, [_p] * 7 + [_i64] * 7 + [_p, _sz, _p]),
     "kb_cache_free": (_int, [_p] * 4 + [_i64] * 4 + [_p]),

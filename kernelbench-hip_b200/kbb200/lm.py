@@ -264,14 +264,19 @@ def cache_reserve(table, lens, refs, seqs, tokens: int, page_size: int):
     return granted
 
 
-def cache_append(k, v, k_pages, v_pages, table, lens, seqs) -> None:
+def cache_append(k, v, k_pages, v_pages, table, lens, seqs, granted=None) -> None:
     """Writes k, v [n, tokens, heads, dim] into the last `tokens` places of the slots seqs [n] int32 (which
-    cache_reserve has made), in one layer's planes k_pages, v_pages [pages, page_size, heads, dim]."""
+    cache_reserve has made), in one layer's planes k_pages, v_pages [pages, page_size, heads, dim].
+
+    granted [n] int32 is what that cache_reserve returned.  A slot that it refused has not grown: its last places
+    hold older keys, which other slots may share, and it is passed over.  Without granted all of seqs are written."""
     fn = "kb_cache_append"
-    if _host.append(k, v, k_pages, v_pages, table, lens, seqs):
+    if _host.append(k, v, k_pages, v_pages, table, lens, seqs, granted):
         return
     dev = _state(fn, table, lens, None)
     n = _slots(fn, "seqs", seqs, dev).shape[0]
+    if granted is not None:
+        _slots(fn, "granted", granted, dev, n)
     _tensor(fn, "k_pages", k_pages, dev, _DTYPES, 4)
     dt = (k_pages.dtype,)
     _tensor(fn, "v_pages", v_pages, dev, dt, 4)
@@ -285,11 +290,11 @@ def cache_append(k, v, k_pages, v_pages, table, lens, seqs) -> None:
             raise RuntimeError(f"{fn}: {what} has shape {tuple(t.shape)}, expected ({n}, {k.shape[1]}, {h}, {d})")
         if t.numel() and ((d > 1 and t.stride(3) != 1) or (h > 1 and t.stride(2) != d)):
             raise RuntimeError(f"{fn}: the heads of a token of {what} must be contiguous")
-    check(fn, LIB.kb_cache_append(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-                                  table.data_ptr(), lens.data_ptr(), seqs.data_ptr(), n, k.shape[1], table.shape[0],
-                                  table.shape[1], pages, page_size, page_size * h * d * e, h * d * e,
-                                  k.stride(0) * e, k.stride(1) * e, v.stride(0) * e, v.stride(1) * e,
-                                  _stream(table)))
+    check(fn, LIB.kb_cache_append_granted(k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+                                          table.data_ptr(), lens.data_ptr(), seqs.data_ptr(), _ptr(granted), n,
+                                          k.shape[1], table.shape[0], table.shape[1], pages, page_size,
+                                          page_size * h * d * e, h * d * e, k.stride(0) * e, k.stride(1) * e,
+                                          v.stride(0) * e, v.stride(1) * e, _stream(table)))
 
 
 def cache_fork(pool, table, lens, refs, parents, children):
