@@ -6,8 +6,10 @@
 // take a few microseconds: the same checks, allocations and ctypes marshalling
 // in Python took 12-20 us a call, here 4-8.  Every function returns None where
 // an argument is not plainly right (another type, size, layout or device than
-// the one the kernels take, or an error of the C ABI); kbb200/lm.py then goes
-// through its checks one by one, says what is wrong, or makes the call itself.
+// the one the kernels take); kbb200/lm.py then goes through its checks one by
+// one, says what is wrong, or makes the call itself.  A call of the C ABI is
+// made once: where it answers an error, that is raised from here, since an
+// operation in several launches may have changed the cache's state before it.
 //
 // The C ABI is reached through the addresses that init() is given, so this
 // module works with whichever libkbb200.so kbb200._lib has loaded.
@@ -33,7 +35,17 @@ struct Abi {
 #define X(name) decltype(&::name) name = nullptr;
   KB_HOST_ENTRIES(X)
 #undef X
+  PyObject* check = nullptr;  // kbb200._lib.check(entry, status), which raises
 } abi;
+
+// Whether the entry answered an error, which is then raised.
+bool failed(const char* entry, int status) {
+  if (status == KB_OK) return false;
+  PyObject* r = PyObject_CallFunction(abi.check, "si", entry, status);
+  if (r) PyErr_Format(PyExc_RuntimeError, "%s failed with status %d", entry, status);
+  Py_XDECREF(r);
+  return true;
+}
 
 using at::Tensor;
 
@@ -122,11 +134,12 @@ PyObject* rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Device dev(tensor(args[0]));
   if (!dev.ok() || !r.read(dev, args)) Py_RETURN_NONE;
   const Tensor q = like(*r.q), k = like(*r.k);
-  if (abi.kb_qk_norm_rope(ptr(r.q), ptr(r.k), ptr(r.qw), ptr(r.kw), static_cast<const float*>(ptr(r.cos)),
-                          static_cast<const float*>(ptr(r.sin)), ptr(r.pos), q.data_ptr(), k.data_ptr(), r.tokens, r.hq,
-                          r.hkv, r.dim, r.rotary, r.rows, r.q->stride(0), r.q->stride(1), r.k->stride(0), r.k->stride(1),
-                          code(r.type), code(r.weights), r.pos64, r.interleaved, r.eps, dev.stream()))
-    Py_RETURN_NONE;
+  const int status = abi.kb_qk_norm_rope(
+      ptr(r.q), ptr(r.k), ptr(r.qw), ptr(r.kw), static_cast<const float*>(ptr(r.cos)), static_cast<const
+      float*>(ptr(r.sin)), ptr(r.pos), q.data_ptr(), k.data_ptr(), r.tokens, r.hq, r.hkv, r.dim, r.rotary, r.rows,
+      r.q->stride(0), r.q->stride(1), r.k->stride(0), r.k->stride(1), code(r.type), code(r.weights), r.pos64,
+      r.interleaved, r.eps, dev.stream());
+  if (failed("kb_qk_norm_rope", status)) return nullptr;
   return pair(q, k);
   END_HANDLE_TH_ERRORS
 }
@@ -145,13 +158,13 @@ PyObject* rope_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor qw = r.qw ? like(*r.qw) : Tensor(), kw = r.kw ? like(*r.kw) : Tensor();
   const size_t need = abi.kb_qk_norm_rope_backward_workspace_size(r.tokens, r.hq, r.hkv, r.dim);
   const Tensor ws = scratch(need, *r.q);
-  if (abi.kb_qk_norm_rope_backward(
-          ptr(dzq), ptr(dzk), ptr(r.q), ptr(r.k), ptr(r.qw), ptr(r.kw), static_cast<const float*>(ptr(r.cos)),
-          static_cast<const float*>(ptr(r.sin)), ptr(r.pos), q.data_ptr(), k.data_ptr(), r.qw ? qw.data_ptr() : nullptr,
-          r.kw ? kw.data_ptr() : nullptr, r.tokens, r.hq, r.hkv, r.dim, r.rotary, r.rows, r.q->stride(0), r.q->stride(1),
-          r.k->stride(0), r.k->stride(1), code(r.type), code(r.weights), r.pos64, r.interleaved, r.eps, ws.data_ptr(), need,
-          dev.stream()))
-    Py_RETURN_NONE;
+  const int status = abi.kb_qk_norm_rope_backward(
+      ptr(dzq), ptr(dzk), ptr(r.q), ptr(r.k), ptr(r.qw), ptr(r.kw), static_cast<const float*>(ptr(r.cos)),
+      static_cast<const float*>(ptr(r.sin)), ptr(r.pos), q.data_ptr(), k.data_ptr(), r.qw ? qw.data_ptr() : nullptr,
+      r.kw ? kw.data_ptr() : nullptr, r.tokens, r.hq, r.hkv, r.dim, r.rotary, r.rows, r.q->stride(0), r.q->stride(1),
+      r.k->stride(0), r.k->stride(1), code(r.type), code(r.weights), r.pos64, r.interleaved, r.eps, ws.data_ptr(), need,
+      dev.stream());
+  if (failed("kb_qk_norm_rope_backward", status)) return nullptr;
   PyObject* out = PyTuple_New(4);
   if (!out) return nullptr;
   const Tensor all[4] = {q, k, qw, kw};
@@ -194,13 +207,13 @@ PyObject* attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor out = like(*q), lse = at::empty({B, Q, hq}, q->options().dtype(at::kFloat));
   const size_t need = abi.kb_shared_prefix_attention_workspace_size(B, Q, hq, hkv, d, pre, width, page, code(type));
   const Tensor ws = need ? scratch(need, *q) : Tensor();
-  if (abi.kb_shared_prefix_attention(
-          ptr(q), ptr(k), ptr(v), static_cast<const int32_t*>(ptr(prefix)), static_cast<const int32_t*>(ptr(table)),
-          static_cast<const int32_t*>(ptr(lens)), out.data_ptr(), static_cast<float*>(lse.data_ptr()), B, Q, hq, hkv, d, pre,
-          width, pages, page, q->stride(0), q->stride(1), q->stride(2), k->stride(0), k->stride(1), k->stride(2), v->stride(0),
-          v->stride(1), v->stride(2), static_cast<float>(scale), code(type), need ? ws.data_ptr() : nullptr, need,
-          dev.stream()))
-    Py_RETURN_NONE;
+  const int status = abi.kb_shared_prefix_attention(
+      ptr(q), ptr(k), ptr(v), static_cast<const int32_t*>(ptr(prefix)), static_cast<const int32_t*>(ptr(table)),
+      static_cast<const int32_t*>(ptr(lens)), out.data_ptr(), static_cast<float*>(lse.data_ptr()), B, Q, hq, hkv, d,
+      pre, width, pages, page, q->stride(0), q->stride(1), q->stride(2), k->stride(0), k->stride(1), k->stride(2),
+      v->stride(0), v->stride(1), v->stride(2), static_cast<float>(scale), code(type), need ? ws.data_ptr() : nullptr,
+      need, dev.stream());
+  if (failed("kb_shared_prefix_attention", status)) return nullptr;
   return pair(out, lse);
   END_HANDLE_TH_ERRORS
 }
@@ -241,9 +254,10 @@ PyObject* reserve(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor granted = like(*seqs);
   const size_t need = abi.kb_cache_reserve_workspace_size(m, tokens, slots, width, pages, page);
   const Tensor ws = scratch(need, *s.table);
-  if (abi.kb_cache_reserve(ints(s.table), ints(s.lens), ints(s.refs), ints(seqs), ints(&granted), m, tokens, slots, width,
-                           pages, page, ws.data_ptr(), need, dev.stream()))
-    Py_RETURN_NONE;
+  const int status = abi.kb_cache_reserve(
+      ints(s.table), ints(s.lens), ints(s.refs), ints(seqs), ints(&granted), m, tokens, slots, width, pages, page,
+      ws.data_ptr(), need, dev.stream());
+  if (failed("kb_cache_reserve", status)) return nullptr;
   return THPVariable_Wrap(granted);
   END_HANDLE_TH_ERRORS
 }
@@ -266,11 +280,11 @@ PyObject* append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t d = kp->size(3), h = kp->size(2), e = static_cast<int64_t>(kp->element_size());
   for (const Tensor* t : {k, v})
     if (t->stride(3) != 1 || t->stride(2) != d) Py_RETURN_NONE;
-  if (abi.kb_cache_append_granted(ptr(k), ptr(v), ptr(kp), ptr(vp), ints(s.table), ints(s.lens), ints(seqs),
-                                  granted ? ints(granted) : nullptr, seqs->size(0), k->size(1), s.table->size(0),
-                                  s.table->size(1), kp->size(0), kp->size(1), kp->size(1) * h * d * e, h * d * e,
-                                  k->stride(0) * e, k->stride(1) * e, v->stride(0) * e, v->stride(1) * e, dev.stream()))
-    Py_RETURN_NONE;
+  const int status = abi.kb_cache_append_granted(
+      ptr(k), ptr(v), ptr(kp), ptr(vp), ints(s.table), ints(s.lens), ints(seqs), granted ? ints(granted) : nullptr,
+      seqs->size(0), k->size(1), s.table->size(0), s.table->size(1), kp->size(0), kp->size(1), kp->size(1) * h * d * e,
+      h * d * e, k->stride(0) * e, k->stride(1) * e, v->stride(0) * e, v->stride(1) * e, dev.stream());
+  if (failed("kb_cache_append", status)) return nullptr;
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -291,10 +305,10 @@ PyObject* fork(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor granted = like(*parents);
   const size_t need = abi.kb_cache_fork_workspace_size(m, slots, width);
   const Tensor ws = scratch(need, *s.table);
-  if (abi.kb_cache_fork(ptr(pool), ints(s.table), ints(s.lens), ints(s.refs), ints(parents), ints(children), ints(&granted),
-                        m, slots, width, pool->size(0), pool->size(1), pool->size(2), bytes, ws.data_ptr(), need,
-                        dev.stream()))
-    Py_RETURN_NONE;
+  const int status = abi.kb_cache_fork(
+      ptr(pool), ints(s.table), ints(s.lens), ints(s.refs), ints(parents), ints(children), ints(&granted), m, slots,
+      width, pool->size(0), pool->size(1), pool->size(2), bytes, ws.data_ptr(), need, dev.stream());
+  if (failed("kb_cache_fork", status)) return nullptr;
   return THPVariable_Wrap(granted);
   END_HANDLE_TH_ERRORS
 }
@@ -307,9 +321,10 @@ PyObject* release(PyObject*, PyObject* const* args, Py_ssize_t n) {
   State s;
   const Tensor* seqs = tensor(args[3]);
   if (!s.read(dev, args[0], args[1], args[2]) || !dev.whole(seqs, at::kInt, 1)) Py_RETURN_NONE;
-  if (abi.kb_cache_free(ints(s.table), ints(s.lens), ints(s.refs), ints(seqs), seqs->size(0), s.table->size(0),
-                        s.table->size(1), s.refs->size(0), dev.stream()))
-    Py_RETURN_NONE;
+  const int status = abi.kb_cache_free(
+      ints(s.table), ints(s.lens), ints(s.refs), ints(seqs), seqs->size(0), s.table->size(0), s.table->size(1),
+      s.refs->size(0), dev.stream());
+  if (failed("kb_cache_free", status)) return nullptr;
   Py_RETURN_TRUE;
   END_HANDLE_TH_ERRORS
 }
@@ -327,9 +342,10 @@ PyObject* compact(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor live = at::empty({1}, s.refs->options());
   const size_t need = abi.kb_cache_compact_workspace_size(s.refs->size(0));
   const Tensor ws = scratch(need, *s.table);
-  if (abi.kb_cache_compact(ptr(pool), ints(s.table), ints(s.refs), ints(&live), s.table->size(0), s.table->size(1),
-                           pool->size(0), pool->size(1), bytes, ws.data_ptr(), need, dev.stream()))
-    Py_RETURN_NONE;
+  const int status = abi.kb_cache_compact(
+      ptr(pool), ints(s.table), ints(s.refs), ints(&live), s.table->size(0), s.table->size(1), pool->size(0),
+      pool->size(1), bytes, ws.data_ptr(), need, dev.stream());
+  if (failed("kb_cache_compact", status)) return nullptr;
   return THPVariable_Wrap(live);
   END_HANDLE_TH_ERRORS
 }
@@ -368,17 +384,23 @@ PyObject* logits(PyObject*, PyObject* const* args, Py_ssize_t n) {
   }
   const Tensor out = like(*x);
   auto f32 = [&](int i) { return static_cast<const float*>(ptr(given[i])); };
-  if (abi.kb_penalize_logits(ptr(x), out.data_ptr(), ptr(given[1]), ptr(given[2]), f32(3), f32(4), f32(5), ptr(given[6]),
-                             f32(7), ptr(given[8]), B, V, x->stride(0), lengths[0], lengths[1], lengths[2], mask_stride,
-                             code(x->scalar_type()), ids64 == 1, dev.stream()))
-    Py_RETURN_NONE;
+  const int status = abi.kb_penalize_logits(
+      ptr(x), out.data_ptr(), ptr(given[1]), ptr(given[2]), f32(3), f32(4), f32(5), ptr(given[6]), f32(7),
+      ptr(given[8]), B, V, x->stride(0), lengths[0], lengths[1], lengths[2], mask_stride, code(x->scalar_type()), ids64
+      == 1, dev.stream());
+  if (failed("kb_penalize_logits", status)) return nullptr;
   return THPVariable_Wrap(out);
   END_HANDLE_TH_ERRORS
 }
 
 // ------------------------------------------------------------ module
-// init({name: address}): the C ABI's entries
+// init({name: address, ..., "check": kbb200._lib.check}): the C ABI's entries
 PyObject* init(PyObject*, PyObject* table) {
+  PyObject* check = PyDict_Check(table) ? PyDict_GetItemString(table, "check") : nullptr;
+  if (!check) {
+    PyErr_SetString(PyExc_ValueError, "kbb200._lm_host: no check");
+    return nullptr;
+  }
 #define X(name)                                                                                          \
   {                                                                                                      \
     PyObject* at = PyDict_Check(table) ? PyDict_GetItemString(table, #name) : nullptr;                   \
@@ -391,6 +413,9 @@ PyObject* init(PyObject*, PyObject* table) {
   }
   KB_HOST_ENTRIES(X)
 #undef X
+  Py_INCREF(check);
+  Py_XDECREF(abi.check);
+  abi.check = check;
   Py_RETURN_NONE;
 }
 

@@ -17,8 +17,9 @@ raises KbError.
 
 Decoding makes these calls once per layer and token, so the way of right
 arguments is native (csrc/lm_host.cpp): it checks them, allocates and calls the
-C ABI, and answers None where anything is not plainly right.  Then the checks
-here run one by one and say what is wrong, or the call is made from here.
+C ABI (whose errors it raises), and answers None where anything is not plainly
+right.  Then the checks here run one by one and say what is wrong, or the call
+is made from here.
 """
 from __future__ import annotations
 
@@ -35,7 +36,8 @@ except ImportError as e:
     raise ImportError("kbb200/_lm_host.so is missing or was built for another torch: build it with "
                       "`python kernelbench-hip_b200/build.py`") from e
 
-_host.init({name: ctypes.cast(getattr(LIB, name), ctypes.c_void_p).value for name in SIGNATURES})
+_ENTRIES = {name: ctypes.cast(getattr(LIB, name), ctypes.c_void_p).value for name in SIGNATURES}
+_host.init({**_ENTRIES, "check": check})
 
 __all__ = ["qk_norm_rope", "qk_norm_rope_backward", "rope_tables", "shared_prefix_attention", "cache_reserve",
            "cache_append", "cache_fork", "cache_free", "cache_compact", "cache_copy", "penalize_logits"]
