@@ -210,12 +210,12 @@ __device__ void fork_row(const ForkArgs& a, int i) {
 __global__ void __launch_bounds__(kColumns) fork_commit(ForkArgs a) {
   allow_next();
   wait_for_previous();
-  const int j = blockIdx.x * kColumns + threadIdx.x, first = blockIdx.y * kRowsAtOnce;
+  const int j = blockIdx.y * kColumns + threadIdx.x, first = blockIdx.x * kRowsAtOnce;  // rows in x: up to 2^16 blocks
   __shared__ int child[kRowsAtOnce];  // or -1 where nothing changes
   if (threadIdx.x < kRowsAtOnce) {
     const int i = first + threadIdx.x, len = i < a.n ? a.len[i] : -1;
     child[threadIdx.x] = len >= 0 ? a.children[i] : -1;
-    if (len >= 0 && blockIdx.x == 0) a.lens[a.children[i]] = len;
+    if (len >= 0 && blockIdx.y == 0) a.lens[a.children[i]] = len;
   }
   __syncthreads();
   if (j >= a.width) return;
@@ -527,8 +527,8 @@ int kb_cache_fork(void* pool, int32_t* table, int32_t* lens, int32_t* refs, cons
   const unsigned copies = planes && page_bytes && pages ? copy_grid(n * planes) : 0;
   if (a.whole) return copies ? launch_after(copy_kernel, dim3(copies), 256u, 0, stream, copy) : (int)KB_OK;
   if (int st = launch_after(fork_rows, dim3((unsigned)n + copies), 256u, 0, stream, a, copy)) return st;
-  return launch_after(fork_commit, dim3((unsigned)std::max<int64_t>(1, kb::ceil_div(width, kColumns)),
-                                        (unsigned)kb::ceil_div(n, kRowsAtOnce)),
+  return launch_after(fork_commit, dim3((unsigned)kb::ceil_div(n, kRowsAtOnce),
+                                        (unsigned)std::max<int64_t>(1, kb::ceil_div(width, kColumns))),
                       (unsigned)kColumns, 0, stream, a);
 }
 

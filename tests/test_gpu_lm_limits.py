@@ -1,0 +1,23 @@
+"""GPU: calls at the limits that the entries state."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tests.test_gpu_lm import ints
+
+pytestmark = pytest.mark.gpu
+
+
+def test_fork_into_the_most_slots(cuda_device):
+    """2^20 requests: every slot a copy of slot 0, which stays what it is."""
+    from kbb200 import lm
+
+    n, page = 1 << 20, 2
+    pool = torch.randn(2, 3, page, 1, 4, device=cuda_device)
+    table = torch.full((n, 1), -1, device=cuda_device, dtype=torch.int32)
+    lens, refs = torch.zeros(n, device=cuda_device, dtype=torch.int32), ints(cuda_device, [0, 1, 0])
+    table[0], lens[0], before = 1, page, pool.clone()
+    granted = lm.cache_fork(pool, table, lens, refs, torch.zeros_like(lens), torch.arange(n, device=cuda_device).int())
+    assert (granted == 1).all() and (table == 1).all() and (lens == page).all()
+    assert refs.tolist() == [0, n, 0] and torch.equal(pool, before)
