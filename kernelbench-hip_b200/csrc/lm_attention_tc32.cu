@@ -2,9 +2,10 @@
 // tensor cores, with every operand as the sum of two fp16 values.
 //
 // x 2^e = hi + lo + r, hi = fp16(x 2^e), lo = fp16(x 2^e - hi): 22 bits of x, r
-// below 2^-22 of it, where 2^e brings the tensor's largest magnitude to
-// 2^13..2^14 (an element far below the largest keeps an absolute error of 2^-38
-// of that).  Products: lo hi + hi lo + hi hi, exact in the tensor cores' fp32;
+// below 2^-22 of it, where 2^e brings the largest magnitude of a query row, or of
+// a key head's keys or values, to 2^13..2^14 (an element far below that largest
+// keeps an absolute error of 2^-38 of it).  So neither another head nor another
+// sequence's queries cost a result its bits.  Products: lo hi + hi lo + hi hi, exact in the tensor cores' fp32;
 // lo lo is below fp32's resolution.  Three fp16 products cost less than the
 // three of half the rate that TF32 halves would take, and 16-bit tiles fit
 // shared memory.  The tensor cores' accumulation truncates, so the small cross
@@ -12,8 +13,7 @@
 // fp32 additions, and S is one chain of 24 steps of which 8 are large.
 //
 // Two launches before the kernel read the part of the prefix that some query
-// sees (and the queries): the largest magnitudes, then the halves of K and V
-// into the workspace, [keys or values][hi, lo][head][key][64 or 128 columns],
+// sees: the largest magnitudes, then the halves of K and V into the workspace, [keys or values][hi, lo][head][key][64 or 128 columns],
 // padded with zeros, from which TMA loads plain tiles.  They move 12 bytes per
 // element where the products take 3 x 4 rows: they pay from a few dozen rows on.
 //
@@ -24,6 +24,8 @@
 // hi and lo, takes S_j's 128 TMEM columns; O_j has two buffers.  TMEM: S 2 x
 // 128, O 2 x 128.  Shared memory: Q, one K tile and one V tile, hi and lo, 64 KB
 // each.
+#include <float.h>
+
 #include "lm_attention.cuh"
 #include "lm_tc.cuh"
 
@@ -56,7 +58,7 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
 
 struct SplitArgs {
   AttnArgs a;
-  uint32_t* largest;  // [3]: magnitudes of q, k, v as bits
+  uint32_t* largest;  // [2][heads_kv]: magnitudes of keys and values as bits
   __half* halves;     // [2][2][heads_kv][keys][cols]
   int keys, cols;     // padded
 };
@@ -88,48 +90,36 @@ __device__ __forceinline__ uint32_t magnitude(float4 x) {
   return max(max(one(x.x), one(x.y)), max(one(x.z), one(x.w)));
 }
 
+// Grid of both: (blocks, key heads).
 __global__ void __launch_bounds__(256) largest_kernel(SplitArgs s) {
   allow_next();
   const AttnArgs& a = s.a;
-  const int seen = seen_keys(a), per_row = a.dim / 4;
-  uint32_t top[3] = {};
-  const int64_t step = (int64_t)gridDim.x * blockDim.x, first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int64_t n = (int64_t)seen * a.heads_kv * per_row;
+  const int seen = seen_keys(a), per_row = a.dim / 4, h = blockIdx.y;
+  uint32_t top[2] = {};
+  const int64_t n = (int64_t)seen * per_row;
 #pragma unroll 4
-  for (int64_t i = first; i < n; i += step) {
-    const int c = (int)(i % per_row) * 4;
-    const int64_t r = i / per_row;
-    const int h = (int)(r % a.heads_kv), j = (int)(r / a.heads_kv);
-    top[1] = max(top[1], magnitude(element4(a, false, j, h, c)));
-    top[2] = max(top[2], magnitude(element4(a, true, j, h, c)));
-  }
-  const int64_t nq = (int64_t)a.batch * a.queries * a.heads_q * per_row;
-  for (int64_t i = first; i < nq; i += step) {
-    const int c = (int)(i % per_row) * 4;
-    const int64_t r = i / per_row, bt = r / a.heads_q;
-    const float* x = static_cast<const float*>(a.q) + bt / a.queries * a.q_b + bt % a.queries * a.q_t + r % a.heads_q * a.q_h;
-    top[0] = max(top[0], magnitude(*reinterpret_cast<const float4*>(x + c)));
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
+    const int j = (int)(i / per_row), c = (int)(i - (int64_t)j * per_row) * 4;
+    top[0] = max(top[0], magnitude(element4(a, false, j, h, c)));
+    top[1] = max(top[1], magnitude(element4(a, true, j, h, c)));
   }
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    top[k] = __reduce_max_sync(0xffffffffu, top[k]);
-    if ((threadIdx.x & 31) == 0 && top[k]) atomicMax(&s.largest[k], top[k]);
+  for (int kv = 0; kv < 2; ++kv) {
+    top[kv] = __reduce_max_sync(0xffffffffu, top[kv]);
+    if ((threadIdx.x & 31) == 0 && top[kv]) atomicMax(&s.largest[kv * a.heads_kv + h], top[kv]);
   }
 }
 
 __global__ void __launch_bounds__(256) halves_kernel(SplitArgs s) {
   allow_next();
   const AttnArgs& a = s.a;
-  const int seen = seen_keys(a), per_row = s.cols / 4;
+  const int seen = seen_keys(a), per_row = s.cols / 4, h = blockIdx.y;
   wait_for_previous();
-  const float scale[2] = {power2(exponent_for(s.largest[1])), power2(exponent_for(s.largest[2]))};
-  const int64_t plane = (int64_t)a.heads_kv * s.keys * s.cols;
-  const int64_t n = (int64_t)s.keys * a.heads_kv * per_row;
+  const float scale[2] = {power2(exponent_for(s.largest[h])), power2(exponent_for(s.largest[a.heads_kv + h]))};
+  const int64_t plane = (int64_t)a.heads_kv * s.keys * s.cols, n = (int64_t)s.keys * per_row;
 #pragma unroll 2
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-    const int c = (int)(i % per_row) * 4;
-    const int64_t r = i / per_row;
-    const int h = (int)(r % a.heads_kv), j = (int)(r / a.heads_kv);
+    const int j = (int)(i / per_row), c = (int)(i - (int64_t)j * per_row) * 4;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
       uint2 hi = make_uint2(0, 0), lo = make_uint2(0, 0);
@@ -161,7 +151,7 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t *s_q = smem, *s_k = smem + 2 * kTileBytes, *s_v = smem + 4 * kTileBytes;  // hi, then lo
   float* s_keep = reinterpret_cast<float*>(smem + 6 * kTileBytes);                  // [4][rows]
-  float* s_sum = s_keep + 4 * kTile;                                                // [rows] sums, [rows] unused
+  float* s_sum = s_keep + 4 * kTile;  // [2][rows]: first the largest magnitudes of a query's halves, at the end its sum
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_sum + 2 * kTile);
   auto bar = [&](int i) { return smem_u32(bars + i); };
   const uint32_t q_full = bar(0), k_full = bar(1), k_empty = bar(2), v_full = bar(3), v_empty = bar(4);
@@ -215,26 +205,39 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
   const uint32_t tmem = *tmem_slot;
   const int end = min(w.k1, *s_end);
   const int n = end > w.k0 ? (end - w.k0 + kTile - 1) / kTile : 0;
-  const int eq = exponent_for(sp.largest[0]), ek = exponent_for(sp.largest[1]), ev = exponent_for(sp.largest[2]);
+  const int ek = exponent_for(sp.largest[w.h]), ev = exponent_for(sp.largest[a.heads_kv + w.h]);
+  int eq = 0;  // of this thread's row
   const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
   auto s_col = [&](int j) { return tmem + (j & 1) * kTile; };
   auto o_col = [&](int j) { return tmem + 2 * kTile + (j & 1) * kTile; };
 
   if (warp < 8 && n > 0) {
     // ---------------- the queries' halves: warps 0-3 the first half of a row's columns, warps 4-7 the second
-    const float scale = a.scale_log2 < 0.0f ? -power2(eq) : power2(eq);
     const float* src = static_cast<const float*>(query_of(a, w, row < w.rows ? row : 0, 4));
     const int side = warp >> 2;
+    float4 x[HALVES * 4][2];  // eight columns each
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = side * HALVES * 4; i < (side + 1) * HALVES * 4; ++i) {  // eight columns each
-      uint4 hi = make_uint4(0, 0, 0, 0), lo = hi;
-      float4 x = make_float4(0, 0, 0, 0), y = x;
-      if (row < w.rows && i * 8 < a.dim) x = *reinterpret_cast<const float4*>(src + i * 8);
-      if (row < w.rows && i * 8 + 4 < a.dim) y = *reinterpret_cast<const float4*>(src + i * 8 + 4);
-      split2(x.x * scale, x.y * scale, hi.x, lo.x);
-      split2(x.z * scale, x.w * scale, hi.y, lo.y);
-      split2(y.x * scale, y.y * scale, hi.z, lo.z);
-      split2(y.z * scale, y.w * scale, hi.w, lo.w);
+    for (int i = 0; i < HALVES * 4; ++i) {
+      const int c = (side * HALVES * 4 + i) * 8;
+      x[i][0] = x[i][1] = make_float4(0, 0, 0, 0);
+      if (row < w.rows && c < a.dim) x[i][0] = *reinterpret_cast<const float4*>(src + c);
+      if (row < w.rows && c + 4 < a.dim) x[i][1] = *reinterpret_cast<const float4*>(src + c + 4);
+      top = max(top, max(magnitude(x[i][0]), magnitude(x[i][1])));
+    }
+    uint32_t* s_top = reinterpret_cast<uint32_t*>(s_sum);
+    s_top[side * kTile + row] = top;
+    asm volatile("bar.sync 1, 256;" ::: "memory");  // warps 0-7
+    eq = exponent_for(max(top, s_top[(side ^ 1) * kTile + row]));
+    const float scale = a.scale_log2 < 0.0f ? -power2(eq) : power2(eq);
+#pragma unroll
+    for (int k = 0; k < HALVES * 4; ++k) {
+      const int i = side * HALVES * 4 + k;
+      uint4 hi, lo;
+      split2(x[k][0].x * scale, x[k][0].y * scale, hi.x, lo.x);
+      split2(x[k][0].z * scale, x[k][0].w * scale, hi.y, lo.y);
+      split2(x[k][1].x * scale, x[k][1].y * scale, hi.z, lo.z);
+      split2(x[k][1].z * scale, x[k][1].w * scale, hi.w, lo.w);
       uint8_t* dst = s_q + (i >> 3) * kHalfBytes + row * 128 + (((i & 7) ^ (row & 7)) << 4);
       *reinterpret_cast<uint4*>(dst) = hi;
       *reinterpret_cast<uint4*>(dst + kTileBytes) = lo;
@@ -318,7 +321,8 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
     }
   } else if (warp < 4) {
     // ---------------- softmax
-    const float c = score_factor(a.scale_log2 * power2(min(max(-eq - ek, -126), 126)));
+    // powers of two, one after the other: their product may lie outside fp32, and infinity x 0 would be a NaN
+    const float c = fminf(score_factor(a.scale_log2 * power2(-eq) * power2(-ek)), FLT_MAX);
     for (int j = 0; j < n; ++j) {
       ok = warp_wait(s_full(j), (j >> 1) & 1, abort_flag);
       if (!ok) break;
@@ -368,7 +372,7 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
       tc_fence_before();
       mbar_arrive(p_full(j));
     }
-    s_sum[row] = l;
+    s_sum[row] = l;  // the magnitudes there were read before the first S
   } else {
     // ---------------- the sum of O
 #pragma unroll
@@ -460,12 +464,14 @@ int launch_as(const SplitArgs& s, cudaStream_t stream) {
     KB_CUDA(cudaFuncSetAttribute(attn_prefix32_kernel<HALVES>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes));
     if (dev < 64) attr_set |= 1ull << dev;
   }
-  KB_CUDA(cudaMemsetAsync(s.largest, 0, 16, stream));
-  const unsigned blocks = (unsigned)std::min<int64_t>(ceil_div((int64_t)s.keys * s.a.heads_kv * s.cols / 4, 256),
-                                                      (int64_t)sm_count() * 8);
+  KB_CUDA(cudaMemsetAsync(s.largest, 0, 2 * s.a.heads_kv * sizeof(uint32_t), stream));
+  const int64_t heads = s.a.heads_kv;
+  const dim3 blocks((unsigned)std::min<int64_t>(ceil_div((int64_t)s.keys * s.cols / 4, 256),
+                                                std::max<int64_t>(1, sm_count() * 8 / heads)),
+                    (unsigned)heads);
   largest_kernel<<<blocks, 256, 0, stream>>>(s);
   if (int st = check_launch("kb_shared_prefix_attention")) return st;
-  if (int st = launch_after(halves_kernel, dim3(blocks), 256u, 0, stream, s)) return st;
+  if (int st = launch_after(halves_kernel, blocks, 256u, 0, stream, s)) return st;
   return launch_after(attn_prefix32_kernel<HALVES>, dim3((unsigned)s.a.prefix_items), (unsigned)kThreads, kSmemBytes,
                       stream, tm, s);
 }
@@ -477,13 +483,15 @@ int launch_as(const SplitArgs& s, cudaStream_t stream) {
 // against 87 at 2.1e9, 162 against 267 at 8.6e9, 245 against 494 at 17e9 and 952
 // against 3394 at 131e9 (calls with short continuations).
 bool tc32_pays(int64_t rows, int64_t heads_kv, int64_t dim, int64_t keys) {
-  return dim <= kTile && rows > 64 && keys > 0 && 4.0 * rows * heads_kv * dim * keys >= 1.2e9;
+  return dim <= kTile && heads_kv <= 65535 && rows > 64 && keys > 0 && 4.0 * rows * heads_kv * dim * keys >= 1.2e9;
 }
+static size_t largest_bytes(int64_t heads_kv) { return (size_t)ceil_div(2 * heads_kv, 4) * 16; }
 size_t tc32_bytes(int64_t heads_kv, int64_t dim, int64_t keys) {
-  return 16 + (size_t)4 * heads_kv * padded_keys(keys) * (dim > 64 ? 128 : 64) * sizeof(__half);
+  return largest_bytes(heads_kv) + (size_t)4 * heads_kv * padded_keys(keys) * (dim > 64 ? 128 : 64) * sizeof(__half);
 }
 int tc32_launch(const AttnArgs& a, void* scratch, cudaStream_t stream) {
-  SplitArgs s{a, static_cast<uint32_t*>(scratch), reinterpret_cast<__half*>(static_cast<char*>(scratch) + 16),
+  SplitArgs s{a, static_cast<uint32_t*>(scratch),
+              reinterpret_cast<__half*>(static_cast<char*>(scratch) + largest_bytes(a.heads_kv)),
               (int)padded_keys((int64_t)a.prefix_pages * a.page_size), a.dim > 64 ? 128 : 64};
   return a.dim > 64 ? launch_as<2>(s, stream) : launch_as<1>(s, stream);
 }
