@@ -28,6 +28,12 @@ constexpr float kShift = std::is_same_v<T, __half> ? 7.0f : 0.0f;
 // scale of zero), since -inf x 0 would be a NaN.
 __device__ __forceinline__ float score_factor(float c) { return c == 0.0f ? 0x1p-126f : fabsf(c); }
 
+// exp2(s c - m) as one multiply-add keeps the product exact but not m = s' c of
+// the reference s', and the difference, half a unit in m's last place, is the
+// same factor for all of a row's weights.  Where m is so large that this factor
+// could leave fp32 or fp16 (from 2^25 on), weights are exp2((s - s') c) instead.
+constexpr float kFar = 0x1p20f;
+
 struct AttnArgs {
   const void *q, *k, *v;
   void* out;

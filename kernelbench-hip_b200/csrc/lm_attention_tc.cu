@@ -250,7 +250,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       fence_proxy_async();
       mbar_arrive(q_full + 8 * t);
     }
-    float m = -INFINITY, l = 0.0f;  // the reference, in units of log2, and the sum
+    float ref = -INFINITY, m = -INFINITY, l = 0.0f;  // the reference, as a score and in units of log2, and the sum
     bool ok = true;
     for (int j = 0; j < n; ++j) {
       ok = warp_wait(s_full(t), j & 1, abort_flag);
@@ -276,12 +276,13 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         for (int k = 0; k < 4; ++k) top[k] = max3(top[k], f(i + k), f(i + k + 4));
 #pragma unroll
       for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], f(kTile - 4 + k));
-      const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;
+      const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), now = best * c;
       // move the reference where the maximum has outgrown it
       const bool move = now > m + kSlack;  // also from -inf; not for a NaN
       if (__any_sync(0xffffffffu, move)) {
-        const float keep = move ? ex2(m - now) : 1.0f;
-        if (move) m = now;
+        const float by = fmaxf(fabsf(m), fabsf(now)) < kFar ? m - now : (ref - best) * c;  // also from -inf
+        const float keep = move ? ex2(by) : 1.0f;
+        if (move) ref = best, m = now;
         l *= keep;
         if (j > 0) {
           ok = warp_wait(o_full(t), (j - 1) & 1, abort_flag);
@@ -299,8 +300,15 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
           tmem_st_wait();
         }
       }
-      const float base = (m == -INFINITY ? 0.0f : m) - kShift<T>;
-      const uint64_t cc = pair(c, c), bb = pair(-base, -base);
+      const bool far = fabsf(m) >= kFar && m != -INFINITY;
+      if (__any_sync(0xffffffffu, far)) {
+        if (far) {
+#pragma unroll
+          for (int i = 0; i < kTile; ++i) x[i] = __float_as_uint((f(i) - ref) * c);
+        }
+      }
+      const float by = far ? 1.0f : c, base = (far || m == -INFINITY ? 0.0f : m) - kShift<T>;
+      const uint64_t cc = pair(by, by), bb = pair(-base, -base);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {

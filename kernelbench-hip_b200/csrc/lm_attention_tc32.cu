@@ -246,7 +246,7 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
     mbar_arrive(q_full);
   }
 
-  float m = -INFINITY, l = 0.0f;          // warps 0-3
+  float m = -INFINITY, l = 0.0f;          // warps 0-3: the maximum in units of log2, and the sum
   float acc[HALVES * 64];                 // warps 4-7
   bool ok = true;
   if (warp == kLoadWarp) {
@@ -323,6 +323,7 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
     // ---------------- softmax
     // powers of two, one after the other: their product may lie outside fp32, and infinity x 0 would be a NaN
     const float c = fminf(score_factor(a.scale_log2 * power2(-eq) * power2(-ek)), FLT_MAX);
+    float ref = -INFINITY;  // the maximum as a score
     for (int j = 0; j < n; ++j) {
       ok = warp_wait(s_full(j), (j >> 1) & 1, abort_flag);
       if (!ok) break;
@@ -347,11 +348,18 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
         for (int k = 0; k < 4; ++k) top[k] = max3(top[k], f(i + k), f(i + k + 4));
 #pragma unroll
       for (int k = 0; k < 4; ++k) top[k] = fmaxf(top[k], f(kTile - 4 + k));
-      const float now = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c);
-      const float keep = ex2(m - (now == -INFINITY ? 0.0f : now));
-      m = now;
+      const float best = fmaxf(ref, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]))), now = best * c;
+      const bool none = now == -INFINITY, far = fabsf(now) >= kFar && !none;
+      const float keep = ex2(far ? (ref - best) * c : m - (none ? 0.0f : now));
+      ref = best, m = now;
       s_keep[(j & 3) * kTile + row] = keep;
-      const float base = (m == -INFINITY ? 0.0f : m) - kShift32;
+      if (__any_sync(0xffffffffu, far)) {
+        if (far) {
+#pragma unroll
+          for (int i = 0; i < kTile; ++i) x[i] = __float_as_uint((f(i) - ref) * c);
+        }
+      }
+      const float by = far ? 1.0f : c, base = (far || none ? 0.0f : m) - kShift32;
       float sum[2] = {};
       // 32 keys at a time: hi over the first 64 columns of S, lo over the others (all of S is in registers)
 #pragma unroll
@@ -359,7 +367,7 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
         uint32_t hi[16], lo[16];
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
-          const float p0 = ex2(fmaf(f(i + k), c, -base)), p1 = ex2(fmaf(f(i + k + 1), c, -base));
+          const float p0 = ex2(fmaf(f(i + k), by, -base)), p1 = ex2(fmaf(f(i + k + 1), by, -base));
           sum[0] += p0;
           sum[1] += p1;
           split2(p0, p1, hi[k >> 1], lo[k >> 1]);

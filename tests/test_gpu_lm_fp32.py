@@ -54,6 +54,15 @@ def test_heads_of_different_magnitudes(shape, cuda_device):
     check_rows((q, k, v, prefix, table, lens))
 
 
+@pytest.mark.parametrize("shape", SHAPES)
+def test_queries_of_different_magnitudes(shape, cuda_device):
+    """One sequence's queries 2^30 times the others', whose scores are ordinary."""
+    q, k, v, prefix, table, lens = attention_inputs(cuda_device, torch.float32, *shape, seed=22)
+    q[3] *= 2.0 ** 30
+    q[4] *= 2.0 ** -20
+    check_rows((q, k, v, prefix, table, lens))
+
+
 @pytest.mark.parametrize("garbage", [1e30, float("inf"), float("nan")])
 @pytest.mark.parametrize("shape", SHAPES)
 def test_ended_slots_hold_anything(shape, garbage, cuda_device):
