@@ -416,9 +416,9 @@ KB_API int kb_qk_norm_rope_backward(const void* dq_out, const void* dk_out, cons
  * Query head h reads key head h / (heads_q / heads_kv).
  * out[batch, queries, heads_q, dim] = softmax(scale q k) v and
  * lse[batch, queries, heads_q] (fp32) = log sum exp; a query that sees no key
- * gets 0 and -inf.  Slots that no query of a sequence sees are not read;
- * where some of its queries see a key that others do not, its values must be
- * finite.  dim <= 256, dim * element size, pointers and strides multiples of
+ * gets 0 and -inf.  Slots that no query of a sequence sees are not read, and
+ * infinite or NaN keys and values reach the queries that see them only.
+ * dim <= 256, dim * element size, pointers and strides multiples of
  * 16 bytes.                                                                */
 KB_API size_t kb_shared_prefix_attention_workspace_size(int64_t batch, int64_t queries,
                                                         int64_t heads_q, int64_t heads_kv,

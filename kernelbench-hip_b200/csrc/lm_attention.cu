@@ -25,8 +25,9 @@
 // 700 of their own 233 us (own keys 72, at 5.1 TB/s).
 //
 // Keys at or past what a row tile sees are not read (they count as zeros), so
-// what stands in unused slots of a page does not matter.  Page ids out of
-// range are clamped into the pool.
+// what stands in unused slots of a page does not matter; infinite and NaN values
+// reach the rows that see their keys only.  Page ids out of range are clamped
+// into the pool.
 #include <type_traits>
 
 #include "lm_attention.cuh"
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(RowsCfg<T, DP, NK>::kThreads) attn_rows_kernel
   T* sq = reinterpret_cast<T*>(raw);
   T* sk = sq + C::kRows * LD;
   T* sv = sk + 2 * NK * LD;
-  __shared__ int s_max[C::kWarps];
+  __shared__ int s_max[C::kWarps], s_least[C::kWarps], s_replaced;
   begin(a);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Item w = item_at(a, a.first_item + blockIdx.x, C::kRows);
@@ -312,21 +313,25 @@ __global__ void __launch_bounds__(RowsCfg<T, DP, NK>::kThreads) attn_rows_kernel
   // this thread's two rows
   const int row[2] = {warp * 16 + (lane >> 2), warp * 16 + (lane >> 2) + 8};
   int vis[2];
-  int top = 0, low = 0x7fffffff;
+  int top = 0, low = 0x7fffffff, least = 0x7fffffff;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     vis[r] = row[r] < w.rows ? visible(a, w.base + (w.row0 + row[r]) / a.group) : 0;
     top = max(top, vis[r]);
     if (row[r] < w.rows) low = min(low, vis[r]);
+    if (vis[r] > w.k0) least = min(least, vis[r]);
   }
   top = __reduce_max_sync(0xffffffffu, top);
   low = __reduce_min_sync(0xffffffffu, low);
-  if (lane == 0) s_max[warp] = top;
+  least = __reduce_min_sync(0xffffffffu, least);
+  if (lane == 0) s_max[warp] = top, s_least[warp] = least;
+  if (tid == 0) s_replaced = kNoKey;
   __syncthreads();
   int end = 0;
 #pragma unroll
-  for (int i = 0; i < C::kWarps; ++i) end = max(end, s_max[i]);
+  for (int i = 0; i < C::kWarps; ++i) end = max(end, s_max[i]), least = min(least, s_least[i]);
   end = min(end, w.k1);
+  const int uneven = least < end ? uneven_from(w, least, NK) : kNoKey;
 
   const T* kp = static_cast<const T*>(a.k) + w.h * a.k_h;
   const T* vp = static_cast<const T*>(a.v) + w.h * a.v_h;
@@ -361,8 +366,8 @@ __global__ void __launch_bounds__(RowsCfg<T, DP, NK>::kThreads) attn_rows_kernel
     for (int i = 0; i < 4; ++i) o[d][i] = 0.0f;
   Running st{{-INFINITY, -INFINITY}, {0.0f, 0.0f}};
   if (w.k0 < end) load(w.k0, 0);
-  int buf = 0;
-  for (int key0 = w.k0; key0 < end; key0 += NK, buf ^= 1) {
+  int buf = 0, key0 = w.k0;
+  auto step = [&](auto look) {  // look: at values that not all rows see
     if (key0 + NK < end) {
       load(key0 + NK, buf ^ 1);
       cp_async_wait<1>();
@@ -370,13 +375,20 @@ __global__ void __launch_bounds__(RowsCfg<T, DP, NK>::kThreads) attn_rows_kernel
       cp_async_wait<0>();
     }
     __syncthreads();
+    if constexpr (look) {
+      if (replace_nonfinite_rows<T, NK, kPerRow, LD, C::kThreads>(smem_addr(sv + buf * NK * LD), tid)) s_replaced = uneven;
+      __syncthreads();
+    }
     float s[NK / 8][4];
     scores<T, DP, NK, LD>(s, sq + warp * 16 * LD, sk + buf * NK * LD, lane);
     const int seen[2] = {min(vis[0], end), min(vis[1], end)};
     softmax_step<T, NK, DP / 8>(s, o, st, a.scale_log2, key0, seen, key0 + NK > min(low, end), lane);
     weigh<T, DP, NK, LD>(o, s, sv + buf * NK * LD, lane);
     __syncthreads();
-  }
+  };
+  // two loops, so that the first has nothing to ask
+  for (; key0 < min(end, uneven); key0 += NK, buf ^= 1) step(std::false_type{});
+  for (; key0 < end; key0 += NK, buf ^= 1) step(std::true_type{});
   cp_async_wait<0>();  // the queries' copies, where there was no key
 
 #pragma unroll
@@ -411,6 +423,13 @@ __global__ void __launch_bounds__(RowsCfg<T, DP, NK>::kThreads) attn_rows_kernel
       }
     }
   }
+  if (s_replaced != kNoKey) {
+    const Item again = item_again(a, a.first_item, C::kRows);
+    for (int i = 0; i < 2 * (DP / 8); ++i) {
+      const int c = (i >> 1) * 8 + (threadIdx.x & 3) * 2;
+      write_nonfinite<T>(a, again, (threadIdx.x >> 5) * 16 + ((threadIdx.x & 31) >> 2) + (i & 1) * 8, s_replaced, c, c + 2);
+    }
+  }
   wait_for_previous();  // as in the keys kernel
 }
 
@@ -425,6 +444,8 @@ __global__ void __launch_bounds__(RowsCfg<T, DP, NK>::kThreads) attn_rows_kernel
 // against 47 us; against four (64 columns): 60 against 89 us for 100 sequences
 // of 8 queries in fp32, 26 against 32 us for 64 of one query in fp16; blocks of
 // 8 against 16 (fp32, 16 sequences of up to 1024 keys): 27 against 37 us.
+// EVEN: the launch has only items whose rows all see the same keys (the own keys of
+// one query a sequence); what the others look at cost these 4 to 7 %.
 template <typename T, int DP, int NK, int STAGES>
 struct KeysCfg {
   static constexpr int kRows = 16, kWarps = 4, kThreads = 128;
@@ -436,7 +457,7 @@ struct KeysCfg {
   static_assert(kSmem + 1024 <= kMaxSmem, "no block holds this");
 };
 
-template <typename T, int DP, int NK, int STAGES>
+template <typename T, int DP, int NK, int STAGES, bool EVEN>
 __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
   using C = KeysCfg<T, DP, NK, STAGES>;
   constexpr int LD = C::LD, kVec = 16 / sizeof(T), kPerRow = DP / kVec;
@@ -444,7 +465,9 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
   T* sq = reinterpret_cast<T*>(raw);
   T* ring = sq + C::kRows * LD;
   __shared__ float s_m[4][16], s_l[4][16];
+  __shared__ int s_replaced;
   begin(a);
+  if (!EVEN && threadIdx.x == 0) s_replaced = kNoKey;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const Item w = item_at(a, a.first_item + blockIdx.x, C::kRows);
   const int64_t n_rows = (int64_t)a.batch * a.queries * a.heads_q;
@@ -483,15 +506,18 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
 #pragma unroll
   for (int i = 0; i < STAGES; ++i) first[i] = place(begin + i * kStep);
   const int row[2] = {lane >> 2, (lane >> 2) + 8};
-  int vis[2], top = 0, low = 0x7fffffff;
+  int vis[2], top = 0, low = 0x7fffffff, least = 0x7fffffff;
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
     vis[r] = row[r] < w.rows ? visible(a, w.base + (w.row0 + row[r]) / a.group) : 0;
     top = max(top, vis[r]);
     if (row[r] < w.rows) low = min(low, vis[r]);
+    if (vis[r] > w.k0) least = min(least, vis[r]);
   }
   const int end = min(w.k1, __reduce_max_sync(0xffffffffu, top));
   low = __reduce_min_sync(0xffffffffu, low);
+  least = __reduce_min_sync(0xffffffffu, least);
+  const int uneven = !EVEN && least < end ? uneven_from(w, least, NK) : kNoKey;
 
   auto load = [&](int key0, const Place& p, int stage) {
     T* sk = mine + stage * C::kStage;
@@ -540,8 +566,8 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
     cp_async_wait<0>();
     queries_there();
   }
-  int stage = 0;
-  for (int key0 = begin; key0 < end; key0 += kStep) {
+  int stage = 0, key0 = begin;
+  auto step = [&](auto look) {  // look: at values that not all rows see
     const int ahead = key0 + (STAGES - 1) * kStep;
     if (ahead < end) load(ahead, next, stage == 0 ? STAGES - 1 : stage - 1);
     cp_async_commit();
@@ -550,13 +576,21 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
     if (key0 == begin) queries_there();
     __syncwarp();
     const T* sk = mine + stage * C::kStage;
+    if constexpr (look) {
+      if (replace_nonfinite_rows<T, NK, kPerRow, LD, 32>(smem_addr(sk + NK * LD), lane)) s_replaced = uneven;
+      __syncwarp();
+    }
     float s[NK / 8][4];
     scores<T, DP, NK, LD>(s, sq, sk, lane);
     softmax_step<T, NK, DP / 8>(s, o, st, a.scale_log2, key0, seen, key0 + NK > min(low, end), lane);
     weigh<T, DP, NK, LD>(o, s, sk + NK * LD, lane);
     __syncwarp();  // all lanes are done with the stage that the next load fills
     stage = stage == STAGES - 1 ? 0 : stage + 1;
-  }
+  };
+  // two loops, so that the first has nothing to ask
+  for (; key0 < min(end, uneven); key0 += kStep) step(std::false_type{});
+  if constexpr (!EVEN)
+    for (; key0 < end; key0 += kStep) step(std::true_type{});
   cp_async_wait<0>();
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
@@ -612,6 +646,11 @@ __global__ void __launch_bounds__(128) attn_keys_kernel(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) z[i] = from_f32<T>(y[i] * inv);
     }
+  }
+  if (!EVEN && s_replaced != kNoKey) {
+    const Item again = item_again(a, a.first_item, C::kRows);
+    for (int d = (threadIdx.x & 7) * 4; d < a.dim; d += 32)
+      write_nonfinite<T>(a, again, threadIdx.x >> 3, s_replaced, d, d + 4);
   }
 }
 
@@ -761,11 +800,16 @@ int launch_rows(const AttnArgs& a, int64_t first, int64_t items, cudaStream_t st
   using C = RowsCfg<T, DP, NK>;
   return launch(attn_rows_kernel<T, DP, NK>, C::kThreads, C::kSmem, a, first, items, attr_set, stream);
 }
+template <typename T, int DP, int NK, int STAGES, bool EVEN>
+int launch_keys_as(const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {
+  static uint64_t attr_set = 0;
+  return launch(attn_keys_kernel<T, DP, NK, STAGES, EVEN>, 128, KeysCfg<T, DP, NK, STAGES>::kSmem, a, first, items,
+                attr_set, stream);
+}
 template <typename T, int DP, int NK, int STAGES>
 int launch_keys(const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {
-  static uint64_t attr_set = 0;
-  return launch(attn_keys_kernel<T, DP, NK, STAGES>, 128, KeysCfg<T, DP, NK, STAGES>::kSmem, a, first, items,
-                attr_set, stream);
+  return first >= a.prefix_items && a.queries == 1 ? launch_keys_as<T, DP, NK, STAGES, true>(a, first, items, stream)
+                                                   : launch_keys_as<T, DP, NK, STAGES, false>(a, first, items, stream);
 }
 template <typename T>
 int launch_kind(Kind kind, const AttnArgs& a, int64_t first, int64_t items, cudaStream_t stream) {

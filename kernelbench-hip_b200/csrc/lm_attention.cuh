@@ -102,6 +102,91 @@ __device__ __forceinline__ const void* query_of(const AttnArgs& a, const Item& w
           (int64_t)(w.h * a.group + rr % a.group) * a.q_h) * element_size;
 }
 
+// Infinite and NaN values.  In a product of a tile of weights with a tile of
+// values a masked key has weight 0, and 0 x NaN is NaN: such a value would reach
+// rows that do not see its key.  So in a tile of which some rows see more than
+// others the values that are not finite are replaced by 0 in shared memory, and
+// at the end, if there were any, their keys are gone through once more: where a
+// row sees one, that is its sum (weights are positive).
+// `least`: the fewest keys seen by a row that sees any of the item's.  The first
+// tile of `keys` keys, from w.k0 on, that needs this:
+__device__ __forceinline__ int uneven_from(const Item& w, int least, int keys) {
+  return w.k0 + (least - w.k0) / keys * keys;
+}
+// Whether a 32-bit word of T holds something that is not finite: an exponent of
+// ones, to which one more carries into the sign's place.
+template <typename T>
+__device__ __forceinline__ bool has_nonfinite(uint32_t x) {
+  constexpr uint32_t kOne = std::is_same_v<T, float> ? 0x00800000u : std::is_same_v<T, __half> ? 0x04000400u : 0x00800080u;
+  constexpr uint32_t kSign = std::is_same_v<T, float> ? 0x80000000u : 0x80008000u;
+  return (((x & (kSign - kOne)) + kOne) & kSign) != 0;
+}
+__device__ __forceinline__ uint4 load_shared(uint32_t p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+  return v;
+}
+// Replaces what is not finite among the 16 bytes at p; whether there was any.
+template <typename T>
+__device__ __forceinline__ bool replace_nonfinite(uint32_t p, uint4 v) {
+  if (!(has_nonfinite<T>(v.x) | has_nonfinite<T>(v.y) | has_nonfinite<T>(v.z) | has_nonfinite<T>(v.w))) return false;
+  union {
+    uint4 v;
+    T t[16 / sizeof(T)];
+  } u;
+  u.v = v;
+#pragma unroll
+  for (int i = 0; i < (int)(16 / sizeof(T)); ++i)
+    if (!isfinite(to_f32(u.t[i]))) u.t[i] = from_f32<T>(0.0f);
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(u.v.x), "r"(u.v.y), "r"(u.v.z), "r"(u.v.w) : "memory");
+  return true;
+}
+// The same for every STEP-th vector, from the `first` on, of ROWS rows of PER
+// vectors, LD elements apart.
+template <typename T, int ROWS, int PER, int LD, int STEP>
+__device__ __forceinline__ bool replace_nonfinite_rows(uint32_t p, int first) {
+  bool any = false;
+#pragma unroll 4
+  for (int i = first; i < ROWS * PER; i += STEP) {
+    const uint32_t at = p + (i / PER * LD) * (int)sizeof(T) + i % PER * 16;
+    any |= replace_nonfinite<T>(at, load_shared(at));
+  }
+  return any;
+}
+// The item of a launch's block, worked out again: what of it is needed at the end
+// only, and hardly ever, takes no registers on the way there.
+__device__ __forceinline__ Item item_again(const AttnArgs& a, int64_t first_item, int tile_rows) {
+  int block = blockIdx.x;
+  asm volatile("" : "+r"(block));
+  return item_at(a, first_item + block, tile_rows);
+}
+constexpr int kNoKey = 0x7fffffff;  // first key whose values were replaced, where there is none
+// Columns first to last - 1 of the item's row r, which this thread or one before a
+// __syncwarp has written: the values that are not finite of keys `from` to its last.
+template <typename T>
+__device__ __forceinline__ void write_nonfinite(const AttnArgs& a, const Item& w, int r, int from, int first, int last) {
+  if (r >= w.rows) return;
+  const int64_t at = row_index(a, w, r), n_rows = (int64_t)a.batch * a.queries * a.heads_q;
+  const int end = min(w.k1, visible(a, w.base + (w.row0 + r) / a.group));
+#pragma unroll 1
+  for (int c = first; c < min(last, a.dim); ++c) {
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int j = from; j < end; ++j) {
+      const int pj = j / a.page_size;
+      const int64_t page = min(max(w.pages[pj], 0), a.pages - 1);
+      const T* v = static_cast<const T*>(a.v) + page * a.v_p + (int64_t)(j - pj * a.page_size) * a.v_s + w.h * a.v_h;
+      const float x = to_f32(v[c]);
+      if (!isfinite(x)) sum += x;
+    }
+    if (isfinite(sum)) continue;
+    if (a.part_o)
+      a.part_o[((int64_t)w.split * n_rows + at) * a.dim + c] = sum;
+    else
+      static_cast<T*>(a.out)[at * a.dim + c] = from_f32<T>(sum);
+  }
+}
+
 // ------------------------------------------------------------------ tensor-core prefix (lm_attention_tc.cu)
 // Whether it can take the prefix (16-bit types, head and page sizes, strides).
 bool tc_fits(const AttnArgs& a, int dtype);

@@ -17,7 +17,8 @@
 //
 // Roles (10 warps): warps 0-3 and 4-7 are the softmax of the two row tiles,
 // warp 8 loads K and V tiles by TMA, one copy per page and 64 columns (the
-// page table is the gather), warp 9 issues the products in the order
+// page table is the gather), and looks at those values that not all rows see
+// (infinities and NaN among them: lm_attention.cuh), warp 9 issues the products in the order
 //   O_0 += P_0 V_j, S_0 = Q_0 K_j+1, O_1 += P_1 V_j, S_1 = Q_1 K_j+1
 // so that one row tile's products run during the other's softmax; O += P V
 // begins with the first 64 keys while the others' exponentials are computed.
@@ -58,10 +59,11 @@ constexpr int kThreads = 320;
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
 constexpr int kSmemBytes = (2 + 2 * kStages) * kTileBytes + 256 + 1024;  // + barriers, alignment
 constexpr float kSlack = 8.0f;                  // log2 of how far a maximum may pass the reference
+
 template <typename T, int HALVES>
 __global__ void __launch_bounds__(kThreads, 1)
-attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, AttnArgs a,
-                   int row_tiles) {
+attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v,
+                   const __grid_constant__ AttnArgs a, int row_tiles) {
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_q = smem;
@@ -77,9 +79,13 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   auto s_full = [&](int t) { return bar(10 + t); };
   auto p_full = [&](int t, int half) { return bar(12 + 2 * t + half); };
   auto o_full = [&](int t) { return bar(16 + t); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 18);
+  const uint32_t v_landed = bar(18);  // a copy of values that are looked at before v_full
+  const uint32_t written = bar(19);   // the rows
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_end = reinterpret_cast<int*>(tmem_slot + 2);
+  int* s_least = s_end + 1;
+  __shared__ int s_replaced;
   // first of all, so that no CTA holds TMEM while a launch before it has to take its own
   wait_for_previous();
 
@@ -100,8 +106,12 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       mbar_init(v_full(s), 1);
       mbar_init(v_empty(s), 1);
     }
+    mbar_init(v_landed, 1);
+    mbar_init(written, row_tiles * kTile);
     *abort_flag = 0;
     *s_end = 0;
+    *s_least = 0x7fffffff;
+    s_replaced = kNoKey;
     fence_barrier_init();
   }
   if (warp == kMmaWarp) {
@@ -116,15 +126,19 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
   int vis = 0;
   if (warp < 4 * row_tiles) {
     if (r < w.rows) vis = visible(a, w.base + (w.row0 + r) / a.group);
-    const int top = __reduce_max_sync(0xffffffffu, vis);
-    if (lane == 0) atomicMax(s_end, top);
+    const int top = __reduce_max_sync(0xffffffffu, vis), low = __reduce_min_sync(0xffffffffu, vis > w.k0 ? vis : 0x7fffffff);
+    if (lane == 0) atomicMax(s_end, top), atomicMin(s_least, low);
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int end = min(w.k1, *s_end);
+  const int end = min(w.k1, *s_end), least = *s_least;
   const int n = end > w.k0 ? (end - w.k0 + kTile - 1) / kTile : 0;
+  // The first tile with values that warp 8 looks at before they are used: some that only some rows see, or that none
+  // does, in a page that is partly seen (they become zeros, for 0 x NaN).
+  const int part_of_page = end < w.k0 + n * kTile && end % a.page_size != 0 ? n - 1 : n;
+  const int look_from = min(part_of_page, least < end ? (uneven_from(w, least, kTile) - w.k0) / kTile : n);
   constexpr int halves = HALVES;  // of 64 columns; columns past dim are zeros
   const uint32_t o_col = row_tiles == 2 ? 256 : 128;
 
@@ -144,7 +158,8 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
       }
       const uint32_t parity = ((j / kStages) & 1) ^ 1;
       for (int kv = 0; kv < 2 && alive; ++kv) {
-        const uint32_t full = kv ? v_full(s) : k_full(s);
+        const bool look = kv && j >= look_from;
+        const uint32_t full = look ? v_landed : kv ? v_full(s) : k_full(s);
         if (!warp_wait(kv ? v_empty(s) : k_empty(s), parity, abort_flag)) {
           alive = false;
           break;
@@ -157,16 +172,29 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
             tma_load(dst + h * kHalfBytes, kv ? &tm_v : &tm_k, full, h * 64, w.h, slot, page);
         }
         ++issued;
+        if (!look) continue;
+        alive = warp_wait(v_landed, (j - look_from) & 1, abort_flag);
+        if (!alive) {
+          drain(v_landed, (j - look_from) & 1);
+          break;
+        }
+        bool any = false;
+        for (int row = lane; row < kTile; row += 32)
+          any |= replace_value_row<T, HALVES>(smem_u32(s_v) + s * kTileBytes + row * 128, key0 + row >= end);
+        if (any) s_replaced = w.k0 + look_from * kTile;
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_full(s));
       }
     }
     // every issued copy must land before the CTA may exit
     if (lane == 0)
       for (int i = max(issued - 2 * kStages, 0); i < issued; ++i) {
         const int j = i / 2, s = j % kStages;
-        const uint64_t t0 = globaltimer();
-        while (!mbar_try_wait(i & 1 ? v_full(s) : k_full(s), (j / kStages) & 1))
-          if (globaltimer() - t0 > kWaitLimitNs) break;
+        if (i % 2 == 0 || j < look_from) drain(i & 1 ? v_full(s) : k_full(s), (j / kStages) & 1);
       }
+    if (alive && s_replaced != kNoKey && warp_wait(written, 0, abort_flag))
+      for (int i = lane; i < w.rows; i += 32) write_nonfinite_row<T>(a, w, i, s_replaced);
   } else if (warp == kMmaWarp) {
     // ---------------- products
     if (lane == 0 && n > 0) {
@@ -323,20 +351,9 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         }
         tmem_st(s_addr + half * 32, x + half * 32);
         tmem_st_wait();
-        // V rows that nobody sees, in a page that is partly seen: zeros, for 0 x NaN
-        if (half == 0 && j == n - 1 && t == 0 && end < w.k0 + n * kTile && end % a.page_size != 0) {
-          ok = warp_wait(v_full(j % kStages), (j / kStages) & 1, abort_flag);
-          if (!ok) break;
-          if (w.k0 + j * kTile + row >= end)
-            for (int i = 0; i < halves * 8; ++i)
-              *reinterpret_cast<uint4*>(s_v + (j % kStages) * kTileBytes + (i >> 3) * kHalfBytes + row * 128 +
-                                        ((i & 7) << 4)) = make_uint4(0, 0, 0, 0);
-          fence_proxy_async();
-        }
         tc_fence_before();
         mbar_arrive(p_full(t, half));
       }
-      if (!ok) break;
       float l0, l1;
       unpair(add2(sum[0], sum[1]), l0, l1);
       l += l0 + l1;
@@ -387,6 +404,7 @@ attn_prefix_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_consta
         __syncwarp();
       }
     }
+    mbar_arrive(written);
   }
   tc_fence_before();
   __syncthreads();

@@ -19,7 +19,8 @@
 //
 // A CTA takes 128 query rows of one key head and a range of keys, in tiles of
 // 128.  Roles (10 warps): warps 0-3 softmax (one thread per row), warps 4-7 the
-// sum of O (one thread per row, in registers), warp 8 TMA, warp 9 products.
+// sum of O (one thread per row, in registers), warp 8 TMA (and a look at values
+// that not all rows see), warp 9 products.
 // S_{j+1} is issued before O_j = P_j V_j, into the other of two S buffers; P_j,
 // hi and lo, takes S_j's 128 TMEM columns; O_j has two buffers.  TMEM: S 2 x
 // 128, O 2 x 128.  Shared memory: Q, one K tile and one V tile, hi and lo, 64 KB
@@ -145,7 +146,7 @@ __device__ __forceinline__ void tma_load3(uint32_t dst, const CUtensorMap* tm, u
 
 template <int HALVES>
 __global__ void __launch_bounds__(kThreads, 1)
-attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
+attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, const __grid_constant__ SplitArgs sp) {
   const AttnArgs& a = sp.a;
   extern __shared__ uint8_t raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -162,9 +163,13 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
   auto p_full = [&](int j) { return bar(7 + (j & 3)); };
   auto o_full = [&](int j) { return bar(11 + (j & 1)); };
   auto o_empty = [&](int j) { return bar(13 + (j & 1)); };
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  const uint32_t v_landed = bar(15);  // a copy of values that are looked at before v_full
+  const uint32_t written = bar(16);   // the rows
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 17);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_end = reinterpret_cast<int*>(tmem_slot + 2);
+  int* s_least = s_end + 1;
+  __shared__ int s_replaced;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Item w = item_at(a, blockIdx.x, kTile);
@@ -174,6 +179,8 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
     mbar_init(k_empty, 1);
     mbar_init(v_full, 1);
     mbar_init(v_empty, 1);
+    mbar_init(v_landed, 1);
+    mbar_init(written, kTile);
     for (int j = 0; j < 2; ++j) {
       mbar_init(s_full(j), 1);
       mbar_init(p_full(j), kTile);
@@ -183,6 +190,8 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
     }
     *abort_flag = 0;
     *s_end = 0;
+    *s_least = 0x7fffffff;
+    s_replaced = kNoKey;
     fence_barrier_init();
   }
   if (warp == kMmaWarp) {
@@ -195,16 +204,19 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
   int vis = 0;
   if (warp < 4) {
     if (row < w.rows) vis = visible(a, w.base + (w.row0 + row) / a.group);
-    const int top = __reduce_max_sync(0xffffffffu, vis);
-    if (lane == 0) atomicMax(s_end, top);
+    const int top = __reduce_max_sync(0xffffffffu, vis), low = __reduce_min_sync(0xffffffffu, vis > w.k0 ? vis : 0x7fffffff);
+    if (lane == 0) atomicMax(s_end, top), atomicMin(s_least, low);
   }
   wait_for_previous();  // the halves and the magnitudes
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int end = min(w.k1, *s_end);
+  const int end = min(w.k1, *s_end), least = *s_least;
   const int n = end > w.k0 ? (end - w.k0 + kTile - 1) / kTile : 0;
+  // The first tile with values that not all rows of this CTA see, some, or only rows of others (they are in the halves,
+  // too): warp 8 looks at them before they are used.
+  const int look_from = max(least - w.k0, 0) / kTile;
   const int ek = exponent_for(sp.largest[w.h]), ev = exponent_for(sp.largest[a.heads_kv + w.h]);
   int eq = 0;  // of this thread's row
   const uint32_t lanes = (uint32_t)(warp & 3) * 32 << 16;
@@ -251,28 +263,42 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
   bool ok = true;
   if (warp == kLoadWarp) {
     // ---------------- K and V tiles, hi and lo
-    if (lane == 0) {
-      bool alive = true;
-      int issued = 0;
-      for (int j = 0; j < n && alive; ++j)
-        for (int kv = 0; kv < 2 && alive; ++kv) {
-          alive = mbar_wait(kv ? v_empty : k_empty, (j & 1) ^ 1, abort_flag);
-          if (!alive) break;
-          const uint32_t full = kv ? v_full : k_full;
+    bool alive = true;
+    int issued = 0;
+    for (int j = 0; j < n && alive; ++j) {
+      for (int kv = 0; kv < 2 && alive; ++kv) {
+        alive = warp_wait(kv ? v_empty : k_empty, (j & 1) ^ 1, abort_flag);
+        if (!alive) break;
+        const bool look = kv && j >= look_from;
+        const uint32_t full = look ? v_landed : kv ? v_full : k_full;
+        if (lane == 0) {
           mbar_expect_tx(full, 2 * HALVES * kHalfBytes);
           for (int part = 0; part < 2; ++part)
             for (int h = 0; h < HALVES; ++h)
               tma_load3(smem_u32(kv ? s_v : s_k) + part * kTileBytes + h * kHalfBytes, &tm, full, h * 64, w.k0 + j * kTile,
                         (2 * kv + part) * a.heads_kv + w.h);
-          ++issued;
         }
-      // every issued copy must land before the CTA may exit
-      for (int i = max(issued - 2, 0); i < issued; ++i) {
-        const uint64_t t0 = globaltimer();
-        while (!mbar_try_wait(i & 1 ? v_full : k_full, (i >> 1) & 1))
-          if (globaltimer() - t0 > kWaitLimitNs) break;
+        __syncwarp();
+        ++issued;
+        if (!look) continue;
+        alive = warp_wait(v_landed, (j - look_from) & 1, abort_flag);
+        if (!alive) {
+          drain(v_landed, (j - look_from) & 1);
+          break;
+        }
+        bool any = false;
+        for (int r = lane; r < kTile; r += 32)
+          any |= replace_value_row<__half, HALVES>(smem_u32(s_v) + r * 128, false);  // lo is 0 where hi is not finite
+        if (any) s_replaced = w.k0 + look_from * kTile;
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(v_full);
       }
     }
+    // every issued copy must land before the CTA may exit
+    if (lane == 0)
+      for (int i = max(issued - 2, 0); i < issued; ++i)
+        if (i % 2 == 0 || i / 2 < look_from) drain(i & 1 ? v_full : k_full, (i >> 1) & 1);
   } else if (warp == kMmaWarp) {
     // ---------------- products
     if (lane == 0 && n > 0) {
@@ -410,7 +436,7 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
       const float lse = none ? -INFINITY : ((m == -INFINITY ? 0.0f : m) - kShift32) * kLn2 + logf(l);
       (a.part_o ? a.part_lse[at * a.splits + w.split] : a.lse[at]) = lse;
     }
-  } else if (warp < 8 && ok) {
+  } else if (warp < 8) {
     // out through shared memory (the queries' room), 32 columns at a time, in whole pieces of rows
     const float sum = s_sum[row];
     const bool none = sum == 0.0f || n == 0;
@@ -421,7 +447,7 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
     const int row0 = (warp & 3) * 32;
 #pragma unroll
     for (int i = 0; i < HALVES * 64; i += 32) {
-      if (i >= a.dim) break;
+      if (i >= a.dim || !ok) break;
 #pragma unroll
       for (int k = 0; k < 32; k += 4) {
         float z[4];
@@ -441,6 +467,9 @@ attn_prefix32_kernel(const __grid_constant__ CUtensorMap tm, SplitArgs sp) {
       }
       __syncwarp();
     }
+    mbar_arrive(written);
+  } else if (warp == kLoadWarp && s_replaced != kNoKey && warp_wait(written, 0, abort_flag)) {
+    for (int r = lane; r < w.rows; r += 32) write_nonfinite_row<float>(a, w, r, s_replaced);
   }
   tc_fence_before();
   __syncthreads();

@@ -7,7 +7,7 @@
 
 #include <type_traits>
 
-#include "lm_common.cuh"
+#include "lm_attention.cuh"
 
 namespace kb {
 namespace lm {
@@ -73,6 +73,12 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // All lanes of the warp leave together.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+// Waits for a copy that has been issued, after an abort, too, but not past the limit.
+__device__ __noinline__ void drain(uint32_t bar, uint32_t parity) {
+  const uint64_t t0 = globaltimer();
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer() - t0 > kWaitLimitNs) break;
 }
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, uint32_t bar, int col, int head, int slot,
                                          int page) {
@@ -194,6 +200,28 @@ __device__ __forceinline__ float max3(float x, float y, float z) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
   return r;
+}
+
+// A row of a tile of values: zeros, or what is finite of it; whether anything was not.
+template <typename T, int HALVES>
+__device__ __noinline__ bool replace_value_row(uint32_t row, bool zeros) {
+  bool any = false;
+#pragma unroll 4
+  for (int i = 0; i < HALVES * 8; ++i) {
+    const uint32_t at = row + (i >> 3) * kHalfBytes + ((i & 7) << 4);
+    if (zeros)
+      asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at), "r"(0) : "memory");
+    else
+      any |= replace_nonfinite<T>(at, load_shared(at));
+  }
+  return any;
+}
+
+// Out of line, and called by a warp that holds little: at the end of the softmax warps
+// it cost their loops registers (256 rows x 8 heads over 32768 keys: 162 against 156 us).
+template <typename T>
+__device__ __noinline__ void write_nonfinite_row(const AttnArgs& a, const Item& w, int r, int from) {
+  write_nonfinite<T>(a, w, r, from, 0, a.dim);
 }
 
 // ------------------------------------------------------------------ host side
