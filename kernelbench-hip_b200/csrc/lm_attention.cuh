@@ -88,7 +88,7 @@ __device__ __forceinline__ Item item_at(const AttnArgs& a, int64_t id, int tile_
 }
 __device__ __forceinline__ int visible(const AttnArgs& a, int bt) {
   const int b = bt / a.queries, t = bt - b * a.queries;
-  return a.lens[b] - a.queries + t + 1;
+  return max(a.lens[b], 0) - a.queries + t + 1;  // the least number stays below zero
 }
 // Row r of the item in the tensors' order [batch, queries, heads_q].
 __device__ __forceinline__ int64_t row_index(const AttnArgs& a, const Item& w, int r) {

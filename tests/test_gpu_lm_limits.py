@@ -21,3 +21,19 @@ def test_fork_into_the_most_slots(cuda_device):
     granted = lm.cache_fork(pool, table, lens, refs, torch.zeros_like(lens), torch.arange(n, device=cuda_device).int())
     assert (granted == 1).all() and (table == 1).all() and (lens == page).all()
     assert refs.tolist() == [0, n, 0] and torch.equal(pool, before)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("batch,n_pre", [(3, 5), (200, 70)])
+def test_attention_of_the_least_length(batch, n_pre, dt, cuda_device):
+    """A length of -2^31, as a sentinel or left over, is a slot without keys."""
+    from kbb200 import lm
+    from tests.test_gpu_lm import attention_inputs
+
+    args = q, k, v, prefix, table, lens = attention_inputs(cuda_device, dt, batch, 4, 4, 1, 128, 16, n_pre, 40, seed=2)
+    lens[1] = 0
+    want, want_lse = lm.shared_prefix_attention(*args)
+    lens[1] = -2 ** 31
+    out, lse = lm.shared_prefix_attention(*args)
+    assert (out[1] == 0).all() and (lse[1] == -float("inf")).all()
+    assert torch.equal(out, want) and torch.equal(lse, want_lse)
