@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
   const int c = a.seqs[i];
   // A refused slot has not grown: its last places are older keys, which other slots may share.
   if (c < 0 || c >= a.slots || (a.granted && !a.granted[i])) return;
-  const int pos = a.lens[c] - a.tokens + t;
+  const int pos = max(a.lens[c], 0) - a.tokens + t;  // the least number stays below zero
   if (pos < 0 || pos / a.page_size >= a.width) return;
   const int p = a.table[(int64_t)c * a.width + pos / a.page_size];
   if (p < 0 || p >= a.pages) return;

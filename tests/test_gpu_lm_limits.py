@@ -37,3 +37,14 @@ def test_attention_of_the_least_length(batch, n_pre, dt, cuda_device):
     out, lse = lm.shared_prefix_attention(*args)
     assert (out[1] == 0).all() and (lse[1] == -float("inf")).all()
     assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+def test_append_to_the_least_length(cuda_device):
+    from kbb200 import lm
+
+    width, page = 1 << 20, 1 << 12  # a row of 2^32 places
+    pool = torch.zeros(2, 2, page, 1, 4, device=cuda_device)
+    table = torch.zeros(1, width, device=cuda_device, dtype=torch.int32)
+    k = torch.ones(1, 3, 1, 4, device=cuda_device)
+    lm.cache_append(k, k, pool[0], pool[1], table, ints(cuda_device, [-2 ** 31]), ints(cuda_device, [0]))
+    assert (pool == 0).all()
