@@ -776,6 +776,14 @@ Plan plan(int64_t batch, int64_t queries, int64_t heads_q, int64_t heads_kv, int
   return {plan_part(heads_kv, batch * rows, prefix_keys, dim, dtype, tensor),
           plan_part(heads_kv * batch, rows, own_keys, dim, dtype, false)};
 }
+// At most 2^30 rows, and keys of a sequence.  One by one before their products, which
+// have to fit 64 bits.
+bool sizes_fit(int64_t batch, int64_t queries, int64_t heads_q, int64_t prefix_pages, int64_t width, int64_t page_size) {
+  constexpr int64_t kMost = 0x3fffffff;
+  return batch <= kMost && queries <= kMost && batch * queries <= kMost && heads_q <= kMost &&
+         batch * queries * heads_q <= kMost && prefix_pages <= kMost && width <= kMost && page_size <= kMost &&
+         std::max(prefix_pages, width) * page_size <= kMost;
+}
 // Parts, then (fp32 on the tensor cores) the prefix in halves.
 size_t part_bytes(const Plan& p, int64_t rows, int64_t dim) {
   return p.splits() <= 1 ? 0 : (size_t)ceil_div(p.splits() * rows * (dim + 1), 4) * 16;
@@ -836,7 +844,7 @@ size_t kb_shared_prefix_attention_workspace_size(int64_t batch, int64_t queries,
                                                  int64_t page_size, int dtype) {
   using namespace kb::lm::attn;
   if (batch <= 0 || queries <= 0 || heads_q <= 0 || heads_kv <= 0 || dim <= 0 || page_size <= 0 || prefix_pages < 0 ||
-      heads_q % heads_kv)
+      heads_q % heads_kv || !sizes_fit(batch, queries, heads_q, prefix_pages, width, page_size))
     return 0;
   const int64_t keys = prefix_pages * page_size;
   auto bytes = [&](bool tensor) {
@@ -867,8 +875,10 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
                  width >= 0 && pages >= 0 && page_size >= 1,
              KB_ERR_INVALID_ARG, "%s: negative size", name);
   KB_REQUIRE(dtype_size(dtype), KB_ERR_INVALID_ARG, "%s: unknown element type", name);
+  if (batch == 0 || queries == 0 || heads_q == 0 || dim == 0) return KB_OK;
+  KB_REQUIRE(sizes_fit(batch, queries, heads_q, prefix_pages, width, page_size), KB_ERR_UNSUPPORTED,
+             "%s: too many rows or keys", name);
   const int64_t rows = batch * queries * heads_q;
-  if (rows == 0 || dim == 0) return KB_OK;
   KB_REQUIRE(heads_kv >= 1 && heads_q % heads_kv == 0, KB_ERR_INVALID_ARG,
              "%s: %lld query heads do not divide into %lld key heads", name, (long long)heads_q, (long long)heads_kv);
   KB_REQUIRE(q && lens && out && lse, KB_ERR_INVALID_ARG, "%s: null pointer", name);
@@ -885,8 +895,7 @@ int kb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
                  whole(k_stride_slot) && whole(k_stride_head) && whole(v_stride_page) && whole(v_stride_slot) &&
                  whole(v_stride_head),
              KB_ERR_UNSUPPORTED, "%s: queries, pools and their strides must be multiples of 16 bytes", name);
-  KB_REQUIRE(rows <= 0x3fffffff && (prefix_pages + own_pages) * page_size <= 0x3fffffff && pages <= 0x7fffffff,
-             KB_ERR_UNSUPPORTED, "%s: too many rows or keys", name);
+  KB_REQUIRE(pages <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many pages", name);
   AttnArgs a{};
   a.q = q, a.k = k_pages, a.v = v_pages, a.out = out, a.lse = lse;
   a.prefix = prefix, a.table = table, a.lens = lens;

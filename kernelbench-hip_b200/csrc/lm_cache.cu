@@ -38,6 +38,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kMaxPages = 1 << 20, kMaxSlots = 1 << 20;
+constexpr int64_t kMaxKeys = 0x3fffffff;  // of a row: a page more is still a number of 32 bits
 constexpr int kSharedSlots = 4096;  // slots whose owners shared memory holds
 constexpr int kWholeRows = 2048;    // table entries that the fork's planning CTA writes itself
 
@@ -505,7 +506,8 @@ int kb_cache_fork(void* pool, int32_t* table, int32_t* lens, int32_t* refs, cons
   using namespace kb::lm;
   KB_CACHE_COMMON(n);
   KB_REQUIRE(planes >= 0 && page_bytes >= 0 && page_size >= 1, KB_ERR_INVALID_ARG, "%s: bad page", name);
-  KB_REQUIRE(page_size * width <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: rows of more than 2^31 keys", name);
+  KB_REQUIRE(page_size <= kMaxKeys && page_size * width <= kMaxKeys && planes <= 0x7fffffff, KB_ERR_UNSUPPORTED,
+             "%s: too many keys or planes", name);
   if (n == 0) return KB_OK;
   KB_REQUIRE(parents && children && granted && (!slots || (lens && (!width || table))) && (!pages || refs),
              KB_ERR_INVALID_ARG, "%s: null pointer", name);
@@ -546,7 +548,8 @@ int kb_cache_reserve(int32_t* table, int32_t* lens, int32_t* refs, const int32_t
   using namespace kb::lm;
   KB_CACHE_COMMON(n);
   KB_REQUIRE(tokens >= 0 && page_size >= 1, KB_ERR_INVALID_ARG, "%s: bad page or token count", name);
-  KB_REQUIRE(page_size * width <= 0x3fffffff && tokens <= 0x3fffffff, KB_ERR_UNSUPPORTED, "%s: too many keys", name);
+  KB_REQUIRE(page_size <= kMaxKeys && page_size * width <= kMaxKeys && tokens <= kMaxKeys, KB_ERR_UNSUPPORTED,
+             "%s: too many keys", name);
   if (n == 0) return KB_OK;
   KB_REQUIRE(seqs && granted && (!slots || (lens && (!width || table))) && (!pages || refs), KB_ERR_INVALID_ARG,
              "%s: null pointer", name);
@@ -565,9 +568,10 @@ int kb_cache_append_granted(const void* k, const void* v, void* k_pages, void* v
   const char* name = "kb_cache_append";
   using namespace kb::lm;
   KB_CACHE_COMMON(n);
-  KB_REQUIRE(tokens >= 0 && page_size >= 1 && key_bytes >= 0 && page_bytes >= page_size * key_bytes,
+  KB_REQUIRE(tokens >= 0 && page_size >= 1 && key_bytes >= 0 && page_bytes / page_size >= key_bytes,
              KB_ERR_INVALID_ARG, "%s: bad page or token count", name);
-  KB_REQUIRE(page_size <= 0x7fffffff && n * tokens <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many tokens", name);
+  KB_REQUIRE(page_size <= 0x7fffffff && tokens <= 0x7fffffff && n * tokens <= 0x7fffffff, KB_ERR_UNSUPPORTED,
+             "%s: too many tokens", name);
   if (n == 0 || tokens == 0 || key_bytes == 0 || slots == 0 || width == 0 || pages == 0) return KB_OK;
   KB_REQUIRE(k && v && k_pages && v_pages && table && lens && seqs, KB_ERR_INVALID_ARG, "%s: null pointer", name);
   AppendArgs a{static_cast<const char*>(k), static_cast<const char*>(v), static_cast<char*>(k_pages),
@@ -608,6 +612,7 @@ int kb_cache_compact(void* pool, int32_t* table, int32_t* refs, int32_t* live, i
   using namespace kb::lm;
   KB_CACHE_COMMON(0);
   KB_REQUIRE(planes >= 0 && page_bytes >= 0, KB_ERR_INVALID_ARG, "%s: negative size", name);
+  KB_REQUIRE(planes <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many planes", name);
   KB_REQUIRE(live && (!pages || refs) && (!slots || !width || table), KB_ERR_INVALID_ARG, "%s: null pointer", name);
   KB_REQUIRE(pool || !planes || !pages || !page_bytes, KB_ERR_INVALID_ARG, "%s: null pool", name);
   KB_CACHE_WORKSPACE(kb_cache_compact_workspace_size(pages));
@@ -633,7 +638,7 @@ int kb_cache_copy(const void* src_pool, const int32_t* src, void* dst_pool, cons
   using namespace kb::lm;
   KB_REQUIRE(n >= 0 && planes >= 0 && page_bytes >= 0 && src_pages >= 0 && dst_pages >= 0, KB_ERR_INVALID_ARG,
              "%s: negative size", name);
-  KB_REQUIRE(n <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many pages", name);
+  KB_REQUIRE(n <= 0x7fffffff && planes <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: too many pages or planes", name);
   if (n == 0 || planes == 0 || page_bytes == 0 || src_pages == 0 || dst_pages == 0) return KB_OK;
   KB_REQUIRE(src_pool && dst_pool && src && dst, KB_ERR_INVALID_ARG, "%s: null pointer", name);
   const CopyArgs copy{static_cast<const char*>(src_pool), static_cast<char*>(dst_pool), src, dst, nullptr, (int)n,

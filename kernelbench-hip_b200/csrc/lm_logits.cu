@@ -49,6 +49,7 @@ constexpr int kMaxTable = 16384;          // slots: 128 KB of keys and words
 constexpr int64_t kLargeBytes = 8 << 20;  // logits from which two launches pay
 constexpr int kCountBits = 20, kBiasShift = 21;   // count | prompt bit | bias index + 1
 constexpr uint32_t kCountMask = (1u << kCountBits) - 1, kPromptBit = 1u << kCountBits;
+constexpr int64_t kMaxPrompt = 1ll << 40;  // sums and places of ids fit 64 bits
 constexpr int64_t kMaxOutput = kCountMask, kMaxBias = (1 << (32 - kBiasShift)) - 1;
 
 struct LogitsArgs {
@@ -338,6 +339,7 @@ int kb_penalize_logits(const void* logits, void* out, const void* prompt, const 
   KB_REQUIRE(output_len <= kMaxOutput, KB_ERR_UNSUPPORTED, "%s: output history longer than %lld", name,
              (long long)kMaxOutput);
   KB_REQUIRE(bias_len <= kMaxBias, KB_ERR_UNSUPPORTED, "%s: more than %lld biases a row", name, (long long)kMaxBias);
+  KB_REQUIRE(prompt_len <= kMaxPrompt, KB_ERR_UNSUPPORTED, "%s: prompt history too long", name);
   KB_REQUIRE(rows <= 65535, KB_ERR_UNSUPPORTED, "%s: more than 65535 rows", name);
   KB_REQUIRE(vocab <= 0x7fffffff, KB_ERR_UNSUPPORTED, "%s: vocabulary too large", name);
   LogitsArgs a{logits, out, prompt, output, bias_ids, repetition, presence, frequency, bias_values,

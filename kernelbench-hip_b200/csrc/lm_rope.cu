@@ -649,7 +649,10 @@ int check_shape(const char* name, int64_t tokens, int64_t heads_q, int64_t heads
              kMaxDim);
   KB_REQUIRE(rotary >= 0 && rotary <= dim && rotary % 2 == 0, KB_ERR_INVALID_ARG,
              "%s: rotary size %lld must be even and at most %lld", name, (long long)rotary, (long long)dim);
-  KB_REQUIRE(heads_q + heads_kv <= 65535, KB_ERR_UNSUPPORTED, "%s: too many heads", name);
+  // one by one before their sums and products, which have to fit 64 bits
+  KB_REQUIRE(heads_q <= 65535 && heads_kv <= 65535 && heads_q + heads_kv <= 65535, KB_ERR_UNSUPPORTED,
+             "%s: too many heads", name);
+  KB_REQUIRE(tokens <= kMaxUnits, KB_ERR_UNSUPPORTED, "%s: too many tokens", name);
   return KB_OK;
 }
 
