@@ -4,8 +4,8 @@ Each csrc/*.cu is compiled by nvcc into _build/*.o in parallel, then linked
 into kbb200/libkbb200.so with the CUDA runtime linked statically, so the
 library needs only the driver at run time.  csrc/lm_host.cpp, the host side
 of kbb200.lm's calls, becomes the Python module kbb200/_lm_host.so, against the
-installed torch.  Rebuilds only what changed (object older than its source or
-any header).
+installed torch; without torch it is left out, and the library is built all the
+same.  Rebuilds only what changed (object older than its source or any header).
 
     python kernelbench-hip_b200/build.py [--clean] [-j N] [--verbose]
 """
@@ -13,10 +13,12 @@ from __future__ import annotations
 
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
@@ -61,10 +63,11 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 
 def _build_host_module(verbose: bool) -> None:
-    import importlib.util
-    import sysconfig
-
-    torch = Path(importlib.util.find_spec("torch").origin).parent  # not imported: only its headers and libraries
+    spec = importlib.util.find_spec("torch")
+    if spec is None or spec.origin is None:
+        print("torch is not installed: kbb200/_lm_host.so, which kbb200.lm needs, is not built", file=sys.stderr)
+        return
+    torch = Path(spec.origin).parent  # not imported: only its headers and libraries
     newest = max(f.stat().st_mtime for f in (HOST_SRC, INCLUDE / "kbb200.h", torch / "version.py"))
     if HOST_MODULE.exists() and HOST_MODULE.stat().st_mtime >= newest and not verbose:
         return
@@ -97,7 +100,6 @@ def build(jobs: int | None = None, clean: bool = False, verbose: bool = False) -
     with cf.ThreadPoolExecutor(max_workers=jobs + 1) as ex:
         host = ex.submit(_build_host_module, verbose)
         list(ex.map(lambda s: _compile(s, verbose), stale))
-        host.result()
     objs = [BUILD / (s.stem + ".o") for s in sources]
     if stale or not LIB.exists() or LIB.stat().st_mtime < max(o.stat().st_mtime for o in objs):
         tmp = LIB.with_suffix(".so.tmp")
@@ -106,6 +108,7 @@ def build(jobs: int | None = None, clean: bool = False, verbose: bool = False) -
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
         os.replace(tmp, LIB)
+    host.result()  # raises what went wrong there, after the library
     return LIB
 
 
