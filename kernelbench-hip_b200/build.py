@@ -5,7 +5,8 @@ into kbb200/libkbb200.so with the CUDA runtime linked statically, so the
 library needs only the driver at run time.  csrc/lm_host.cpp, the host side
 of kbb200.lm's calls, becomes the Python module kbb200/_lm_host.so, against the
 installed torch; without torch it is left out, and the library is built all the
-same.  Rebuilds only what changed (object older than its source or any header).
+same.  Rebuilds only what changed (object older than its source or any header,
+module built for another Python or torch).
 
     python kernelbench-hip_b200/build.py [--clean] [-j N] [--verbose]
 """
@@ -29,6 +30,7 @@ INCLUDE = REPO / "include"
 LIB = PKG_ROOT / "kbb200" / "libkbb200.so"
 HOST_SRC = CSRC / "lm_host.cpp"
 HOST_MODULE = PKG_ROOT / "kbb200" / "_lm_host.so"
+HOST_FOR = BUILD / "lm_host.for"  # which Python and torch it was built for
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH + [
@@ -68,8 +70,10 @@ def _build_host_module(verbose: bool) -> None:
         print("torch is not installed: kbb200/_lm_host.so, which kbb200.lm needs, is not built", file=sys.stderr)
         return
     torch = Path(spec.origin).parent  # not imported: only its headers and libraries
-    newest = max(f.stat().st_mtime for f in (HOST_SRC, INCLUDE / "kbb200.h", torch / "version.py"))
-    if HOST_MODULE.exists() and HOST_MODULE.stat().st_mtime >= newest and not verbose:
+    made_for = f"{sysconfig.get_config_var('SOABI')}\n{torch}\n{(torch / 'version.py').read_text()}"
+    newest = max(HOST_SRC.stat().st_mtime, (INCLUDE / "kbb200.h").stat().st_mtime)
+    if (HOST_MODULE.exists() and HOST_MODULE.stat().st_mtime >= newest and not verbose
+            and HOST_FOR.exists() and HOST_FOR.read_text() == made_for):
         return
     cuda = Path(nvcc()).resolve().parent.parent
     tmp = HOST_MODULE.with_suffix(".so.tmp")
@@ -81,6 +85,7 @@ def _build_host_module(verbose: bool) -> None:
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed on {HOST_SRC.name}:\n{r.stdout}\n{r.stderr}")
     os.replace(tmp, HOST_MODULE)
+    HOST_FOR.write_text(made_for)
 
 
 def build(jobs: int | None = None, clean: bool = False, verbose: bool = False) -> Path:

@@ -1,4 +1,4 @@
-"""CPU: the library is built with or without torch."""
+"""CPU: the library is built with or without torch, and the host module again for another Python or torch."""
 from __future__ import annotations
 
 import importlib.util
@@ -17,7 +17,7 @@ def kb_build(tmp_path, monkeypatch):
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
     mod.BUILD, mod.LIB = tmp_path / "build", tmp_path / "libkbb200.so"
-    mod.HOST_MODULE = tmp_path / "_lm_host.so"
+    mod.HOST_MODULE, mod.HOST_FOR = tmp_path / "_lm_host.so", tmp_path / "build" / "lm_host.for"
     mod.ran = []
 
     def run(cmd, **_):
@@ -52,3 +52,26 @@ def test_library_before_a_host_module_that_fails(kb_build, monkeypatch):
     with pytest.raises(RuntimeError, match="no such header"):
         kb_build.build()
     assert kb_build.LIB.exists()
+
+
+def test_host_module_for_another_torch(kb_build, tmp_path, monkeypatch):
+    pytest.importorskip("torch")
+    kb_build.build()
+    assert kb_build.ran.count("g++") == 1
+    kb_build.build()
+    assert kb_build.ran.count("g++") == 1  # up to date
+    # an older installation of another version, as files come out of an archive
+    other = tmp_path / "site" / "torch"
+    other.mkdir(parents=True)
+    (other / "__init__.py").touch()
+    (other / "version.py").write_text("__version__ = '1.0'\n")
+    spec = importlib.util.spec_from_file_location("torch", other / "__init__.py")
+    real = importlib.util.find_spec
+    with monkeypatch.context() as m:
+        m.setattr(importlib.util, "find_spec", lambda name, *a: spec if name == "torch" else real(name, *a))
+        kb_build.build()
+        assert kb_build.ran.count("g++") == 2
+        kb_build.build()
+        assert kb_build.ran.count("g++") == 2
+    kb_build.build()
+    assert kb_build.ran.count("g++") == 3
