@@ -87,6 +87,8 @@ def _out(name: str, t: torch.Tensor | None, like: torch.Tensor, shape, dtype=Non
 def rope_tables(length: int, rotary: int, base: float = 10000.0, device="cuda"):
     """The cos and sin tables [length, rotary / 2] of angles p * base^(-2 i / rotary), computed in fp64 and
     rounded to fp32 once; a program makes them once and keeps them."""
+    if rotary < 0 or rotary % 2:
+        raise RuntimeError(f"rope_tables: rotary must be even (whole pairs), got {rotary}")
     f = base ** (-torch.arange(0, rotary, 2, device=device, dtype=torch.float64) / max(rotary, 1))
     a = torch.arange(length, device=device, dtype=torch.float64)[:, None] * f
     return a.cos().float().contiguous(), a.sin().float().contiguous()
