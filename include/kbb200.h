@@ -449,7 +449,10 @@ KB_API int kb_shared_prefix_attention(const void* q, const void* k_pages, const 
  * leaves its slot as it was: slots out of range, a slot listed again, no
  * room in the row, or more pages asked for, up to and including this
  * request, than are free.  At most 2^20 pages, slots, entries of a row and
- * requests.
+ * requests.  A program may lower lens itself, to drop the newest keys of a
+ * slot (drafts that were rejected), though not into pages that other slots
+ * share: the pages past it stay in the row, where the slot's next reserve
+ * uses them first and free gives them back.
  *   reserve  lens += tokens, with the pages that takes
  *   append   k, v [n, tokens, key_bytes] (strides in BYTES) into the last
  *            `tokens` places of slots seqs, of one layer's two planes.  A slot

@@ -5,7 +5,9 @@
 // layer), a table [slots, width] of page ids (-1: none), the number of keys
 // lens[slots], and refs[pages], the number of table entries that hold each
 // page (0: free).  A slot holds ceil(lens / page_size) pages from the start
-// of its row; a page that is not full belongs to one slot alone.
+// of its row, and more where its program has lowered lens (drafts that were
+// rejected): they stay in the row until its next reserve uses them or it is
+// freed.  A page that is not full belongs to one slot alone.
 //
 //   reserve  grows slots by `tokens` keys, taking pages
 //   append   writes keys and values at a slot's last `tokens` places, where
@@ -312,7 +314,10 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(ReserveArgs a) {
   const int mine = threadIdx.x;
   const int first = mine < a.pages ? a.refs[mine] : 1;
   const int seq0 = mine < a.n ? a.seqs[mine] : -1;
-  const int len0 = seq0 >= 0 && seq0 < a.slots ? a.lens[seq0] : 0;
+  const int len0 = seq0 >= 0 && seq0 < a.slots ? a.lens[seq0] : -1;
+  // the entry past the slot's pages, on its way while the free pages are looked for
+  const bool inside = len0 >= 0 && len0 < a.width * a.page_size;
+  const int next0 = inside ? a.table[(int64_t)seq0 * a.width + (len0 + a.page_size - 1) / a.page_size % a.width] : -1;
   for (int i = mine; i < a.slots; i += kPlanThreads) owner[i] = a.n;
   __syncthreads();
   for (int i = mine; i < a.n; i += kPlanThreads) {
@@ -324,7 +329,7 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(ReserveArgs a) {
   int asked = 0;
   for (int base = 0; base < a.n; base += kPlanThreads) {
     const int i = base + mine;
-    int need = 0, ok = 0, held = 0, len = 0, c = -1;
+    int need = 0, kept = 0, ok = 0, held = 0, len = 0, c = -1;
     if (i < a.n) {
       c = base ? a.seqs[i] : seq0;
       ok = c >= 0 && c < a.slots && owner[c] == i;
@@ -336,6 +341,12 @@ __global__ void __launch_bounds__(kPlanThreads) reserve_kernel(ReserveArgs a) {
         held = (len + a.page_size - 1) / a.page_size;
         // capped past the pool, so that sums over a block stay in 32 bits
         need = min((len + a.tokens + a.page_size - 1) / a.page_size - held, a.pages + 1);
+        // pages that the row still holds from before lens was lowered
+        const int* row = a.table + (int64_t)c * a.width + held;
+        if (base || next0 >= 0)
+          while (kept < need && row[kept] >= 0 && row[kept] < a.pages) ++kept;
+        held += kept;
+        need -= kept;
       }
     }
     int total;
@@ -395,19 +406,15 @@ __global__ void __launch_bounds__(128) append_kernel(AppendArgs a) {
 
 // ------------------------------------------------------------------ free
 __global__ void free_kernel(int* table, int* lens, int* refs, const int* seqs, int slots, int width, int pages) {
-  __shared__ int len;
   allow_next();
   wait_for_previous();
   const int c = seqs[blockIdx.x];
   if (c < 0 || c >= slots) return;
-  if (threadIdx.x == 0) len = atomicExch(&lens[c], 0);  // a slot that is listed twice is emptied once
-  __syncthreads();
-  if (len <= 0) return;
+  if (threadIdx.x == 0) lens[c] = 0;
   int* row = table + (int64_t)c * width;
   for (int j = threadIdx.x; j < width; j += blockDim.x) {
-    const int p = row[j];
+    const int p = atomicExch(&row[j], -1);  // a slot that is listed twice gives its pages back once
     if (p >= 0 && p < pages) atomicSub(&refs[p], 1);
-    row[j] = -1;
   }
 }
 

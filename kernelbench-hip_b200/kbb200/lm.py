@@ -252,7 +252,10 @@ def cache_reserve(table, lens, refs, seqs, tokens: int, page_size: int):
     """Grows the slots seqs [n] int32 by `tokens` keys each: lens += tokens, with the free pages that takes
     (lowest first, in the order of seqs).  table [slots, width], lens [slots] and refs [pages] are int32 and
     changed in place.  Returns granted [n] int32: 0 for a request that got nothing (the row or the pool is
-    full, or the slot is out of range or listed again)."""
+    full, or the slot is out of range or listed again).
+
+    To drop a slot's newest keys (drafts that were rejected), lower its lens, though not into pages that other slots
+    share: the pages past it stay in its row, where its next reserve uses them first."""
     fn = "kb_cache_reserve"
     granted = _host.reserve(table, lens, refs, seqs, tokens, page_size)
     if granted is not None:
