@@ -13,7 +13,7 @@ needs beside the norms, products and softmax of `kbb200.ops`.
 Tensors are fp32, fp16 or bf16 on one CUDA device.  Every function checks its
 tensors, allocates outputs and scratch through torch's caching allocator and
 launches on torch's current stream; it never waits for the GPU.  A C-ABI error
-raises KbError.
+raises KbError.  Outputs take no part in autograd, whatever the inputs require.
 
 Decoding makes these calls once per layer and token, so the way of right
 arguments is native (csrc/lm_host.cpp): it checks them, allocates and calls the
