@@ -21,8 +21,9 @@
 // lm_attention_tc.cu (16-bit) and lm_attention_tc32.cu (fp32) cannot take the
 // prefix or do not pay; plan_part() chooses.  bf16, 32 query and 8 key heads x
 // 128, on a B200: 64 samples of an 8192-token prompt with up to 1000 keys of
-// their own 64 us (own keys alone 41), 256 samples of 32768 tokens with up to
-// 700 of their own 233 us (own keys 72, at 5.1 TB/s).
+// their own 64 us (own keys alone 39), 256 samples of 32768 tokens with up to
+// 700 of their own 227 us where L2 holds what the call before left (own keys 71,
+// at 5.1 TB/s) and 260 where all inputs come from HBM.
 //
 // Keys at or past what a row tile sees are not read (they count as zeros), so
 // what stands in unused slots of a page does not matter; infinite and NaN values

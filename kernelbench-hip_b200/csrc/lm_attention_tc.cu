@@ -5,8 +5,13 @@
 // A CTA takes up to two tiles of 128 query rows and a range of keys, in tiles
 // of 128.  Per key tile j and row tile t:
 //   S_t = Q_t K_j^T            tcgen05.mma, 128 x 128, accumulators in TMEM
-//   P_t = exp2(S_t c - m)      one thread per row (tcgen05.ld), rounded to 16
-//                              bits into TMEM over S_t (tcgen05.st)
+//   P_t = exp2(S_t c - m)      one thread per row (tcgen05.ld), rounded to the
+//                              values' 16 bits into TMEM over S_t (tcgen05.st):
+//                              a product has operands of one type, and two
+//                              halves of P would take two products.  Each
+//                              weight is off by half a unit, out by that much
+//                              of softmax |v|: bf16 0.0022 against 0.0017 of
+//                              an output that is only rounded once
 //   O_t += P_t V_j             tcgen05.mma with P from TMEM, O in TMEM
 // c = scale log2(e).  m is a row's reference, not its exact maximum: it only
 // moves when the maximum has grown past it by more than 2^kSlack, and then the
@@ -33,12 +38,13 @@
 //
 // Bound: 4 rows keys dim operations on the tensor cores, and as many cycles
 // again of exponentials (16 per clock and SM against 128 x 128 x 128 products
-// in 512 cycles), which overlap.  What it measured: per key tile and row tile a
-// softmax takes 2400 cycles (85 for the load, 320 for the maximum, 1800 for the
-// exponentials, 170 for the store), O 520, S 820 (both operands from shared
-// memory: 8 KB per 64 cycles of product), and this chain, not a unit, sets the
-// pace.  256 samples x 32 heads x 128 over 32768 keys, bf16: 0.16 ms,
-// 850 TFLOP/s, 52 % of a large library product's 1650.  Tried and slower: steps
+// in 512 cycles), which overlap.  What it measured, by clocks read in a copy of
+// this kernel: per key tile and row tile a softmax takes 2400 cycles (85 for the
+// load, 320 for the maximum, 1800 for the exponentials, 170 for the store), O 520,
+// S 820 (both operands from shared memory: 8 KB per 64 cycles of product), and
+// this chain, not a unit, sets the pace.  256 samples x 32 heads x 128 over 32768
+// keys, bf16: 0.167 ms from a cold cache, 820 TFLOP/s, half of a large library
+// product's 1650.  Tried and slower: steps
 // of 64 keys with two buffers for S (a product of 128 x 64 takes as long as one
 // of 128 x 128), two threads per row (spills at 96 registers).
 //

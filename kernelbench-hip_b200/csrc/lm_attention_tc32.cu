@@ -518,7 +518,8 @@ int launch_as(const SplitArgs& s, cudaStream_t stream) {
 // Where the split pays, by the operations: against the kernel of mma.sync it
 // took 74 against 65 us at 1.07e9 (256 rows x 8 heads x 1024 keys x 128), 66
 // against 87 at 2.1e9, 162 against 267 at 8.6e9, 245 against 494 at 17e9 and 952
-// against 3394 at 131e9 (calls with short continuations).
+// against 3394 at 131e9 (calls with short continuations).  With magnitudes by row
+// and head it takes 64, 136 and 191 us at the three in the middle, 739 at 137e9.
 bool tc32_pays(int64_t rows, int64_t heads_kv, int64_t dim, int64_t keys) {
   return dim <= kTile && heads_kv <= 65535 && rows > 64 && keys > 0 && 4.0 * rows * heads_kv * dim * keys >= 1.2e9;
 }

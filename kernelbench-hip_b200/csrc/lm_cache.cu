@@ -29,7 +29,8 @@
 // us for 134 MB written, the parent's page from L2).  Each launch starts while
 // the one before ends.  A fork of few table entries is two launches, the plan's
 // CTA writing the rows as well (4 children of 63 pages, with the reserve and the
-// append that follow: 12.4 against 14.4 us; 32 of 101 pages: 16.4 against 14.4).
+// append that follow, in a graph: 12.4 against 14.4 us in three, 10.3 by now; 32 of
+// 101 pages: 16.4 against 14.4, 14.5 by now).
 // Else rows of children that share their pages meet in refs: a thread takes one
 // column of 16 rows and adds a page's changes up before its atomic.
 #include "lm_common.cuh"
