@@ -182,7 +182,8 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix, table, lens, scale: flo
     query t sees the keys below lens - queries + t + 1.  scale: dim ** -0.5 unless given.
 
     Returns (out, lse): out like q, contiguous, and lse [batch, queries, heads_q] fp32, the logarithm of the sum
-    of the exponentials; a query without keys (a slot whose lens is 0) gets zeros and -inf."""
+    of the exponentials; a query without keys (a slot whose lens is 0) gets zeros and -inf.  What stands in slots that
+    no query sees does not matter, and infinite or NaN keys and values reach the queries that see them only."""
     fn = "kb_shared_prefix_attention"
     if out is None:
         made = _host.attention(q, k_pages, v_pages, prefix, table, lens, scale)
