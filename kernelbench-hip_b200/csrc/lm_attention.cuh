@@ -180,10 +180,12 @@ __device__ __forceinline__ void write_nonfinite(const AttnArgs& a, const Item& w
       if (!isfinite(x)) sum += x;
     }
     if (isfinite(sum)) continue;
-    if (a.part_o)
-      a.part_o[((int64_t)w.split * n_rows + at) * a.dim + c] = sum;
-    else
-      static_cast<T*>(a.out)[at * a.dim + c] = from_f32<T>(sum);
+    if (a.part_o) {  // added to what is there: a row of NaN stays one
+      a.part_o[((int64_t)w.split * n_rows + at) * a.dim + c] += sum;
+    } else {
+      T* y = static_cast<T*>(a.out) + at * a.dim + c;
+      *y = from_f32<T>(to_f32(*y) + sum);
+    }
   }
 }
 

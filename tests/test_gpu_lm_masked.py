@@ -120,3 +120,29 @@ def test_values_beside_those_that_nobody_sees(shape, length, dt, what, cuda_devi
     page = shape[5]
     lens[:] = length
     check(args, [(int(prefix[key // page]), key % page, key, None) for key in (length - 1, length, length + 1, length // 2)], what)
+
+
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("shape", [(2, 3, 2, 1, 64, 16, 0, 40), (1, 90, 2, 1, 128, 16, 0, 100), (200, 1, 2, 1, 128, 16, 30, 0)])
+def test_a_query_of_nan_stays_so(shape, dt, cuda_device):
+    """The newest query of a sequence is NaN, and it alone sees values that are infinite."""
+    from kbb200 import lm
+
+    q, k, v, prefix, table, lens = args = attention_inputs(cuda_device, dt, *shape, seed=sum(shape))
+    page = shape[5]
+    if shape[1] > 1:
+        lens.clamp_(min=shape[1])
+        last = int(lens[0]) - 1
+        page_id = int(table[0, last // page])
+    else:  # one query a sequence: all others end a key earlier
+        last = prefix.numel() * page - 1
+        lens[:], page_id = last, int(prefix[-1])
+        lens[0] = last + 1
+    want, want_lse = lm.shared_prefix_attention(*args)
+    q[0, -1] = NAN
+    v[page_id, last % page] = INF
+    out, lse = lm.shared_prefix_attention(*args)
+    assert torch.isnan(out[0, -1]).all() and torch.isnan(lse[0, -1]).all()
+    others = torch.ones(out.shape[:2], dtype=torch.bool, device=cuda_device)
+    others[0, -1] = False
+    assert torch.equal(out[others], want[others]) and torch.equal(lse[others], want_lse[others])
